@@ -213,6 +213,44 @@ int lq_dequant(const lq_dims* d, void* ssm, const void* Kbuf, const void* Ubuf, 
 int lq_lowrank(const float* x, const float* Q0, float* U, float* Q, int32_t n, int32_t K, int32_t V, int32_t r,
                int32_t iters, void* stream);
 
+/* ---- the operators around the decode step (no counterpart in the reference, which leaves them to the engine) ----
+ *
+ * Gated delta rule of packed sequences on the fp32 states of their slots: what an engine runs between lq_dequant and lq_quantize.
+ * Of d only NS, HV, H, K, V and SS are read; ssm holds fp32 states here, not checkpoints.  Sequence n owns the rows
+ * cu[n] .. cu[n+1] - 1 of the T rows and the state of slot idx[n]; per value head, with key head hv / (HV / H):
+ *     g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b), q^ = scale q / sqrt(|q|^2 + 1e-6), k^ = k / sqrt(|k|^2 + 1e-6)
+ *     S <- e^g S;  u = beta (v - S k^);  S <- S + u k^T;  o = S q^                    (fp32; o rounded to bf16 once)
+ *   - mixed bf16 rows q | k | v (2 H K + HV V elements, row stride mixed_stride, a multiple of 8); a, b bf16 [T, HV] with row strides;
+ *     A_log, dt_bias f32 [HV]; cu i32 [N + 1], ascending; idx i32 [N]; o bf16 [T, HV, V] contiguous.  scale <= 0 selects K^-1/2.
+ *   - has_initial (u8 [N], may be NULL = all): 0 starts the sequence from a zero state instead of its slot's.
+ *   - A sequence without tokens touches nothing.  idx[n] <= 0 or >= NS, or a slot that an earlier entry names too: padding, the
+ *     sequence's rows of o are zeros and no state is touched.  Rows of o that no sequence owns are left as they are.  Offsets
+ *     outside 0 .. T are cut to it. */
+int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
+                   const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
+                   const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale, void* stream);
+/* The same rule for one token per row (row n is sequence n, and continues its state): the decode of states kept in fp32. */
+int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
+                     const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* idx, void* o,
+                     int32_t N, float scale, void* stream);
+/* Causal conv1d + SiLU of packed prompts: per sequence and channel, with the inputs before the sequence's first token from its slot
+ * (zeros where has_initial[n] is 0),  out[t] = silu(bias + sum_j weight[j] in[t - 3 + j])  in fp32, rounded once; the slot's state
+ * becomes the last three inputs.  conv: the operands of lq_causal_conv1d_update, x with T rows; cu, idx, has_initial as above;
+ * out bf16 [T, out_stride], not overlapping x.  Sequences without tokens or with a padding slot are skipped (nothing read or
+ * written).  channels must be a multiple of 8 and bias 16-byte aligned. */
+int lq_causal_conv1d_prompt(const lq_conv1d* conv, const int32_t* cu, const int32_t* idx, const uint8_t* has_initial, int32_t N,
+                            int64_t T, int32_t channels, int32_t NS, void* out, int64_t out_stride, void* stream);
+/* Gated RMS norm of the rule's output: y = o / sqrt(mean(o^2) + eps) * weight * silu(z) over every head's V = 128 values, in fp32,
+ * rounded once.  o, y bf16 [T, HV, V] contiguous (y may be o); z bf16 [T, HV * V] with row stride z_stride; weight bf16 [V]. */
+int lq_gated_norm(const void* o, const void* z, int64_t z_stride, const void* weight, void* y, int64_t T, int32_t HV, int32_t V,
+                  float eps, void* stream);
+/* Residual and RMS norm: h = residual + scale x (fp32);  residual <- bf16(h);  y = h / sqrt(mean(h^2) + eps) * weight.
+ * All bf16 [T, D] with row strides in elements (multiples of 8); weight bf16 [D]; D a multiple of 8 up to LQ_NORM_MAX_DIM.
+ * y may be x, not residual. */
+#define LQ_NORM_MAX_DIM 16384
+int lq_add_norm(const void* x, int64_t x_stride, void* residual, int64_t r_stride, const void* weight, void* y, int64_t y_stride,
+                int64_t T, int32_t D, float scale, float eps, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

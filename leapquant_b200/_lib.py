@@ -15,7 +15,8 @@ LIB_PATH = os.environ.get("LEAPQUANT_B200_LIB") or os.path.join(_HERE, "libleapq
 EXPORTS = ("lq_version", "lq_strerror", "lq_last_cuda_error", "lq_device_status", "lq_set_option", "lq_gdn_step", "lq_kda_step",
            "lq_flush", "lq_gdn_decode", "lq_kda_decode", "lq_gdn_decode_conv", "lq_kda_decode_conv", "lq_causal_conv1d_update",
            "lq_decode_work_bytes", "lq_gdn_decode_noalloc",
-           "lq_quantize", "lq_dequant", "lq_lowrank")
+           "lq_quantize", "lq_dequant", "lq_lowrank", "lq_gdn_prefill", "lq_gdn_recurrent", "lq_causal_conv1d_prompt",
+           "lq_gated_norm", "lq_add_norm")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -72,9 +73,15 @@ def lib():
         L.lq_quantize.argtypes = [D, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _P]
         L.lq_dequant.argtypes = [D, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]
         L.lq_lowrank.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]
+        L.lq_gdn_prefill.argtypes = [D, _P, _P, I64, _P, I64, _P, I64, _P, _P, _P, _P, _P, _P, _I, I64, _F, _P]
+        L.lq_gdn_recurrent.argtypes = [D, _P, _P, I64, _P, I64, _P, I64, _P, _P, _P, _P, _I, _F, _P]
+        L.lq_causal_conv1d_prompt.argtypes = [C, _P, _P, _P, _I, I64, _I, _I, _P, I64, _P]
+        L.lq_gated_norm.argtypes = [_P, _P, I64, _P, _P, I64, _I, _I, _F, _P]
+        L.lq_add_norm.argtypes = [_P, I64, _P, I64, _P, _P, I64, I64, _I, _F, _F, _P]
         for name in ("lq_device_status", "lq_gdn_step", "lq_kda_step", "lq_flush", "lq_quantize", "lq_dequant", "lq_lowrank",
                      "lq_gdn_decode", "lq_kda_decode", "lq_gdn_decode_conv", "lq_kda_decode_conv", "lq_causal_conv1d_update",
-                     "lq_gdn_decode_noalloc"):
+                     "lq_gdn_decode_noalloc", "lq_gdn_prefill", "lq_gdn_recurrent", "lq_causal_conv1d_prompt", "lq_gated_norm",
+                     "lq_add_norm"):
             getattr(L, name).restype = _I
         _lib = L
     return _lib
@@ -104,6 +111,36 @@ def conv1d(x, conv_state, weight, bias):
         raise LeapQuantError(f"conv state must be (slot, channel, width - 1), got {tuple(conv_state.shape)}")
     return LqConv1d(ptr(x), x.stride(0), ptr(conv_state), conv_state.stride(0), conv_state.stride(1), conv_state.stride(2),
                     ptr(weight), ptr(bias) if bias is not None else None, int(weight.shape[1]))
+
+
+def same_device(t, *others):
+    """Refuses host tensors, and tensors on different devices."""
+    if not t.is_cuda:
+        not_cuda()
+    for x in others:
+        if x is not None and x.device != t.device:
+            if not x.is_cuda:
+                not_cuda()
+            raise LeapQuantError(f"tensors on different devices: {t.device} and {x.device}")
+
+
+def rows(t, dtype, shape, what):
+    """Element stride between the rows of `t` (first dimension), whose other dimensions have to be packed; refuses another type or
+    shape."""
+    if t.dtype != dtype or tuple(t.shape) != shape:
+        raise LeapQuantError(f"{what}: expected {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
+    n = 1
+    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+        if size > 1 and stride != n:
+            raise LeapQuantError(f"{what}: the elements of a row must be contiguous, got strides {t.stride()}")
+        n *= size
+    return t.stride(0) if t.shape[0] > 1 else max(n, 1)
+
+
+def whole(t, dtype, shape, what):
+    """Refuses a tensor that is not contiguous with this type and shape."""
+    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
+        raise LeapQuantError(f"{what}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
 
 
 def ptr(t):

@@ -4,3 +4,5 @@
 #include "lq_quant.cu"
 #include "lq_flush.cu"
 #include "lq_step.cu"
+#include "lq_rule.cu"
+#include "lq_rows.cu"

@@ -122,6 +122,14 @@ __device__ __forceinline__ void named_bar(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// Whether entry n of idx is the first with its slot (the whole warp asks).  Two sequences cannot both own a state: a later entry
+// with the same slot is treated as padding.
+__device__ __forceinline__ bool first_of_slot(const int32_t* idx, int n, int slot, int lane) {
+    bool dup = false;
+    for (int i = lane; i < n; i += 32) dup |= idx[i] == slot;
+    return !__any_sync(0xffffffffu, dup);
+}
+
 // ---- global loads that bypass L1 allocation (streamed once) ----
 __device__ __forceinline__ uint4 ldg_stream(const void* p) {
     uint4 r;
@@ -208,9 +216,9 @@ static std::atomic<int> g_pdl{1};       // set by lq_set_option from any thread,
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... KArgs, typename... Args>
-inline cudaError_t launch_dependent(void (*kern)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
+inline cudaError_t launch_dependent(void (*kern)(KArgs...), dim3 grid, unsigned block, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;

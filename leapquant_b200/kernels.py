@@ -8,6 +8,12 @@ leapquant/kernels.py, backed by hand-written sm_100a CUDA behind a C ABI (includ
   make_quantize    fp32 -> 8-bit in place     (reference leapquant/kernels.py:2127, launch signature :2136-2142)
   make_lowrank / lowrank_factor               (reference leapquant/kernels.py:2247, :2321)
 
+The operators around them, which the reference leaves to the engine, have no counterpart there:
+
+  make_gdn_prefill     gated delta rule of packed sequences on fp32 states     make_gdn_recurrent   one token per row of the same
+  make_conv1d_prompt   causal conv1d + SiLU of packed prompts                  make_conv1d_update   one token per row of the same
+  make_gated_norm      RMS norm of every head's output, times silu(gate)       make_add_norm        residual + RMS norm
+
 Each factory returns a callable that takes the same tensors in the same order as the reference's compiled kernel.
 The several aliasing views of the state tensor the reference passes (Sq, Sk, Sv, Skv, UQ, Sq16) all point into one
 fp32 tensor; the callable takes the base address from the first of them and the slot stride SS from the factory.
@@ -231,6 +237,139 @@ def make_lowrank(K, V, R, ITERS, threads=128):
         _launch(fn, "lq_lowrank", S, p(S), p(Q0), p(U), p(Q), int(S.shape[0]), K, V, R, iters)
 
     return lowrank
+
+
+def _rule_operands(who, dims, S0, mixed, a, b, A_log, dt_bias, idx, o):
+    """Checks the tensors that both forms of the gated delta rule take; returns the row strides of mixed, a and b."""
+    NS, HV, H, K, V, SS = dims
+    T = mixed.shape[0]
+    _lib.same_device(S0, mixed, a, b, A_log, dt_bias, idx, o)
+    if S0.dtype != torch.float32 or tuple(S0.shape) != (NS, HV, V, K) or S0.stride() != (SS, V * K, K, 1):
+        raise _lib.LeapQuantError(f"{who}: expected float32 states {(NS, HV, V, K)} with strides {(SS, V * K, K, 1)}, got {S0.dtype} "
+                                  f"{tuple(S0.shape)}, strides {S0.stride()}")
+    _lib.whole(o, torch.bfloat16, (T, HV, V), f"{who}, outputs")
+    _lib.whole(A_log, torch.float32, (HV,), f"{who}, A_log")
+    _lib.whole(dt_bias, torch.float32, (HV,), f"{who}, dt_bias")
+    return (_lib.rows(mixed, torch.bfloat16, (T, 2 * H * K + HV * V), f"{who}, q | k | v rows"),
+            _lib.rows(a, torch.bfloat16, (T, HV), f"{who}, a"), _lib.rows(b, torch.bfloat16, (T, HV), f"{who}, b"))
+
+
+def _sequences(who, cu, idx, has_initial):
+    """Checks the tensors that describe packed sequences; returns their number and the address of has_initial (or None)."""
+    N = idx.shape[0]
+    _lib.whole(idx, torch.int32, (N,), f"{who}, slots")
+    _lib.whole(cu, torch.int32, (N + 1,), f"{who}, offsets of the sequences")
+    if has_initial is None:
+        return N, None
+    if has_initial.dtype not in (torch.bool, torch.uint8) or tuple(has_initial.shape) != (N,) or not has_initial.is_contiguous():
+        raise _lib.LeapQuantError(f"{who}, has_initial: expected contiguous bool ({N},), got {has_initial.dtype} {tuple(has_initial.shape)}")
+    return N, has_initial.data_ptr()
+
+
+def make_gdn_prefill(NS, HV, H, K, V, SS, scale=None):
+    """Gated delta rule of packed sequences on the fp32 states of their slots.  Returns
+    prefill(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o): S0 f32 [NS, HV, V, K] with slot stride SS, updated in place;
+    mixed bf16 [T, 2HK + HV V] and a, b bf16 [T, HV] (row strides free); A_log, dt_bias f32 [HV]; cu i32 [N + 1], the first row of
+    every sequence and the end of the last; idx i32 [N], their slots; has_initial bool [N] or None (all): False starts from a zero
+    state; o bf16 [T, HV, V].  A sequence without tokens touches nothing; one with idx <= 0, idx >= NS or a slot that an earlier
+    one names gets zeros in o and touches no state; rows of o that no sequence owns are left as they are."""
+    _need_128(K, V, "make_gdn_prefill")
+    dims, d = (NS, HV, H, K, V, SS), _lib.dims(NS, HV, H, K, V, 0, 0, SS)
+    sc = float(K ** -0.5 if scale is None else scale)
+    fn = _lib.lib().lq_gdn_prefill
+
+    def prefill(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
+        ms, as_, bs = _rule_operands("gdn prefill", dims, S0, mixed, a, b, A_log, dt_bias, idx, o)
+        _lib.same_device(S0, cu, has_initial)
+        N, hp = _sequences("gdn prefill", cu, idx, has_initial)
+        _launch(fn, "lq_gdn_prefill", S0, d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
+                dt_bias.data_ptr(), cu.data_ptr(), idx.data_ptr(), hp, o.data_ptr(), N, mixed.shape[0], sc)
+
+    return prefill
+
+
+def make_gdn_recurrent(NS, HV, H, K, V, SS, scale=None):
+    """Gated delta rule for one token per row on fp32 states.  Returns recurrent(S0, mixed, a, b, A_log, dt_bias, idx, o), the operands
+    of make_gdn_prefill with T = N rows; rows with idx <= 0, idx >= NS or the slot of an earlier row write zeros and touch no state."""
+    _need_128(K, V, "make_gdn_recurrent")
+    dims, d = (NS, HV, H, K, V, SS), _lib.dims(NS, HV, H, K, V, 0, 0, SS)
+    sc = float(K ** -0.5 if scale is None else scale)
+    fn = _lib.lib().lq_gdn_recurrent
+
+    def recurrent(S0, mixed, a, b, A_log, dt_bias, idx, o):
+        ms, as_, bs = _rule_operands("gdn recurrent", dims, S0, mixed, a, b, A_log, dt_bias, idx, o)
+        _lib.whole(idx, torch.int32, (mixed.shape[0],), "gdn recurrent, slots")
+        _launch(fn, "lq_gdn_recurrent", S0, d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
+                dt_bias.data_ptr(), idx.data_ptr(), o.data_ptr(), mixed.shape[0], sc)
+
+    return recurrent
+
+
+def make_conv1d_prompt(NS, channels):
+    """Causal conv1d (width 4) + SiLU of packed prompts.  Returns prompt(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out):
+    x bf16 [T, >= channels], conv_state, conv_weight, conv_bias as for make_conv1d_update, cu, idx, has_initial as for
+    make_gdn_prefill, out bf16 [T, channels] (not overlapping x).  conv_state receives the last three inputs of every sequence.
+    The sums are fp32 and rounded once, without the update's rounding of every tap's product.  Sequences without tokens, and those
+    with idx <= 0, idx >= NS or the slot of an earlier one, are skipped (nothing read or written)."""
+    fn = _lib.lib().lq_causal_conv1d_prompt
+
+    def prompt(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out):
+        _lib.same_device(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out)
+        N, hp = _sequences("conv1d prompt", cu, idx, has_initial)
+        if x.dim() != 2 or x.shape[1] < channels or tuple(conv_weight.shape) != (channels, 4) or conv_state.shape[:2] != (NS, channels) or (
+                conv_bias is not None and tuple(conv_bias.shape) != (channels,)):
+            raise _lib.LeapQuantError(f"conv1d prompt: x {tuple(x.shape)}, state {tuple(conv_state.shape)}, weight {tuple(conv_weight.shape)} "
+                                      f"do not fit {NS} slots of {channels} channels")
+        cv = _lib.conv1d(x, conv_state, conv_weight, conv_bias)
+        if x.shape[0] == 1:
+            cv.x_stride = -(-x.shape[1] // 8) * 8
+        os_ = _lib.rows(out, torch.bfloat16, (x.shape[0], channels), "conv1d prompt, outputs")
+        _launch(fn, "lq_causal_conv1d_prompt", x, cv, cu.data_ptr(), idx.data_ptr(), hp, N, x.shape[0], int(channels), int(NS),
+                out.data_ptr(), os_)
+
+    return prompt
+
+
+def make_gated_norm(V, eps=1e-6):
+    """Gated RMS norm of every head's output.  Returns norm(o, z, weight, y): y = o / sqrt(mean(o^2) + eps) * weight * silu(z) over the
+    V values of a head; o, y bf16 [T, HV, V] (y may be o), z bf16 [T, HV * V] (row stride free), weight bf16 [V]."""
+    if V != 128:
+        raise NotImplementedError(f"make_gated_norm: V = {V}; this build implements heads of 128 only")
+    eps = float(eps)
+    fn = _lib.lib().lq_gated_norm
+
+    def norm(o, z, weight, y):
+        _lib.same_device(o, z, weight, y)
+        if o.dim() != 3:
+            raise _lib.LeapQuantError(f"gated norm: the outputs are [rows, heads, {V}], got {tuple(o.shape)}")
+        T, HV = o.shape[:2]
+        _lib.whole(o, torch.bfloat16, (T, HV, V), "gated norm, o")
+        _lib.whole(y, torch.bfloat16, (T, HV, V), "gated norm, y")
+        _lib.whole(weight, torch.bfloat16, (V,), "gated norm, weight")
+        zs = _lib.rows(z, torch.bfloat16, (T, HV * V), "gated norm, z")
+        _launch(fn, "lq_gated_norm", o, o.data_ptr(), z.data_ptr(), zs, weight.data_ptr(), y.data_ptr(), T, HV, V, eps)
+
+    return norm
+
+
+def make_add_norm(D, eps=1e-6, scale=1.0):
+    """Residual stream and the norm that the next block reads.  Returns norm(x, residual, weight, y): residual <- residual + scale x;
+    y = residual / sqrt(mean(residual^2) + eps) * weight, of the fp32 sum.  x, residual, y bf16 [T, D] (row strides free; y may be
+    x), weight bf16 [D]."""
+    if D < 8 or D % 8 or D > 16384:
+        raise NotImplementedError(f"make_add_norm: D = {D}; a multiple of 8 up to 16384 is supported")
+    eps, scale = float(eps), float(scale)
+    fn = _lib.lib().lq_add_norm
+
+    def norm(x, residual, weight, y):
+        _lib.same_device(x, residual, weight, y)
+        T = x.shape[0]
+        strides = [_lib.rows(t, torch.bfloat16, (T, D), f"add norm, {n}") for t, n in ((x, "x"), (residual, "residual"), (y, "y"))]
+        _lib.whole(weight, torch.bfloat16, (D,), "add norm, weight")
+        _launch(fn, "lq_add_norm", x, x.data_ptr(), strides[0], residual.data_ptr(), strides[1], weight.data_ptr(), y.data_ptr(),
+                strides[2], T, D, scale, eps)
+
+    return norm
 
 
 _mk_lowrank = functools.lru_cache(maxsize=None)(make_lowrank)

@@ -105,6 +105,10 @@ class LeapQuantState:
         self.work = torch.zeros(KN.decode_work_ints(NS, HV), dtype=torch.int32, device=dev)
         self.kdeq = KN.make_dequant(NS, HV, K, V, L, SS, buf_dtype=KN.BF16, R=R, kda=kda)
         self.kquant = KN.make_quantize(NS, HV, K, V, L, SS, R=R, ITERS=3 if kda else 1, kda=kda)
+        # the fp32 states between dequantize() and quantize(), or kept in fp32 altogether (Gated DeltaNet)
+        self.kprefill = None if kda else KN.make_gdn_prefill(NS, HV, H, K, V, SS)
+        self.kdense = None if kda else KN.make_gdn_recurrent(NS, HV, H, K, V, SS)
+        self._kconv_prompt = None
         self._vkey = None
         self._v = None
         self._f32 = {}
@@ -190,6 +194,42 @@ class LeapQuantState:
         v = self.views(ssm)
         bufs = (self.Kbuf, self.Ubuf, self.Wbuf, self.Pbuf) + ((self.Gbuf,) if self.kda else ()) + (self.hcnt,)
         self.kdecode_conv(v["q32"], *bufs, x, conv_state, conv_weight, conv_bias, a, b, A_log, dt_bias, self.Q0, idx, out, self.work)
+
+    def _need_gdn(self, who):
+        if self.kda:
+            raise NotImplementedError(f"{who}: the fp32 states of Gated DeltaNet layers only (no gate per key channel)")
+
+    def prefill(self, ssm, mixed, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial=None):
+        """Many tokens of packed sequences through the gated delta rule, on the fp32 states of their slots: between dequantize() and
+        quantize(), in place of the engine's own kernel.
+
+        mixed bf16 [T, 2HK + HV*V], a, b bf16 [T, HV] (row strides free); sequence n owns the rows cu_seqlens[n] .. cu_seqlens[n + 1] - 1
+        and slot idx[n]; has_initial bool [N] or None: False starts it from a zero state; out bf16 [T, HV, V] written in place.
+        Gated DeltaNet only.  No host synchronisation, no allocation when the dtypes match."""
+        self._need_gdn("prefill")
+        self.kprefill(ssm, mixed, a, b, A_log if A_log.dtype == torch.float32 else self._p32(A_log),
+                      dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), cu_seqlens.to(torch.int32), idx.to(torch.int32),
+                      has_initial, out)
+
+    def prefill_conv(self, ssm, x, conv_state, conv_weight, conv_bias, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial=None):
+        """prefill() from the raw q | k | v projections x: the causal conv1d of the prompts first (operands as for decode_conv; the
+        conv state of every sequence is advanced, or starts at zero where has_initial is False).  The T activated rows are
+        allocated from torch's allocator for the call."""
+        self._need_gdn("prefill_conv")
+        C = 2 * self.H * self.K + self.HV * self.V
+        if self._kconv_prompt is None:
+            self._kconv_prompt = KN.make_conv1d_prompt(self.NS, C)
+        mixed = torch.empty(x.shape[0], C, dtype=torch.bfloat16, device=x.device)
+        idx, cu_seqlens = idx.to(torch.int32), cu_seqlens.to(torch.int32)
+        self._kconv_prompt(x, conv_state, conv_weight, conv_bias, cu_seqlens, idx, has_initial, mixed)
+        self.prefill(ssm, mixed, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial)
+
+    def decode_dense(self, ssm, mixed, a, b, A_log, dt_bias, idx, out):
+        """decode() on fp32 states: one token per row on slots that hold a state and no checkpoint (a sequence that stays in fp32, or
+        the other side of a comparison).  Operands as for decode(), a and b with free row strides.  Gated DeltaNet only."""
+        self._need_gdn("decode_dense")
+        self.kdense(ssm, mixed, a, b, A_log if A_log.dtype == torch.float32 else self._p32(A_log),
+                    dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), idx.to(torch.int32), out)
 
     def dequantize(self, ssm, idx):
         """Materialize the fp32 state of the slots idx in place (before the engine's own prefill kernel runs on them)."""
