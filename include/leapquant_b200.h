@@ -67,6 +67,7 @@ int lq_device_status(int* status);
  * (row, head) in registers (GDN only; KDA keeps the default).  1 and 2 exist for debugging and comparison.
  * "pdl": 1 (default) launches the step and flush kernels with programmatic stream serialisation, so that the launch and
  * set-up of one overlap the tail of its predecessor on the stream; 0 = plain launches.
+ * "rule_impl": how lq_gdn_prefill works: 0 = by the mean length of the sequences (default), 1 = token by token, 2 = in chunks.
  * "work_list_min_programs": the fewest (row, head) programs of a fused decode call for which the `work` list passed to it
  * is used (-1 = default, sixteen per SM; 0 = whenever `work` is given).  The mailboxes cost an atomic round trip or two
  * per launch and save the flush of one head when the due heads sit unevenly on the CTAs. */

@@ -5,4 +5,5 @@
 #include "lq_flush.cu"
 #include "lq_step.cu"
 #include "lq_rule.cu"
+#include "lq_chunk.cu"
 #include "lq_rows.cu"

@@ -213,6 +213,7 @@ void set_last_cuda_error(cudaError_t e);
 // (shared-memory carve, barrier initialisation) and then blocks in pdl_wait() until the predecessor has completed and its
 // writes are visible.  Every kernel launched this way calls pdl_trigger() and pdl_wait() before it touches global memory.
 static std::atomic<int> g_pdl{1};       // set by lq_set_option from any thread, read by every launch
+static std::atomic<int> g_rule_impl{0};  // likewise: 0 = by length, 1 = token by token, 2 = in chunks
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <typename... KArgs, typename... Args>

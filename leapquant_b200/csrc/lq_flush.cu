@@ -17,6 +17,7 @@
 // heads are left and ONE team of 16 warps for a last single head -- the common case of a serving batch whose sequences
 // fill their windows at different steps, where the latency of one flush is what the step pays.
 #include "lq_linalg.cuh"
+#include "lq_tc.cuh"
 
 namespace lq {
 
@@ -91,48 +92,7 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 }
 __device__ __forceinline__ float2 unpack_h2(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
 
-// ---- fifth-generation tensor cores: tensor memory, instruction and operand descriptors ----
-// Tensor memory is allocated by one whole warp (a power of two >= 32 of columns; the address lands in shared memory) and
-// must be freed by a whole warp before the CTA exits.
-__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(ncols) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// D[tmem] (+)= A[smem] B[smem]: one instruction of M = 128, N = 128, K = 16, issued by ONE thread
-__device__ __forceinline__ void umma_bf16_ss(uint32_t d_tmem, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t"
-        "}\n" ::"r"(d_tmem),
-        "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
-        : "memory");
-}
-// arrives on the mbarrier once every tensor-core instruction this thread has issued so far is complete
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// 32 consecutive fp32 columns of this thread's lane of tensor memory (lane = 32 (warp % 4) + lane id)
-__device__ __forceinline__ void tmem_ld_32cols(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-
+// ---- operand descriptors of the rebuild ----
 // Instruction descriptor: fp32 accumulator, bf16 A and B, both operands "MN-major" (the M / N index is the contiguous one in
 // shared memory, because the window rows are stored [j][128]), N = 128, M = 128.
 constexpr uint32_t UMMA_IDESC = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -610,8 +570,8 @@ __device__ __forceinline__ bool flush_head(const FlushSmem& s, const FlushArgs& 
         const uint64_t db0 = umma_desc(KDA ? s.tile[1] : s.tile[2], Lp), db1 = umma_desc(s.tile[2], Lp);
         const int nk = Lp >> 4;
         // one K step = 16 rows j = two swizzle atoms of eight rows = 2 048 bytes = 128 units of the descriptor's address field
-        for (int ks = 0; ks < nk; ++ks) umma_bf16_ss(tm, da0 + uint64_t(ks) * 128u, db0 + uint64_t(ks) * 128u, UMMA_IDESC, ks > 0);
-        for (int ks = 0; ks < nk; ++ks) umma_bf16_ss(tm, da1 + uint64_t(ks) * 128u, db1 + uint64_t(ks) * 128u, UMMA_IDESC, 1u);
+        for (int ks = 0; ks < nk; ++ks) umma_ss(tm, da0 + uint64_t(ks) * 128u, db0 + uint64_t(ks) * 128u, UMMA_IDESC, ks > 0);
+        for (int ks = 0; ks < nk; ++ks) umma_ss(tm, da1 + uint64_t(ks) * 128u, db1 + uint64_t(ks) * 128u, UMMA_IDESC, 1u);
         umma_commit(s.mbar);
         const uint32_t ph = uint32_t(s.flags[0]);
         bool ok = false;

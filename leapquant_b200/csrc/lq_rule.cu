@@ -158,59 +158,4 @@ __global__ void __launch_bounds__(32 * RW_WARPS) rule_recurrent_kernel(RuleParam
         for (int j = 0; j < 4; ++j) __stcs(reinterpret_cast<float4*>(base + 4 * p * KD + 32 * j), s[p][j]);
 }
 
-static int rule_check(const lq_dims* d, const RuleParams& P) {
-    if (d->K != KD || d->V != VD) return LQ_ERR_UNSUPPORTED;
-    if (d->NS < 1 || d->HV < 1 || d->H < 1 || d->HV % d->H != 0 || d->SS < int64_t(d->HV) * d->V * d->K) return LQ_ERR_RANGE;
-    if (d->SS & 3) return LQ_ERR_ALIGN;
-    if (P.N < 0 || P.T < 0) return LQ_ERR_RANGE;
-    if (P.N == 0 || P.T == 0) return LQ_OK;
-    if (!P.ssm || !P.mixed || !P.a || !P.b || !P.A_log || !P.dt_bias || !P.idx || !P.o) return LQ_ERR_NULL;
-    if (P.mixed_stride < 2 * int64_t(d->H) * KD + int64_t(d->HV) * VD || P.a_stride < d->HV || P.b_stride < d->HV) return LQ_ERR_RANGE;
-    if ((P.mixed_stride & 7) || misaligned16({P.ssm, P.mixed, P.o})) return LQ_ERR_ALIGN;
-    if (int64_t(P.N) * d->HV > (int64_t(1) << 29)) return LQ_ERR_RANGE;            // programs: the grid's first dimension
-    return LQ_OK;
-}
-static int launch_recurrent(const RuleParams& P, cudaStream_t st) {
-    const unsigned grid = unsigned(P.N) * unsigned(P.HV) * (VD / (RW_ROWS * RW_WARPS));
-    const cudaError_t e = launch_dependent(rule_recurrent_kernel, grid, 32 * RW_WARPS, 0, st, P);
-    if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
-    return finish_launch();
-}
-static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
-                              const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
-                              const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale) {
-    RuleParams P;
-    P.ssm = ssm; P.SS = d->SS; P.mixed = (const uint16_t*)mixed; P.mixed_stride = mixed_stride; P.a = (const uint16_t*)a;
-    P.b = (const uint16_t*)b; P.a_stride = a_stride; P.b_stride = b_stride; P.A_log = A_log; P.dt_bias = dt_bias; P.cu = cu;
-    P.idx = idx; P.has_initial = has_initial; P.o = (uint16_t*)o; P.NS = d->NS; P.H = d->H; P.HV = d->HV; P.N = N; P.T = T;
-    P.scale = scale > 0.f ? scale : 1.0f / sqrtf(float(KD));
-    return P;
-}
-
 }  // namespace lq
-
-extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
-                              const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
-                              const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale,
-                              void* stream) {
-    using namespace lq;
-    if (!d) return LQ_ERR_NULL;
-    const RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
-                                     T, scale);
-    const int rc = rule_check(d, P);
-    if (rc || N == 0 || T == 0) return rc;
-    if (!cu) return LQ_ERR_NULL;
-    return launch_recurrent(P, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
-                                const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* idx, void* o,
-                                int32_t N, float scale, void* stream) {
-    using namespace lq;
-    if (!d) return LQ_ERR_NULL;
-    const RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, nullptr, idx, nullptr, o, N,
-                                     N, scale);
-    const int rc = rule_check(d, P);
-    if (rc || N == 0) return rc;
-    return launch_recurrent(P, static_cast<cudaStream_t>(stream));
-}

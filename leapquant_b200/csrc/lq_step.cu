@@ -1462,6 +1462,11 @@ extern "C" int lq_set_option(const char* name, int32_t value) {
         lq::g_work_list_min.store(value < 0 ? -1 : value, std::memory_order_relaxed);
         return LQ_OK;
     }
+    if (strcmp(name, "rule_impl") == 0) {
+        if (value < 0 || value > 2) return LQ_ERR_RANGE;
+        lq::g_rule_impl.store(value, std::memory_order_relaxed);
+        return LQ_OK;
+    }
     if (strcmp(name, "pdl") == 0) {
         lq::g_pdl.store(value != 0, std::memory_order_relaxed);
         return LQ_OK;
