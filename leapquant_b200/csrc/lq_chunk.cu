@@ -25,11 +25,16 @@ constexpr int RULE_SHORT = 8;                                // mean length from
 constexpr int CT = 64;                                       // tokens of a chunk
 // T and A lie within [-1, 1]; times 2^13 their small entries keep eleven bits down to 2^-27 as well
 constexpr float MAT_UP = 8192.f, MAT_DOWN = 1.f / 8192.f;
-constexpr int CK_MAIN = 256, CK_PREP = 128, CK_THREADS = CK_MAIN + CK_PREP;
+// two warpgroups of main warps and two of prep warps; the main warps hold the state and take registers over from the others:
+// 256 * 168 + 256 * 88 = 512 * 128 = 65 536
+constexpr int CK_MAIN = 256, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP;
+constexpr int CK_MAIN_REGS = 168, CK_PREP_REGS = 88;
 
-// tensor memory: 512 columns.  D takes the place of X | XQ once both have been read, AU that of Y.
+// tensor memory: 512 columns.  D takes the place of X | XQ once both have been read, AU that of Y, and the operand of A u that of the
+// state's heads once S q is through.  G: Gram matrix of the even and of the odd chunks.
 constexpr uint32_t TM_SHI = 0, TM_SLO = 64, TM_X = 128, TM_XQ = 192, TM_D = 128, TM_PHI = 256, TM_PLO = 288, TM_Y = 320, TM_AU = 320,
-                   TM_UOP = 384, TM_G = 448;
+                   TM_UOP = 0;
+__host__ __device__ constexpr uint32_t tm_gram(int buf) { return buf ? 384u : 448u; }
 
 // f16 operands, fp32 accumulator; B with the reduction contiguous (K-major) or, for S += u k^T, the 128 key columns (MN-major)
 __host__ __device__ constexpr uint32_t ck_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24); }
@@ -49,18 +54,21 @@ struct ChunkScalars {                                        // of one chunk, by
     float decay;                                             // e^{G_C}
     int len;                                                 // tokens of the chunk, 1 .. 64
 };
+struct PrepSmem {                                            // of one prep group
+    float L[CT][CT + 4];
+    float tdiag[4][16][16], t32[2][32][32], w[32][32];       // inverses of the diagonal blocks of 16 and 32; products on the way
+    float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
+    float kr[CT], qr[CT], ws[32], beta[CT];                  // ws: kr_s times the decay from s to token 31, for s < 32
+};
 struct ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
     unsigned char thi[2][8192], tlo[2][8192], amat[2][8192];
-    unsigned char raw[32768];                                // rows of k and q as they come: [128][128] bf16
-    float L[CT][CT + 4];
-    float tdiag[2][32][32], w[32][32];
+    uint16_t v[2][CT][VD];                                   // bf16 values; once they are used, the chunk's outputs on their way out
+    PrepSmem prep[2];
     ChunkScalars sc[2];
-    double G[CT];                                            // log2 of the decay from the chunk's start
-    float kr[CT], qr[CT], ws[CT], gate_beta[CT];             // ws: kr_s times the decay from s to the end of its block of 16
     float2 part[2][CK_MAIN];
-    uint64_t tile_full[2], ta_full[2], main_done[2], au_full[2], g_full, ks_full, qs_full, y_full, d_full, fin;
+    uint64_t tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, fin;
     uint32_t tm;
     int dead;
 };
@@ -85,71 +93,123 @@ __device__ __forceinline__ int scale_exponent(float b) {
     return e < -100 ? -100 : e > 100 ? 100 : e;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
-// two fp32 values as an f16 head and an f16 remainder
+// two fp32 values as an f16 head, the leading eleven bits, and an f16 remainder: 22 bits
 __device__ __forceinline__ void split_h2(float2 x, uint32_t& hi, uint32_t& lo) {
-    const __half2 h = __floats2half2_rn(x.x, x.y);
-    const float2 f = __half22float2(h);
-    hi = h2_bits(h);
-    lo = h2_bits(__floats2half2_rn(x.x - f.x, x.y - f.y));
+    const float2 f = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u), __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
+    hi = h2_bits(__floats2half2_rn(f.x, f.y));
+    const float2 r = __fadd2_rn(x, make_float2(-f.x, -f.y));
+    lo = h2_bits(__floats2half2_rn(r.x, r.y));
 }
 
 // ---- prep warps -----------------------------------------------------------------------------------------------------------
-// k and q rows of a chunk into the raw buffer (zeros behind the chunk's last token); every thread copies what it converts later
-__device__ __forceinline__ void ck_fetch(ChunkSmem& s, const RuleParams& P, int hk, int64_t t0, int len, int pt) {
-    const int lane = pt & 31, w = pt >> 5;
+// Group p prepares the chunks p, p + 2, ...: its latencies (a dozen dependent phases) are spread over two chunks of the main warps.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// decay from one token to a later one, of sums in two floats: their difference is good to 2^-24 of itself however large the sums are
+__device__ __forceinline__ float decay_between(float2 to, float2 from) { return ex2((to.x - from.x) + (to.y - from.y)); }
+__device__ __forceinline__ void prep_bar(int grp) { named_bar(2 + grp, CK_PREP); }
+
+// k and q rows of a chunk, as they come, into the places of the tile where their f16 form goes (zeros behind the chunk's last token),
+// and the rows of v; every thread converts what it has copied
+__device__ __forceinline__ void ck_fetch(unsigned char* tile, uint16_t* vbuf, const RuleParams& P, int hk, int hv, int64_t t0, int len, int w,
+                                         int lane) {
+    const int c = lane & 15, t1 = 32 * (w & 1) + (lane >> 4);                    // token of the thread's first piece; two further each
+    const uint16_t* src = P.mixed + (t0 + t1) * P.mixed_stride + ((w < 2 ? P.H : 0) + hk) * KD + 8 * c;
+    unsigned char* dst = tile + (c >> 3) * 16384;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const int r = 32 * w + 2 * i + (lane >> 4), t = r & 63, c = lane & 15;
-        const bool in = t < len;
-        const uint16_t* src = P.mixed + (in ? t0 + t : t0) * P.mixed_stride + ((r < 64 ? P.H : 0) + hk) * KD + 8 * c;
-        cp_async16(s.raw + r * 256 + c * 16, src, in ? 16u : 0u);
+        const int r = 32 * w + 2 * i + (lane >> 4);
+        const bool in = t1 + 2 * i < len;
+        cp_async16(dst + ck_off(r, c & 7), in ? src : P.mixed, in ? 16u : 0u);
+        src += 2 * P.mixed_stride;
+    }
+    const int tv = 2 * w + (lane >> 4);
+    src = P.mixed + (t0 + tv) * P.mixed_stride + 2 * P.H * KD + hv * VD + 8 * c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool in = tv + 8 * i < len;
+        cp_async16(vbuf + (tv + 8 * i) * VD + 8 * c, in ? src : P.mixed, in ? 16u : 0u);
+        src += 8 * P.mixed_stride;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void ck_convert(ChunkSmem& s, int buf, int pt) {
-    const int lane = pt & 31, w = pt >> 5;
+// Sum of eight values over the sixteen lanes that share lane >> 4, eight shuffles: every exchange halves what a lane keeps.  Lane l
+// returns the total of value 4 (l >> 3 & 1) + 2 (l >> 2 & 1) + (l >> 1 & 1).
+__device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const bool up = lane & 8;
+        a[i] = (up ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[4 + i], 8);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const bool up = lane & 4;
+        b[i] = (up ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, up ? a[i] : a[2 + i], 4);
+    }
+    const bool up = lane & 2;
+    float s = (up ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, up ? b[0] : b[1], 2);
+    return s + __shfl_xor_sync(0xffffffffu, s, 1);
+}
+__device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w, int lane) {
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll 4
-    for (int i = 0; i < 16; ++i) {
-        const int r = 32 * w + 2 * i + (lane >> 4), c = lane & 15;
-        const uint4 x = *reinterpret_cast<const uint4*>(s.raw + r * 256 + c * 16);
-        const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
-        float2 f[4], a2 = make_float2(0.f, 0.f);
+    const int c = lane & 15;
+    tile += (c >> 3) * 16384;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            f[j] = bf16x2_to_f2(xw[j]);
-            a2 = __ffma2_rn(f[j], f[j], a2);
+    for (int hf = 0; hf < 2; ++hf) {
+        float2 f[8][4];
+        float ss[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7));
+            f[i][0] = bf16x2_to_f2(x.x);
+            f[i][1] = bf16x2_to_f2(x.y);
+            f[i][2] = bf16x2_to_f2(x.z);
+            f[i][3] = bf16x2_to_f2(x.w);
+            const float2 a = __ffma2_rn(f[i][1], f[i][1], __fmul2_rn(f[i][0], f[i][0])), b = __ffma2_rn(f[i][3], f[i][3], __fmul2_rn(f[i][2], f[i][2]));
+            ss[i] = (a.x + a.y) + (b.x + b.y);
         }
-        float ss = a2.x + a2.y;
-#pragma unroll
-        for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        const float sum = fold8(ss, lane);                   // of piece (lane >> 1) & 7 with its three bits as fold8 says
         // the row times 2^-e has a norm in [1, 2); a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
-        int e = (int((__float_as_uint(ss) >> 23) & 255u) - 127) >> 1;
+        int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
         e = e < -60 ? -60 : e;
-        const float m = ss <= 3.4e38f ? pow2f(-e) : 0.f;
-        uint32_t h[4];
+        const float m = sum <= 3.4e38f ? pow2f(-e) : 0.f;
+        const int mine = ((lane >> 3) & 1) * 4 + ((lane >> 2) & 1) * 2 + ((lane >> 1) & 1);
+        if (!(lane & 1)) rs[32 * (w & 1) + 16 * hf + 2 * mine + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 y = __fmul2_rn(f[j], make_float2(m, m));
-            h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
+        for (int i = 0; i < 8; ++i) {
+            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | ((i >> 2) << 3) | (((i >> 1) & 1) << 2) | ((i & 1) << 1));
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 y = __fmul2_rn(f[i][j], make_float2(mi, mi));
+                h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
+            }
+            *reinterpret_cast<uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
-        *reinterpret_cast<uint4*>(s.tile[buf] + (c >> 3) * 16384 + ck_off(r, c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-        if (c == 0) (r < 64 ? s.kr : s.qr)[r & 63] = rsqrtf(ss + 1e-6f) * pow2f(e);
     }
 }
-// gates of the chunk, by one warp: lane l has the tokens 2 l and 2 l + 1
-__device__ __forceinline__ void ck_gates(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int len, float ea, float dtb, int lane) {
+// raw gates of the tokens 2 l and 2 l + 1 of a chunk: a | b << 16
+__device__ __forceinline__ void ck_load_gates(const RuleParams& P, int hv, int64_t t0, int len, int lane, uint32_t (&g)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int t = 2 * lane + i;
+        g[i] = t < len ? uint32_t(__ldg(P.a + (t0 + t) * P.a_stride + hv)) | uint32_t(__ldg(P.b + (t0 + t) * P.b_stride + hv)) << 16 : 0u;
+    }
+}
+// decays and beta of the chunk, by one warp; sums in fp64
+__device__ __forceinline__ void ck_gates(PrepSmem& s, const uint32_t (&raw)[2], int len, float ea, float dtb, int lane) {
     double g[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int t = 2 * lane + i;
-        float x = 0.f, beta = 0.f;
-        if (t < len) {
-            x = fmaxf(-ea * softplus_full(bf16_to_f(P.a[(t0 + t) * P.a_stride + hv]) + dtb) * 1.4426950408889634f, -1e30f);
-            beta = sigmoidf_(bf16_to_f(P.b[(t0 + t) * P.b_stride + hv]));
-        }
-        g[i] = double(x);
-        s.gate_beta[t] = beta;
+        // a decay of 2^-200 leaves nothing in fp32; bounded, the differences stay finite
+        const float x = -ea * softplus_full(bf16lo(raw[i]) + dtb) * 1.4426950408889634f;
+        g[i] = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
+        s.beta[t] = t < len ? sigmoidf_(bf16hi(raw[i])) : 0.f;
     }
     double sum = g[0] + g[1];
 #pragma unroll
@@ -157,186 +217,228 @@ __device__ __forceinline__ void ck_gates(ChunkSmem& s, const RuleParams& P, int 
         const double o = __shfl_up_sync(0xffffffffu, sum, d);
         if (lane >= d) sum += o;
     }
-    s.G[2 * lane] = sum - g[1];
-    s.G[2 * lane + 1] = sum;
+    const double first = sum - g[1];
+    const float h0 = float(first), h1 = float(sum);
+    s.G[2 * lane] = make_float2(h0, float(first - double(h0)));
+    s.G[2 * lane + 1] = make_float2(h1, float(sum - double(h1)));
 }
-__device__ __forceinline__ float decay_between(double to, double from) { return exp2f(float(to - from)); }
 
-// Gram rows -> L (fp32, k rows) and A (f16 operand, q rows).  The decay from s to t is taken in two steps over the end of s's block
-// of 16 tokens, neither of which exceeds 1; inside the diagonal blocks it is taken in one.
-__device__ __forceinline__ void ck_gram(ChunkSmem& s, int buf, uint32_t tm, int pt) {
-    const int w = pt >> 5, t = pt & 63, tb = t >> 4;
-    const bool isq = pt >= 64;
-    const double Gt = s.G[t];
-    const float rowf = isq ? s.qr[t] * MAT_UP : s.kr[t] * s.gate_beta[t];
-    const uint32_t ta = tm + (uint32_t(32 * w) << 16) + TM_G;
-#pragma unroll
-    for (int hb = 0; hb < 2; ++hb) {
+// Gram rows -> L (fp32, k rows) and A (f16 operand, q rows); a thread has a row.  Inside a diagonal block of 32 tokens the decay is
+// taken pair by pair; from the first block to the second in two steps over token 31, neither of which exceeds 1.
+__device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32_t gram, int w, int lane) {
+    const bool isq = w >= 2;
+    const int blk = w & 1, t = 32 * blk + lane;
+    const float2 Gt = s.G[t];
+    const float rowf = isq ? s.qr[t] * MAT_UP : s.kr[t] * s.beta[t];
+    gram += uint32_t(32 * w) << 16;
+    if (blk == 1) {
         uint32_t g[32];
-        tmem_ld_32(ta + 32 * hb, g);
-        float v[32];
+        tmem_ld_32(gram, g);
+        const float f = rowf * decay_between(Gt, s.G[31]);
 #pragma unroll
-        for (int b2 = 0; b2 < 2; ++b2) {
-            const int b = 2 * hb + b2;
-            if (b < tb) {
-                const float f = rowf * decay_between(Gt, s.G[16 * b + 15]);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[16 * b2 + j] = __uint_as_float(g[16 * b2 + j]) * (f * s.ws[16 * b + j]);
-            } else if (b == tb) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int c = 16 * b + j;
-                    const bool in = isq ? c <= t : c < t;
-                    v[16 * b2 + j] = in ? __uint_as_float(g[16 * b2 + j]) * (rowf * s.kr[c] * decay_between(Gt, s.G[c])) : 0.f;
-                }
+        for (int c = 0; c < 8; ++c) {
+            const float4 ws = *reinterpret_cast<const float4*>(&s.ws[4 * c]);
+            const float2 a = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(g[4 * c]), __uint_as_float(g[4 * c + 1])), make_float2(f, f)), make_float2(ws.x, ws.y));
+            const float2 b = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(g[4 * c + 2]), __uint_as_float(g[4 * c + 3])), make_float2(f, f)), make_float2(ws.z, ws.w));
+            if (isq) {
+                g[2 * c] = h2_bits(__floats2half2_rn(a.x, a.y));
+                g[2 * c + 1] = h2_bits(__floats2half2_rn(b.x, b.y));
             } else {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) v[16 * b2 + j] = 0.f;
+                *reinterpret_cast<float4*>(&s.L[t][4 * c]) = make_float4(a.x, a.y, b.x, b.y);
             }
         }
-        if (isq) {
+        if (isq)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t h[4];
+            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(amat + ck_off(t, c)) = make_uint4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
+    }
+    uint32_t g[32];
+    tmem_ld_32(gram + 32 * blk, g);
+    const int last = isq ? lane : lane - 1;                  // last column of the block that counts
 #pragma unroll
-                for (int j = 0; j < 4; ++j) h[j] = h2_bits(__floats2half2_rn(v[8 * c + 2 * j], v[8 * c + 2 * j + 1]));
-                *reinterpret_cast<uint4*>(s.amat[buf] + ck_off(t, 4 * hb + c)) = make_uint4(h[0], h[1], h[2], h[3]);
-            }
-        } else {
+    for (int c = 0; c < 32; ++c) {
+        const float d = s.kr[32 * blk + c] * decay_between(Gt, s.G[32 * blk + c]);
+        g[c] = c <= last ? __float_as_uint(__uint_as_float(g[c]) * (rowf * d)) : 0u;
+    }
+    if (isq) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c)
-                *reinterpret_cast<float4*>(&s.L[t][32 * hb + 4 * c]) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+        for (int c = 0; c < 4; ++c) {
+            uint32_t h[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[j] = h2_bits(__floats2half2_rn(__uint_as_float(g[8 * c + 2 * j]), __uint_as_float(g[8 * c + 2 * j + 1])));
+            *reinterpret_cast<uint4*>(amat + ck_off(t, 4 * blk + c)) = make_uint4(h[0], h[1], h[2], h[3]);
         }
+    } else {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(&s.L[t][32 * blk + 4 * c]) = make_uint4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
     }
 }
-__device__ __forceinline__ void ck_put_t(ChunkSmem& s, int buf, int t, int c, float x) {
+__device__ __forceinline__ void ck_put_t(unsigned char* thi, unsigned char* tlo, int t, int c, float x) {
     x *= MAT_UP;
     const __half h = __float2half_rn(x);
     const uint32_t off = ck_off(t, c >> 3) + 2 * (c & 7);
-    *reinterpret_cast<__half*>(s.thi[buf] + off) = h;
-    *reinterpret_cast<__half*>(s.tlo[buf] + off) = __float2half_rn(x - __half2float(h));
+    *reinterpret_cast<__half*>(thi + off) = h;
+    *reinterpret_cast<__half*>(tlo + off) = __float2half_rn(x - __half2float(h));
 }
-// T = (I + L)^-1 by 32 x 32 blocks: the two diagonal blocks by substitution (a lane has a column), then -T22 (L21 T11)
-__device__ __forceinline__ void ck_invert(ChunkSmem& s, int buf, int pt) {
-    const int w = pt >> 5, lane = pt & 31;
-    if (w < 2) {
-        const int o = 32 * w;
-        float2 x[16];
+// sum over m < 4 N of row[m] x[m], row in shared memory (the same for all lanes), x in registers
+template <int N>
+__device__ __forceinline__ float dot_row(const float* row, const float2 (&x)[2 * N]) {
+    float2 a = make_float2(0.f, 0.f), b = a;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float2 acc = make_float2(0.f, 0.f);
-            float last = 0.f;
+    for (int m = 0; m < N; ++m) {
+        const float4 l = *reinterpret_cast<const float4*>(row + 4 * m);
+        a = __ffma2_rn(make_float2(l.x, l.y), x[2 * m], a);
+        b = __ffma2_rn(make_float2(l.z, l.w), x[2 * m + 1], b);
+    }
+    return (a.x + b.x) + (a.y + b.y);
+}
+// T = (I + L)^-1 in blocks: 16 x 16 by substitution (warp w has diagonal block w, a lane a column), then twice the lower left block
+// -T22 (L21 T11) of a square twice as large.
+__device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsigned char* tlo, int grp, int w, int lane) {
+    {
+        const int o = 16 * w, c = lane & 15;
+        float x[16];
 #pragma unroll
-            for (int m = 0; m + 4 <= ((i + 3) & ~3) && m < i; m += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(&s.L[o + i][o + m]);
-                if (m + 2 <= i) acc = __ffma2_rn(make_float2(l.x, l.y), x[m / 2], acc);
-                else last = fmaf(l.x, x[m / 2].x, last);
-                if (m + 4 <= i) acc = __ffma2_rn(make_float2(l.z, l.w), x[m / 2 + 1], acc);
-                else if (m + 3 <= i) last = fmaf(l.z, x[m / 2 + 1].x, last);
+        for (int i = 0; i < 16; ++i) {
+            float4 l[4];
+#pragma unroll
+            for (int m = 0; m < i; m += 4) l[m / 4] = *reinterpret_cast<const float4*>(&s.L[o + i][o + m]);
+            const float* lf = &l[0].x;
+            float a = c == i ? 1.f : 0.f, b = 0.f;
+#pragma unroll
+            for (int m = 0; m < i; ++m) {
+                if (m & 1) b = fmaf(-lf[m], x[m], b);
+                else a = fmaf(-lf[m], x[m], a);
             }
-            const float v = (lane == i ? 1.f : 0.f) - ((acc.x + acc.y) + last);
-            if (i & 1) x[i / 2].y = v;
-            else x[i / 2].x = v;
-            s.tdiag[w][i][lane] = v;
-            ck_put_t(s, buf, o + i, o + lane, v);
+            x[i] = a + b;
+        }
+        if (lane < 16)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s.tdiag[w][i][c] = x[i];
+    }
+    prep_bar(grp);
+    const int sq = w >> 1;                                   // the square of 32 this warp works on, with the other one of its pair
+    {
+        const int c = lane & 15, r0 = 8 * (w & 1) + 4 * (lane >> 4);               // rows r0 .. r0 + 3 of L21 T11
+        float2 x[8];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) x[m] = make_float2(s.tdiag[2 * sq][2 * m][c], s.tdiag[2 * sq][2 * m + 1][c]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.w[16 * sq + r0 + r][c] = dot_row<4>(&s.L[32 * sq + 16 + r0 + r][32 * sq], x);
+    }
+    prep_bar(grp);
+    {
+        const int c = lane & 15, r0 = 8 * (w & 1) + 4 * (lane >> 4);
+        float2 x[8];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) x[m] = make_float2(s.w[16 * sq + 2 * m][c], s.w[16 * sq + 2 * m + 1][c]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = r0 + r;
+            const float v = -dot_row<4>(&s.tdiag[2 * sq + 1][i][0], x), d0 = s.tdiag[2 * sq][i][c], d1 = s.tdiag[2 * sq + 1][i][c];
+            s.t32[sq][16 + i][c] = v;
+            s.t32[sq][i][c] = d0;
+            s.t32[sq][16 + i][16 + c] = d1;
+            s.t32[sq][i][16 + c] = 0.f;
+            ck_put_t(thi, tlo, 32 * sq + 16 + i, 32 * sq + c, v);
+            ck_put_t(thi, tlo, 32 * sq + i, 32 * sq + c, d0);
+            ck_put_t(thi, tlo, 32 * sq + 16 + i, 32 * sq + 16 + c, d1);
         }
     }
-    named_bar(2, CK_PREP);
+    prep_bar(grp);
     {
         float2 x[16];
 #pragma unroll
-        for (int m = 0; m < 16; ++m) x[m] = make_float2(s.tdiag[0][2 * m][lane], s.tdiag[0][2 * m + 1][lane]);
+        for (int m = 0; m < 16; ++m) x[m] = make_float2(s.t32[0][2 * m][lane], s.t32[0][2 * m + 1][lane]);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                const float4 l = *reinterpret_cast<const float4*>(&s.L[32 + 8 * w + r][4 * m]);
-                acc = __ffma2_rn(make_float2(l.x, l.y), x[2 * m], acc);
-                acc = __ffma2_rn(make_float2(l.z, l.w), x[2 * m + 1], acc);
-            }
-            s.w[8 * w + r][lane] = acc.x + acc.y;
-        }
+        for (int r = 0; r < 8; ++r) s.w[8 * w + r][lane] = dot_row<8>(&s.L[32 + 8 * w + r][0], x);
     }
-    named_bar(2, CK_PREP);
+    prep_bar(grp);
     {
         float2 x[16];
 #pragma unroll
         for (int m = 0; m < 16; ++m) x[m] = make_float2(s.w[2 * m][lane], s.w[2 * m + 1][lane]);
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int m = 0; m < 8; ++m) {
-                const float4 l = *reinterpret_cast<const float4*>(&s.tdiag[1][8 * w + r][4 * m]);
-                acc = __ffma2_rn(make_float2(l.x, l.y), x[2 * m], acc);
-                acc = __ffma2_rn(make_float2(l.z, l.w), x[2 * m + 1], acc);
-            }
-            ck_put_t(s, buf, 32 + 8 * w + r, lane, -(acc.x + acc.y));
-        }
+        for (int r = 0; r < 8; ++r) ck_put_t(thi, tlo, 32 + 8 * w + r, lane, -dot_row<8>(&s.t32[1][8 * w + r][0], x));
     }
 }
 
 __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
-                                        int pt) {
-    const int lane = pt & 31;
+                                        int grp, int w, int lane) {
+    const uint32_t el = elect_one();
+    const int pt = 32 * w + lane;
+    PrepSmem& ps = s.prep[grp];
+    ChunkScalars& q = s.sc[grp];
+    unsigned char* tile = s.tile[grp];
     const float ea = expf(P.A_log[hv]), dtb = P.dt_bias[hv];
-    ck_fetch(s, P, hk, t0, int(len < CT ? len : CT), pt);
-    for (int c = 0; c < nchunk; ++c) {
-        const int buf = c & 1;
-        const int64_t at = t0 + int64_t(c) * CT;
-        const int64_t left = len - int64_t(c) * CT;
+    uint32_t graw[2] = {0u, 0u};
+    if (w == 3 && grp < nchunk) ck_load_gates(P, hv, t0 + grp * CT, int(len - grp * CT < CT ? len - grp * CT : CT), lane, graw);
+    for (int c = grp; c < nchunk; c += 2) {
+        const uint32_t ph = uint32_t(c >> 1) & 1u;
+        const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
-        if (c >= 2) ck_wait(s, &s.main_done[buf], uint32_t((c >> 1) - 1) & 1u);
-        ck_convert(s, buf, pt);
-        if (pt >= 96) ck_gates(s, P, hv, at, n, ea, dtb, lane);
+        if (w == 3) ck_gates(ps, graw, n, ea, dtb, lane);
+        if (c >= 2) ck_wait(s, &s.main_done[grp], ph ^ 1u);
+        ck_fetch(tile, &s.v[grp][0][0], P, hk, hv, at, n, w, lane);
+        if (w == 3 && c + 2 < nchunk) ck_load_gates(P, hv, at + 2 * CT, int(left - 2 * CT < CT ? left - 2 * CT : CT), lane, graw);
+        ck_convert(tile, w < 2 ? ps.kr : ps.qr, w, lane);
         fence_async_smem();
-        tc_fence_before_sync();                              // (the Gram matrix of the chunk before has been read)
-        named_bar(2, CK_PREP);
-        if (pt == 0) {
+        tc_fence_before_sync();                              // (this group's last Gram matrix has been read)
+        prep_bar(grp);
+        if (w == 0) {
             tc_fence_after_sync();
-            const uint32_t ti = smem_u32(s.tile[buf]);
+            const uint64_t d0 = ck_desc(smem_u32(tile), 16);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                const uint64_t d = ck_desc(ti + (ks >> 2) * 16384 + (ks & 3) * 32, 16);
-                umma_ss(tm + TM_G, d, d, ck_idesc(64, false), ks > 0);
+                const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+                umma_f16_ss(el, tm + tm_gram(grp), d, d, ck_idesc(64, false), ks > 0);
             }
-            umma_commit(&s.g_full);
+            umma_commit_if(el, &s.g_full[grp]);
         }
-        if (c + 1 < nchunk) ck_fetch(s, P, hk, at + CT, int(left - CT < CT ? left - CT : CT), pt);
+        __syncwarp();
         if (pt < 64) {
-            ChunkScalars& q = s.sc[buf];
-            const double G = s.G[pt], Gc = s.G[CT - 1];
-            const float e = exp2f(float(G)), kr = s.kr[pt], b = s.gate_beta[pt];
+            const float2 G = ps.G[pt], Gc = ps.G[CT - 1];
+            const float e = ex2(G.x + G.y), kr = ps.kr[pt], b = ps.beta[pt];
             q.c1[pt] = b * e * kr;
             q.beta[pt] = b;
-            q.c2[pt] = e * s.qr[pt];
+            q.c2[pt] = e * ps.qr[pt];
             q.c3[pt] = decay_between(Gc, G) * kr * MAT_DOWN;
-            s.ws[pt] = decay_between(s.G[pt | 15], G) * kr;
+            if (pt < 32) ps.ws[pt] = decay_between(ps.G[31], G) * kr;
             if (pt == 0) {
-                q.decay = exp2f(float(Gc));
+                q.decay = ex2(Gc.x + Gc.y);
                 q.len = n;
             }
         }
-        named_bar(2, CK_PREP);
-        if (pt == 0) mbar_arrive(&s.tile_full[buf]);
+        prep_bar(grp);
+        if (pt == 0) mbar_arrive(&s.tile_full[grp]);
         __syncwarp();
-        ck_wait(s, &s.g_full, uint32_t(c) & 1u);
+        ck_wait(s, &s.g_full[grp], ph);
         tc_fence_after_sync();
-        ck_gram(s, buf, tm, pt);
-        named_bar(2, CK_PREP);
-        ck_invert(s, buf, pt);
+        ck_gram(ps, s.amat[grp], tm + tm_gram(grp), w, lane);
+        prep_bar(grp);
+        ck_invert(ps, s.thi[grp], s.tlo[grp], grp, w, lane);
         fence_async_smem();
-        named_bar(2, CK_PREP);
-        if (pt == 0) mbar_arrive(&s.ta_full[buf]);
+        prep_bar(grp);
+        if (pt == 0) mbar_arrive(&s.ta_full[grp]);
         __syncwarp();
     }
-    if (pt == 0) umma_commit(&s.fin);
+    if (w == 0) umma_commit_if(el, &s.fin);
 }
 
 // ---- main warps -----------------------------------------------------------------------------------------------------------
+// outputs of a chunk from shared memory to global, by all main threads
+__device__ __forceinline__ void ck_store(const uint16_t* ob, const RuleParams& P, int hv, int64_t at, int len, int tid) {
+    const int r = tid >> 4, c = tid & 15;
+    uint16_t* op = P.o + ((at + r) * P.HV + hv) * VD + 8 * c;
+    const int64_t step = int64_t(16) * P.HV * VD;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (r + 16 * i < len) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(ob + (r + 16 * i) * VD + 8 * c);
+        op += step;
+    }
+}
 __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
-    const int lane = tid & 31, warp = tid >> 5, h = warp >> 2, v = 32 * (warp & 3) + lane;
+    const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
+    const uint32_t el = elect_one();
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
     float2 S[32];                                            // S[v][64 h ..]
     float* Srow = Sg + v * KD + 64 * h;
@@ -346,25 +448,20 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         S[2 * i] = make_float2(x.x, x.y);
         S[2 * i + 1] = make_float2(x.z, x.w);
     }
-    const uint16_t* vrow = P.mixed + t0 * P.mixed_stride + 2 * P.H * KD + hv * VD + v;
-    float back = 0.f, decay = 0.f;                           // 2^-eB and the decay of the chunk whose D is still to come
+    float back = 0.f, decay = 0.f;                           // of the chunk whose D is still to come: 2^-eB and its decay,
+    int plen = 0;                                            // and its tokens
     for (int c = 0; c <= nchunk; ++c) {
         const int buf = c & 1;
         const uint32_t ph = uint32_t(c >> 1) & 1u;
         const ChunkScalars& q = s.sc[buf];
-        int len = 0;
         uint32_t vv[16];
         float va = 0.f;
         if (c < nchunk) {
             ck_wait(s, &s.tile_full[buf], ph);
-            len = q.len;
-            const uint16_t* vp = vrow + (int64_t(c) * CT + 32 * h) * P.mixed_stride;
-            uint32_t r[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = 32 * h + i < len ? uint32_t(__ldg(vp + i * P.mixed_stride)) : 0u;
+            const uint16_t* vp = &s.v[buf][32 * h][v];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                vv[i] = r[2 * i] | (r[2 * i + 1] << 16);
+                vv[i] = uint32_t(vp[2 * i * VD]) | (uint32_t(vp[(2 * i + 1) * VD]) << 16);
                 va += fabsf(bf16lo(vv[i])) + fabsf(bf16hi(vv[i]));
             }
         }
@@ -382,18 +479,27 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                     S[16 * p + i] = __ffma2_rn(d, b2, __fmul2_rn(S[16 * p + i], d2));
                 }
             }
-            if (c == nchunk) break;
-            // every product of that chunk is through and its scalars have been read: its buffers are free
-            if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
-            __syncwarp();
+            if (c == nchunk) {
+                named_bar(1, CK_MAIN);
+                ck_store(&s.v[buf ^ 1][0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
+                break;
+            }
         }
         // the row's powers of two, from the whole row
-        float2 n2 = make_float2(0.f, 0.f);
+        float2 n2[4];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) n2 = __ffma2_rn(S[i], S[i], n2);
-        s.part[buf][tid] = make_float2(n2.x + n2.y, va);
+        for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
+#pragma unroll
+        for (int i = 4; i < 32; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
+        n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
+        s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
+        if (c > 0) {                                         // outputs of the chunk before; with them its buffers are free
+            ck_store(&s.v[buf ^ 1][0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
+            __syncwarp();
+            if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
+        }
         const float2 mine = s.part[buf][tid], other = s.part[buf][tid ^ 128];
         const float norm = sqrtf(mine.x + other.x);
         const int eS = scale_exponent(norm), eB = scale_exponent(norm + (mine.y + other.y));
@@ -410,19 +516,19 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
         const uint32_t ti = smem_u32(s.tile[buf]);
-        if (tid == 0) {                                      // S k^T, then S q^T
+        if (warp == 0) {                                     // S k^T, then S q^T
             tc_fence_after_sync();
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
                 const uint64_t d = ck_desc(ti + (ks >> 2) * 16384 + (ks & 3) * 32, 16);
-                umma_f16_ts(tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
-                umma_f16_ts(tm + TM_X, tm + TM_SLO + 8 * ks, d, ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
+                umma_f16_ts(el, tm + TM_X, tm + TM_SLO + 8 * ks, d, ck_idesc(64, false), 1u);
             }
-            umma_commit(&s.ks_full);
+            umma_commit_if(el, &s.ks_full);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-                umma_f16_ts(tm + TM_XQ, tm + TM_SHI + 8 * ks, ck_desc(ti + (ks >> 2) * 16384 + 8192 + (ks & 3) * 32, 16), ck_idesc(64, false), ks > 0);
-            umma_commit(&s.qs_full);
+                umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, ck_desc(ti + (ks >> 2) * 16384 + 8192 + (ks & 3) * 32, 16), ck_idesc(64, false), ks > 0);
+            umma_commit_if(el, &s.qs_full);
         }
         __syncwarp();
         const float fB = pow2f(eB), fX = pow2f(eB - eS < -126 ? -126 : eB - eS);
@@ -445,16 +551,16 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
         if (warp == 0) ck_wait(s, &s.ta_full[buf], ph);
-        if (tid == 0) {                                      // u = T r
+        if (warp == 0) {                                     // u = T r
             tc_fence_after_sync();
             const uint32_t th = smem_u32(s.thi[buf]), tl = smem_u32(s.tlo[buf]);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                umma_f16_ts(tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), ks > 0);
-                umma_f16_ts(tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(tl + ks * 32, 16), ck_idesc(64, false), 1u);
-                umma_f16_ts(tm + TM_Y, tm + TM_PLO + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), ks > 0);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(tl + ks * 32, 16), ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PLO + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), 1u);
             }
-            umma_commit(&s.y_full);
+            umma_commit_if(el, &s.y_full);
         }
         __syncwarp();
         float2 o[16];                                        // e^G S q^, in outputs' units
@@ -487,23 +593,24 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         }
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
-        if (tid == 0) {                                      // A u, then the chunk's part of the state
+        if (warp == 0) {                                     // A u, then the chunk's part of the state
             tc_fence_after_sync();
             const uint32_t am = smem_u32(s.amat[buf]);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-                umma_f16_ts(tm + TM_AU, tm + TM_UOP + 8 * ks, ck_desc(am + ks * 32, 16), ck_idesc(64, false), ks > 0);
-            umma_commit(&s.au_full[buf]);
+                umma_f16_ts(el, tm + TM_AU, tm + TM_UOP + 8 * ks, ck_desc(am + ks * 32, 16), ck_idesc(64, false), ks > 0);
+            umma_commit_if(el, &s.au_full[buf]);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
                 const uint64_t d = ck_desc(ti + ks * 2048, 16384);
-                umma_f16_ts(tm + TM_D, tm + TM_PHI + 8 * ks, d, ck_idesc(128, true), ks > 0);
-                umma_f16_ts(tm + TM_D, tm + TM_PLO + 8 * ks, d, ck_idesc(128, true), 1u);
+                umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, d, ck_idesc(128, true), ks > 0);
+                umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, d, ck_idesc(128, true), 1u);
             }
-            umma_commit(&s.d_full);
+            umma_commit_if(el, &s.d_full);
         }
         __syncwarp();
         decay = q.decay;
+        plen = q.len;
         back = pow2f(-eB);
         ck_wait(s, &s.au_full[buf], ph);
         tc_fence_after_sync();
@@ -511,25 +618,20 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             uint32_t x[32];
             tmem_ld_32(row + TM_AU + 32 * h, x);
             const float f = P.scale * back * MAT_DOWN;
-            uint16_t* op = P.o + ((t0 + int64_t(c) * CT + 32 * h) * P.HV + hv) * VD + v;
-            const int64_t step = int64_t(P.HV) * VD;
-            const int m = len - 32 * h;
+            uint16_t* op = &s.v[buf][32 * h][v];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float y = fmaf(__uint_as_float(x[i]), f, (i & 1) ? o[i >> 1].y : o[i >> 1].x);
-                if (i < m) op[i * step] = f_to_bf16(y);
-            }
+            for (int i = 0; i < 32; ++i) op[i * VD] = f_to_bf16(fmaf(__uint_as_float(x[i]), f, (i & 1) ? o[i >> 1].y : o[i >> 1].x));
         }
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i)
         *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
-    if (tid == 0) umma_commit(&s.fin);
+    if (warp == 0) umma_commit_if(el, &s.fin);
 }
 
 __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P) {
-    extern __shared__ unsigned char dyn[];
-    ChunkSmem& s = *reinterpret_cast<ChunkSmem*>((reinterpret_cast<uintptr_t>(dyn) + 1023) & ~uintptr_t(1023));
+    extern __shared__ __align__(128) unsigned char rule_smem[];
+    ChunkSmem& s = *reinterpret_cast<ChunkSmem*>(rule_smem + ((1024u - (smem_u32(rule_smem) & 1023u)) & 1023u));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_trigger();
     if (tid == 0) {
@@ -538,13 +640,13 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P)
             mbar_init(&s.ta_full[i], 1);
             mbar_init(&s.main_done[i], CK_MAIN / 32);
             mbar_init(&s.au_full[i], 1);
+            mbar_init(&s.g_full[i], 1);
         }
-        mbar_init(&s.g_full, 1);
         mbar_init(&s.ks_full, 1);
         mbar_init(&s.qs_full, 1);
         mbar_init(&s.y_full, 1);
         mbar_init(&s.d_full, 1);
-        mbar_init(&s.fin, 2);
+        mbar_init(&s.fin, 3);
         s.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -559,9 +661,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P)
             *reinterpret_cast<uint4*>(P.o + ((t0 + i / (VD / 8)) * P.HV + hv) * VD + 8 * (i % (VD / 8))) = make_uint4(0u, 0u, 0u, 0u);
         return;
     }
-    for (int i = tid; i < 2 * 8192 / 16; i += CK_THREADS) {                        // the upper right block of T stays zero
+    for (int i = tid; i < 2 * 8192 / 16; i += CK_THREADS) {                        // the upper right blocks of T and A stay zero
         reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);
         reinterpret_cast<uint4*>(s.tlo)[i] = make_uint4(0u, 0u, 0u, 0u);
+        reinterpret_cast<uint4*>(s.amat)[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     if (warp == 0) tmem_alloc(&s.tm, 512);
     fence_async_smem();
@@ -570,8 +673,14 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P)
     tc_fence_after_sync();
     const uint32_t tm = s.tm;
     const int nchunk = int((len + CT - 1) / CT);
-    if (tid >= CK_MAIN) ck_prep(s, P, hk, hv, t0, len, nchunk, tm, tid - CK_MAIN);
-    else ck_main(s, P, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
+    const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
+    if (uw >= CK_MAIN / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
+        ck_prep(s, P, hk, hv, t0, len, nchunk, tm, (uw >> 2) & 1, uw & 3, lane);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_MAIN_REGS));
+        ck_main(s, P, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
+    }
     ck_wait(s, &s.fin, 0);                                   // no tensor-core instruction is left
     tc_fence_before_sync();
     __syncthreads();
