@@ -17,6 +17,8 @@
 // a power of two of its own, from bounds that hold whatever the inputs: |k^| <= 1, 0 <= beta <= 1 and decays <= 1 make the rule a
 // contraction, |r_t|, |u_t| / 2, |S| <= |S_0| + sum |v_t| =: B per row.  T is bounded by 1 for the same reason.  The products that
 // only reach the bf16 outputs (S q, A u) take one piece, 2^-12.
+#include <stddef.h>
+
 #include "lq_tc.cuh"
 
 namespace lq {
@@ -46,25 +48,25 @@ __device__ __forceinline__ uint64_t ck_desc(uint32_t addr, uint32_t lbo) {
 // byte offset of 16-byte chunk c (of 8) of a row in such a tile
 __device__ __forceinline__ uint32_t ck_off(int row, int c) { return uint32_t(row) * 128u + (uint32_t(c ^ (row & 7)) << 4); }
 
-struct ChunkScalars {                                        // of one chunk, by token
-    float c1[CT];                                            // beta e^{G_t} kr_t: takes S k to what is subtracted from beta v
+struct alignas(16) ChunkScalars {                                        // of one chunk, by token
+    float c1[CT];                                            // -beta e^{G_t} kr_t: takes S k to what is added to beta v
     float beta[CT];
     float c2[CT];                                            // e^{G_t} qr_t
     float c3[CT];                                            // e^{G_C - G_t} kr_t 2^-13 (u comes with the 2^13 of T)
     float decay;                                             // e^{G_C}
     int len;                                                 // tokens of the chunk, 1 .. 64
 };
-struct PrepSmem {                                            // of one prep group
-    float L[CT][CT + 4];
-    float tdiag[4][16][16], t32[2][32][32], w[32][32];       // inverses of the diagonal blocks of 16 and 32; products on the way
-    float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
+struct alignas(16) PrepSmem {                                            // of one prep group
+    float L[CT][CT + 4];                                     // times 2^13, like everything that becomes f16 on the way to T
+    float tt[2][32][36];                                     // transposed inverses of the two diagonal blocks of 32, times 2^13
+    float2 G[CT], Gk[CT];                                    // log2 of the decay from the chunk's start, head and remainder; Gk: over kr
     float kr[CT], qr[CT], ws[32], beta[CT];                  // ws: kr_s times the decay from s to token 31, for s < 32
 };
-struct ChunkSmem {
+struct alignas(16) ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
     unsigned char thi[2][8192], tlo[2][8192], amat[2][8192];
-    uint16_t v[2][CT][VD];                                   // bf16 values; once they are used, the chunk's outputs on their way out
+    uint16_t v[2][CT][VD], o[CT][VD];                        // bf16 values, and outputs on their way out
     PrepSmem prep[2];
     ChunkScalars sc[2];
     float2 part[2][CK_MAIN];
@@ -72,6 +74,12 @@ struct ChunkSmem {
     uint32_t tm;
     int dead;
 };
+
+static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
+                  offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 16 == 0 && offsetof(ChunkSmem, o) % 16 == 0 &&
+                  offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(PrepSmem, tt) % 16 == 0 &&
+                  offsetof(PrepSmem, Gk) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, tile_full) % 8 == 0,
+              "vector accesses and swizzled tiles");
 
 // Waits like warp_wait_bounded; once one wait of the CTA has run out, all later ones of every warp return at once, so that the CTA
 // runs to its end (on rubbish) instead of waiting that long again and again.
@@ -116,23 +124,26 @@ __device__ __forceinline__ void prep_bar(int grp) { named_bar(2 + grp, CK_PREP);
 // and the rows of v; every thread converts what it has copied
 __device__ __forceinline__ void ck_fetch(unsigned char* tile, uint16_t* vbuf, const RuleParams& P, int hk, int hv, int64_t t0, int len, int w,
                                          int lane) {
-    const int c = lane & 15, t1 = 32 * (w & 1) + (lane >> 4);                    // token of the thread's first piece; two further each
+    const int c = lane & 15, t1 = 32 * (w & 1) + (lane >> 4), tv = 2 * w + (lane >> 4);   // token of the thread's first piece
     const uint16_t* src = P.mixed + (t0 + t1) * P.mixed_stride + ((w < 2 ? P.H : 0) + hk) * KD + 8 * c;
-    unsigned char* dst = tile + (c >> 3) * 16384;
+    const uint16_t* vsrc = P.mixed + (t0 + tv) * P.mixed_stride + 2 * P.H * KD + hv * VD + 8 * c;
+    unsigned char* dst = tile + (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128;
+    uint16_t* vdst = vbuf + tv * VD + 8 * c;
+    const int64_t step = 2 * P.mixed_stride, vstep = 8 * P.mixed_stride;
+    if (len == CT) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int r = 32 * w + 2 * i + (lane >> 4);
-        const bool in = t1 + 2 * i < len;
-        cp_async16(dst + ck_off(r, c & 7), in ? src : P.mixed, in ? 16u : 0u);
-        src += 2 * P.mixed_stride;
-    }
-    const int tv = 2 * w + (lane >> 4);
-    src = P.mixed + (t0 + tv) * P.mixed_stride + 2 * P.H * KD + hv * VD + 8 * c;
+        for (int i = 0; i < 16; ++i, src += step) cp_async16(dst + 256 * i + (((c & 7) ^ ((2 * i + (lane >> 4)) & 7)) << 4), src, 16u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bool in = tv + 8 * i < len;
-        cp_async16(vbuf + (tv + 8 * i) * VD + 8 * c, in ? src : P.mixed, in ? 16u : 0u);
-        src += 8 * P.mixed_stride;
+        for (int i = 0; i < 8; ++i, vsrc += vstep) cp_async16(vdst + 8 * i * VD, vsrc, 16u);
+    } else {
+        for (int i = 0; i < 16; ++i, src += step) {
+            const bool in = t1 + 2 * i < len;
+            cp_async16(dst + 256 * i + (((c & 7) ^ ((2 * i + (lane >> 4)) & 7)) << 4), in ? src : P.mixed, in ? 16u : 0u);
+        }
+        for (int i = 0; i < 8; ++i, vsrc += vstep) {
+            const bool in = tv + 8 * i < len;
+            cp_async16(vdst + 8 * i * VD, in ? vsrc : P.mixed, in ? 16u : 0u);
+        }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -160,16 +171,14 @@ __device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w
     tile += (c >> 3) * 16384;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-        float2 f[8][4];
+        uint4 x[8];
         float ss[8];
 #pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7));
+#pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7));
-            f[i][0] = bf16x2_to_f2(x.x);
-            f[i][1] = bf16x2_to_f2(x.y);
-            f[i][2] = bf16x2_to_f2(x.z);
-            f[i][3] = bf16x2_to_f2(x.w);
-            const float2 a = __ffma2_rn(f[i][1], f[i][1], __fmul2_rn(f[i][0], f[i][0])), b = __ffma2_rn(f[i][3], f[i][3], __fmul2_rn(f[i][2], f[i][2]));
+            const float2 f0 = bf16x2_to_f2(x[i].x), f1 = bf16x2_to_f2(x[i].y), f2 = bf16x2_to_f2(x[i].z), f3 = bf16x2_to_f2(x[i].w);
+            const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2));
             ss[i] = (a.x + a.y) + (b.x + b.y);
         }
         const float sum = fold8(ss, lane);                   // of piece (lane >> 1) & 7 with its three bits as fold8 says
@@ -182,10 +191,11 @@ __device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | ((i >> 2) << 3) | (((i >> 1) & 1) << 2) | ((i & 1) << 1));
+            const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
             uint32_t h[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 y = __fmul2_rn(f[i][j], make_float2(mi, mi));
+                const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), make_float2(mi, mi));
                 h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
             }
             *reinterpret_cast<uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
@@ -229,7 +239,7 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
     const bool isq = w >= 2;
     const int blk = w & 1, t = 32 * blk + lane;
     const float2 Gt = s.G[t];
-    const float rowf = isq ? s.qr[t] * MAT_UP : s.kr[t] * s.beta[t];
+    const float rowf = (isq ? s.qr[t] : s.kr[t] * s.beta[t]) * MAT_UP;
     gram += uint32_t(32 * w) << 16;
     if (blk == 1) {
         uint32_t g[32];
@@ -255,9 +265,12 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
     tmem_ld_32(gram + 32 * blk, g);
     const int last = isq ? lane : lane - 1;                  // last column of the block that counts
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-        const float d = s.kr[32 * blk + c] * decay_between(Gt, s.G[32 * blk + c]);
-        g[c] = c <= last ? __float_as_uint(__uint_as_float(g[c]) * (rowf * d)) : 0u;
+    for (int c = 0; c < 32; c += 2) {
+        const float4 from = *reinterpret_cast<const float4*>(&s.Gk[32 * blk + c]);
+        const float2 d = __fmul2_rn(make_float2(rowf, rowf), make_float2(decay_between(Gt, make_float2(from.x, from.y)), decay_between(Gt, make_float2(from.z, from.w))));
+        const float2 y = __fmul2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), d);
+        g[c] = c <= last ? __float_as_uint(y.x) : 0u;
+        g[c + 1] = c < last ? __float_as_uint(y.y) : 0u;
     }
     if (isq) {
 #pragma unroll
@@ -272,93 +285,119 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(&s.L[t][32 * blk + 4 * c]) = make_uint4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
     }
 }
-__device__ __forceinline__ void ck_put_t(unsigned char* thi, unsigned char* tlo, int t, int c, float x) {
-    x *= MAT_UP;
-    const __half h = __float2half_rn(x);
-    const uint32_t off = ck_off(t, c >> 3) + 2 * (c & 7);
-    *reinterpret_cast<__half*>(thi + off) = h;
-    *reinterpret_cast<__half*>(tlo + off) = __float2half_rn(x - __half2float(h));
+struct Pieces { uint32_t hi, lo; };
+__device__ __forceinline__ Pieces pieces(float2 x) {
+    Pieces p;
+    split_h2(x, p.hi, p.lo);
+    return p;
 }
-// sum over m < 4 N of row[m] x[m], row in shared memory (the same for all lanes), x in registers
-template <int N>
-__device__ __forceinline__ float dot_row(const float* row, const float2 (&x)[2 * N]) {
-    float2 a = make_float2(0.f, 0.f), b = a;
-#pragma unroll
-    for (int m = 0; m < N; ++m) {
-        const float4 l = *reinterpret_cast<const float4*>(row + 4 * m);
-        a = __ffma2_rn(make_float2(l.x, l.y), x[2 * m], a);
-        b = __ffma2_rn(make_float2(l.z, l.w), x[2 * m + 1], b);
-    }
-    return (a.x + b.x) + (a.y + b.y);
+// D += A B for one m16n8k16 tile of operands in two pieces
+__device__ __forceinline__ void mma_pieces(float (&d)[4], const Pieces (&a)[4], const Pieces& b0, const Pieces& b1) {
+    mma_h_16816(d, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b0.hi, b1.hi);
+    mma_h_16816(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.lo, b1.lo);
+    mma_h_16816(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.hi, b1.hi);
+}
+__device__ __forceinline__ float2 lds2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+// two neighbours of a row of T, which is kept transposed
+__device__ __forceinline__ float2 t_pair(const float (&tt)[32][36], int i, int n) { return make_float2(tt[n][i], tt[n + 1][i]); }
+__device__ __forceinline__ void put_t(unsigned char* thi, unsigned char* tlo, int t, int c, Pieces p) {
+    const uint32_t off = ck_off(t, c >> 3) + 2 * (c & 7);
+    *reinterpret_cast<uint32_t*>(thi + off) = p.hi;
+    *reinterpret_cast<uint32_t*>(tlo + off) = p.lo;
 }
 // T = (I + L)^-1 in blocks: 16 x 16 by substitution (warp w has diagonal block w, a lane a column), then twice the lower left block
-// -T22 (L21 T11) of a square twice as large.
+// -T22 (L21 T11) of a square twice as large, on mma.sync.  The first product is taken transposed, (L21 T11)^T = T11^T L21^T: its
+// accumulators are then the B operand of the second as they are.  Scales: L and T times 2^13, their product back to 2^10 (a sum of 32).
 __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsigned char* tlo, int grp, int w, int lane) {
+    const int gid = lane >> 2, tig = lane & 3;
     {
         const int o = 16 * w, c = lane & 15;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            float4 l[4];
+            float a = 0.f, b = 0.f;
 #pragma unroll
-            for (int m = 0; m < i; m += 4) l[m / 4] = *reinterpret_cast<const float4*>(&s.L[o + i][o + m]);
-            const float* lf = &l[0].x;
-            float a = c == i ? 1.f : 0.f, b = 0.f;
-#pragma unroll
-            for (int m = 0; m < i; ++m) {
-                if (m & 1) b = fmaf(-lf[m], x[m], b);
-                else a = fmaf(-lf[m], x[m], a);
+            for (int m = 0; m < i; m += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(&s.L[o + i][o + m]);
+                a = fmaf(l.x, x[m], a);
+                if (m + 1 < i) b = fmaf(l.y, x[m + 1], b);
+                if (m + 2 < i) a = fmaf(l.z, x[m + 2], a);
+                if (m + 3 < i) b = fmaf(l.w, x[m + 3], b);
             }
-            x[i] = a + b;
+            x[i] = fmaf(a + b, -MAT_DOWN, c == i ? MAT_UP : 0.f);
         }
         if (lane < 16)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s.tdiag[w][i][c] = x[i];
-    }
-    prep_bar(grp);
-    const int sq = w >> 1;                                   // the square of 32 this warp works on, with the other one of its pair
-    {
-        const int c = lane & 15, r0 = 8 * (w & 1) + 4 * (lane >> 4);               // rows r0 .. r0 + 3 of L21 T11
-        float2 x[8];
-#pragma unroll
-        for (int m = 0; m < 8; ++m) x[m] = make_float2(s.tdiag[2 * sq][2 * m][c], s.tdiag[2 * sq][2 * m + 1][c]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) s.w[16 * sq + r0 + r][c] = dot_row<4>(&s.L[32 * sq + 16 + r0 + r][32 * sq], x);
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4*>(&s.tt[w >> 1][(o & 16) + c][(o & 16) + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
     }
     prep_bar(grp);
     {
-        const int c = lane & 15, r0 = 8 * (w & 1) + 4 * (lane >> 4);
-        float2 x[8];
+        const int sq = w >> 1, nt = w & 1, o = 32 * sq;      // the square of 32, and which eight of its first sixteen columns
+        const float (&tt)[32][36] = s.tt[sq];
+        float X[2][4] = {};
+        Pieces a[4], wb[2];
 #pragma unroll
-        for (int m = 0; m < 8; ++m) x[m] = make_float2(s.w[16 * sq + 2 * m][c], s.w[16 * sq + 2 * m + 1][c]);
+        for (int r = 0; r < 4; ++r) a[r] = pieces(lds2(&tt[gid + 8 * (r & 1)][2 * tig + 8 * (r >> 1)]));
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = r0 + r;
-            const float v = -dot_row<4>(&s.tdiag[2 * sq + 1][i][0], x), d0 = s.tdiag[2 * sq][i][c], d1 = s.tdiag[2 * sq + 1][i][c];
-            s.t32[sq][16 + i][c] = v;
-            s.t32[sq][i][c] = d0;
-            s.t32[sq][16 + i][16 + c] = d1;
-            s.t32[sq][i][16 + c] = 0.f;
-            ck_put_t(thi, tlo, 32 * sq + 16 + i, 32 * sq + c, v);
-            ck_put_t(thi, tlo, 32 * sq + i, 32 * sq + c, d0);
-            ck_put_t(thi, tlo, 32 * sq + 16 + i, 32 * sq + 16 + c, d1);
+        for (int j = 0; j < 2; ++j) {
+            const float* l = &s.L[o + 16 + 8 * j + gid][o + 2 * tig];
+            mma_pieces(X[j], a, pieces(lds2(l)), pieces(lds2(l + 8)));
+            const float2 y = nt ? make_float2(X[j][2], X[j][3]) : make_float2(X[j][0], X[j][1]);
+            wb[j] = pieces(__fmul2_rn(y, make_float2(0x1p-16f, 0x1p-16f)));
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) a[r] = pieces(t_pair(tt, 16 + gid + 8 * (r & 1), 16 + 2 * tig + 8 * (r >> 1)));
+        float d[4] = {};
+        mma_pieces(d, a, wb[0], wb[1]);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int i = gid + 8 * r, n = 8 * nt + 2 * tig;
+            const float2 y = __fmul2_rn(make_float2(d[2 * r], d[2 * r + 1]), make_float2(-0x1p-10f, -0x1p-10f));
+            put_t(thi, tlo, o + 16 + i, o + n, pieces(y));
+            put_t(thi, tlo, o + 16 + i, o + 16 + n, nt ? a[2 + r] : a[r]);
+            put_t(thi, tlo, o + i, o + n, pieces(t_pair(tt, i, n)));
+            s.tt[sq][n][16 + i] = y.x;
+            s.tt[sq][n + 1][16 + i] = y.y;
         }
     }
     prep_bar(grp);
     {
-        float2 x[16];
+        const int n0 = 16 * (w & 1), i0 = 16 * (w >> 1);     // sixteen columns of T11, sixteen rows of T22
+        float X[4][4] = {};
+        Pieces a[4];
 #pragma unroll
-        for (int m = 0; m < 16; ++m) x[m] = make_float2(s.t32[0][2 * m][lane], s.t32[0][2 * m + 1][lane]);
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 0 && n0) continue;                     // T11 is lower triangular
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s.w[8 * w + r][lane] = dot_row<8>(&s.L[32 + 8 * w + r][0], x);
-    }
-    prep_bar(grp);
-    {
-        float2 x[16];
+            for (int r = 0; r < 4; ++r) a[r] = pieces(lds2(&s.tt[0][n0 + gid + 8 * (r & 1)][16 * ks + 2 * tig + 8 * (r >> 1)]));
 #pragma unroll
-        for (int m = 0; m < 16; ++m) x[m] = make_float2(s.w[2 * m][lane], s.w[2 * m + 1][lane]);
+            for (int j = 0; j < 4; ++j) {
+                const float* l = &s.L[32 + 8 * j + gid][16 * ks + 2 * tig];
+                mma_pieces(X[j], a, pieces(lds2(l)), pieces(lds2(l + 8)));
+            }
+        }
+        float d[2][4] = {};
 #pragma unroll
-        for (int r = 0; r < 8; ++r) ck_put_t(thi, tlo, 32 + 8 * w + r, lane, -dot_row<8>(&s.t32[1][8 * w + r][0], x));
+        for (int ks = 0; ks < 2; ++ks) {
+            if (ks == 1 && !i0) continue;                    // so is T22
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[r] = pieces(t_pair(s.tt[1], i0 + gid + 8 * (r & 1), 16 * ks + 2 * tig + 8 * (r >> 1)));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                Pieces b[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    b[j] = pieces(__fmul2_rn(make_float2(X[2 * ks + j][2 * q], X[2 * ks + j][2 * q + 1]), make_float2(0x1p-16f, 0x1p-16f)));
+                mma_pieces(d[q], a, b[0], b[1]);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+                put_t(thi, tlo, 32 + i0 + gid + 8 * r, n0 + 8 * q + 2 * tig,
+                      pieces(__fmul2_rn(make_float2(d[q][2 * r], d[q][2 * r + 1]), make_float2(-0x1p-10f, -0x1p-10f))));
     }
 }
 
@@ -398,10 +437,11 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, int h
         if (pt < 64) {
             const float2 G = ps.G[pt], Gc = ps.G[CT - 1];
             const float e = ex2(G.x + G.y), kr = ps.kr[pt], b = ps.beta[pt];
-            q.c1[pt] = b * e * kr;
+            q.c1[pt] = -(b * e * kr);
             q.beta[pt] = b;
             q.c2[pt] = e * ps.qr[pt];
             q.c3[pt] = decay_between(Gc, G) * kr * MAT_DOWN;
+            ps.Gk[pt] = make_float2(G.x, G.y - log2f(kr));
             if (pt < 32) ps.ws[pt] = decay_between(ps.G[31], G) * kr;
             if (pt == 0) {
                 q.decay = ex2(Gc.x + Gc.y);
@@ -436,11 +476,15 @@ __device__ __forceinline__ void ck_store(const uint16_t* ob, const RuleParams& P
         op += step;
     }
 }
+__device__ __forceinline__ float2 f2_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Chunk c's outputs are finished while S k of chunk c + 1 is under way, and leave for memory while T r of it is.
 __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
     const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
     const uint32_t el = elect_one();
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
-    float2 S[32];                                            // S[v][64 h ..]
+    float2 S[32];                                            // S[v][64 h ..] times 2^e
     float* Srow = Sg + v * KD + 64 * h;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -448,8 +492,9 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         S[2 * i] = make_float2(x.x, x.y);
         S[2 * i + 1] = make_float2(x.z, x.w);
     }
-    float back = 0.f, decay = 0.f;                           // of the chunk whose D is still to come: 2^-eB and its decay,
-    int plen = 0;                                            // and its tokens
+    int e = 0, plen = 0;
+    float decay = 0.f, of = 0.f;                             // of the chunk before: its decay, 2^-e scale of its outputs
+    float2 o[16];                                            // e^G S q^ of the chunk before, times 2^e
     for (int c = 0; c <= nchunk; ++c) {
         const int buf = c & 1;
         const uint32_t ph = uint32_t(c >> 1) & 1u;
@@ -459,90 +504,111 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         if (c < nchunk) {
             ck_wait(s, &s.tile_full[buf], ph);
             const uint16_t* vp = &s.v[buf][32 * h][v];
+            __nv_bfloat162 sum = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 vv[i] = uint32_t(vp[2 * i * VD]) | (uint32_t(vp[(2 * i + 1) * VD]) << 16);
-                va += fabsf(bf16lo(vv[i])) + fabsf(bf16hi(vv[i]));
+                const uint32_t a = vv[i] & 0x7fff7fffu;
+                sum = __hadd2(sum, *reinterpret_cast<const __nv_bfloat162*>(&a));
             }
+            va = (__low2float(sum) + __high2float(sum)) * 1.0625f;       // sixteen roundings to 8 bits: not below the sum of |v|
         }
         if (c > 0) {                                         // the state behind the chunk before
             ck_wait(s, &s.d_full, uint32_t(c - 1) & 1u);
             tc_fence_after_sync();
-            const float2 d2 = make_float2(decay, decay), b2 = make_float2(back, back);
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
                 uint32_t r[32];
                 tmem_ld_32(row + TM_D + 64 * h + 32 * p, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float2 d = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-                    S[16 * p + i] = __ffma2_rn(d, b2, __fmul2_rn(S[16 * p + i], d2));
-                }
+                for (int i = 0; i < 16; ++i) S[16 * p + i] = __ffma2_rn(S[16 * p + i], both(decay), f2_of(r[2 * i], r[2 * i + 1]));
             }
-            if (c == nchunk) {
-                named_bar(1, CK_MAIN);
-                ck_store(&s.v[buf ^ 1][0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
-                break;
-            }
-        }
-        // the row's powers of two, from the whole row
-        float2 n2[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
-#pragma unroll
-        for (int i = 4; i < 32; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
-        n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
-        s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
-        tc_fence_before_sync();
-        named_bar(1, CK_MAIN);
-        if (c > 0) {                                         // outputs of the chunk before; with them its buffers are free
-            ck_store(&s.v[buf ^ 1][0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
-            __syncwarp();
+            // every product of that chunk is through, and its scalars and values have been read: its buffers are free
             if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
+            __syncwarp();
         }
-        const float2 mine = s.part[buf][tid], other = s.part[buf][tid ^ 128];
-        const float norm = sqrtf(mine.x + other.x);
-        const int eS = scale_exponent(norm), eB = scale_exponent(norm + (mine.y + other.y));
-        {
-            const float2 f = make_float2(pow2f(eS), pow2f(eS));
-            uint32_t hi[32], lo[32];
+        if (c < nchunk) {
+            // the row's power of two: B = |S| + sum |v| becomes 2^13 or more
+            float2 n2[4];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) split_h2(__fmul2_rn(S[i], f), hi[i], lo[i]);
+            for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
+#pragma unroll
+            for (int i = 4; i < 32; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
+            n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
+            s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
+            tc_fence_before_sync();
+            named_bar(1, CK_MAIN);
+            const float2 other = s.part[buf][tid ^ 128];
+            const float bound = sqrtf(n2[0].x + n2[0].y + other.x) * pow2f(-e) + (va + other.y);
+            const int en = scale_exponent(bound), de = en - e;
+            const float2 up = both(pow2f(de < -126 ? -126 : de > 127 ? 127 : de));
+            e = en;
             tc_fence_after_sync();
-            tmem_st_32(row + TM_SHI + 32 * h, hi);
-            tmem_st_32(row + TM_SLO + 32 * h, lo);
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                uint32_t hi[16], lo[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    S[16 * p + i] = __fmul2_rn(S[16 * p + i], up);
+                    split_h2(S[16 * p + i], hi[i], lo[i]);
+                }
+                tmem_st_16(row + TM_SHI + 32 * h + 16 * p, hi);
+                tmem_st_16(row + TM_SLO + 32 * h + 16 * p, lo);
+            }
             tmem_st_wait();
+            tc_fence_before_sync();
+            named_bar(1, CK_MAIN);
         }
-        tc_fence_before_sync();
-        named_bar(1, CK_MAIN);
         const uint32_t ti = smem_u32(s.tile[buf]);
-        if (warp == 0) {                                     // S k^T, then S q^T
+        if (warp == 0 && c < nchunk) {                       // S k^T, then S q^T
             tc_fence_after_sync();
+            const uint64_t d0 = ck_desc(ti, 16);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                const uint64_t d = ck_desc(ti + (ks >> 2) * 16384 + (ks & 3) * 32, 16);
+                const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
                 umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
                 umma_f16_ts(el, tm + TM_X, tm + TM_SLO + 8 * ks, d, ck_idesc(64, false), 1u);
             }
             umma_commit_if(el, &s.ks_full);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-                umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, ck_desc(ti + (ks >> 2) * 16384 + 8192 + (ks & 3) * 32, 16), ck_idesc(64, false), ks > 0);
+                umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, d0 + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
             umma_commit_if(el, &s.qs_full);
         }
         __syncwarp();
-        const float fB = pow2f(eB), fX = pow2f(eB - eS < -126 ? -126 : eB - eS);
-        ck_wait(s, &s.ks_full, uint32_t(c) & 1u);
-        tc_fence_after_sync();
-        {                                                    // r = beta (v - e^G S k^), times 2^eB
-            uint32_t x[32], hi[16], lo[16];
-            tmem_ld_32(row + TM_X + 32 * h, x);
+        if (c > 0) {                                         // outputs of the chunk before
+            ck_wait(s, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
+            tc_fence_after_sync();
+            uint32_t x[32];
+            tmem_ld_32(row + TM_AU + 32 * h, x);
+            uint16_t* op = &s.o[32 * h][v];
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float2 c1 = *reinterpret_cast<const float2*>(&q.c1[32 * h + 2 * i]), be = *reinterpret_cast<const float2*>(&q.beta[32 * h + 2 * i]);
-                const float2 xs = __fmul2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), make_float2(-fX, -fX));
-                const float2 bv = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(vv[i]), make_float2(fB, fB)), be);
-                split_h2(__ffma2_rn(c1, xs, bv), hi[i], lo[i]);
+                const float2 y = __fmul2_rn(__ffma2_rn(f2_of(x[2 * i], x[2 * i + 1]), both(MAT_DOWN), o[i]), both(of));
+                const uint32_t b = f2_to_bf16x2(y.x, y.y);
+                op[2 * i * VD] = uint16_t(b);
+                op[(2 * i + 1) * VD] = uint16_t(b >> 16);
+            }
+            tc_fence_before_sync();
+        }
+        if (c == nchunk) {
+            named_bar(1, CK_MAIN);
+            ck_store(&s.o[0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
+            break;
+        }
+        ck_wait(s, &s.ks_full, uint32_t(c) & 1u);
+        tc_fence_after_sync();
+        {                                                    // r = beta (v - e^G S k^), times 2^e
+            uint32_t x[32], hi[16], lo[16];
+            tmem_ld_32(row + TM_X + 32 * h, x);
+            const float2 up = both(pow2f(e));
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float4 c1 = *reinterpret_cast<const float4*>(&q.c1[32 * h + 2 * i]), be = *reinterpret_cast<const float4*>(&q.beta[32 * h + 2 * i]);
+                const float2 v0 = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(vv[i]), up), make_float2(be.x, be.y));
+                const float2 v1 = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(vv[i + 1]), up), make_float2(be.z, be.w));
+                split_h2(__ffma2_rn(make_float2(c1.x, c1.y), f2_of(x[2 * i], x[2 * i + 1]), v0), hi[i], lo[i]);
+                split_h2(__ffma2_rn(make_float2(c1.z, c1.w), f2_of(x[2 * i + 2], x[2 * i + 3]), v1), hi[i + 1], lo[i + 1]);
             }
             tmem_st_16(row + TM_PHI + 16 * h, hi);
             tmem_st_16(row + TM_PLO + 16 * h, lo);
@@ -550,41 +616,49 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         }
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
-        if (warp == 0) ck_wait(s, &s.ta_full[buf], ph);
         if (warp == 0) {                                     // u = T r
+            ck_wait(s, &s.ta_full[buf], ph);
             tc_fence_after_sync();
-            const uint32_t th = smem_u32(s.thi[buf]), tl = smem_u32(s.tlo[buf]);
+            const uint64_t th = ck_desc(smem_u32(s.thi[buf]), 16), tl = ck_desc(smem_u32(s.tlo[buf]), 16);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), ks > 0);
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, ck_desc(tl + ks * 32, 16), ck_idesc(64, false), 1u);
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PLO + 8 * ks, ck_desc(th + ks * 32, 16), ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_Y, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
             }
             umma_commit_if(el, &s.y_full);
         }
         __syncwarp();
-        float2 o[16];                                        // e^G S q^, in outputs' units
+        if (c > 0) ck_store(&s.o[0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
         ck_wait(s, &s.qs_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {
             uint32_t x[32];
             tmem_ld_32(row + TM_XQ + 32 * h, x);
-            const float f = P.scale * pow2f(-eS);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                o[i] = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1])), make_float2(f, f)),
-                                  *reinterpret_cast<const float2*>(&q.c2[32 * h + 2 * i]));
+            for (int i = 0; i < 16; i += 2) {
+                const float4 c2 = *reinterpret_cast<const float4*>(&q.c2[32 * h + 2 * i]);
+                o[i] = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), make_float2(c2.x, c2.y));
+                o[i + 1] = __fmul2_rn(f2_of(x[2 * i + 2], x[2 * i + 3]), make_float2(c2.z, c2.w));
+            }
         }
+        decay = q.decay;
+        plen = q.len;
+        of = P.scale * pow2f(-e);
         ck_wait(s, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {                                                    // u for A u (one piece), u e^{G_C - G} kr for the state (two)
             uint32_t y[32], un[16], hi[16], lo[16];
             tmem_ld_32(row + TM_Y + 32 * h, y);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 u = make_float2(__uint_as_float(y[2 * i]), __uint_as_float(y[2 * i + 1]));
-                un[i] = h2_bits(__floats2half2_rn(u.x * MAT_DOWN, u.y * MAT_DOWN));
-                split_h2(__fmul2_rn(u, *reinterpret_cast<const float2*>(&q.c3[32 * h + 2 * i])), hi[i], lo[i]);
+            for (int i = 0; i < 16; i += 2) {
+                const float4 c3 = *reinterpret_cast<const float4*>(&q.c3[32 * h + 2 * i]);
+                const float2 u0 = f2_of(y[2 * i], y[2 * i + 1]), u1 = f2_of(y[2 * i + 2], y[2 * i + 3]);
+                const float2 d0 = __fmul2_rn(u0, both(MAT_DOWN)), d1 = __fmul2_rn(u1, both(MAT_DOWN));
+                un[i] = h2_bits(__floats2half2_rn(d0.x, d0.y));
+                un[i + 1] = h2_bits(__floats2half2_rn(d1.x, d1.y));
+                split_h2(__fmul2_rn(u0, make_float2(c3.x, c3.y)), hi[i], lo[i]);
+                split_h2(__fmul2_rn(u1, make_float2(c3.z, c3.w)), hi[i + 1], lo[i + 1]);
             }
             tmem_st_16(row + TM_UOP + 16 * h, un);
             tmem_st_16(row + TM_PHI + 16 * h, hi);
@@ -595,37 +669,25 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         named_bar(1, CK_MAIN);
         if (warp == 0) {                                     // A u, then the chunk's part of the state
             tc_fence_after_sync();
-            const uint32_t am = smem_u32(s.amat[buf]);
+            const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16), kt = ck_desc(ti, 16384);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-                umma_f16_ts(el, tm + TM_AU, tm + TM_UOP + 8 * ks, ck_desc(am + ks * 32, 16), ck_idesc(64, false), ks > 0);
+            for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, tm + TM_AU, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), ks > 0);
             umma_commit_if(el, &s.au_full[buf]);
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) {
-                const uint64_t d = ck_desc(ti + ks * 2048, 16384);
-                umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, d, ck_idesc(128, true), ks > 0);
-                umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, d, ck_idesc(128, true), 1u);
+                umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
+                umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
             }
             umma_commit_if(el, &s.d_full);
         }
         __syncwarp();
-        decay = q.decay;
-        plen = q.len;
-        back = pow2f(-eB);
-        ck_wait(s, &s.au_full[buf], ph);
-        tc_fence_after_sync();
-        {
-            uint32_t x[32];
-            tmem_ld_32(row + TM_AU + 32 * h, x);
-            const float f = P.scale * back * MAT_DOWN;
-            uint16_t* op = &s.v[buf][32 * h][v];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) op[i * VD] = f_to_bf16(fmaf(__uint_as_float(x[i]), f, (i & 1) ? o[i >> 1].y : o[i >> 1].x));
-        }
     }
+    const float2 down = both(pow2f(-e));
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(S[2 * i].x, S[2 * i].y, S[2 * i + 1].x, S[2 * i + 1].y);
+    for (int i = 0; i < 16; ++i) {
+        const float2 a = __fmul2_rn(S[2 * i], down), b = __fmul2_rn(S[2 * i + 1], down);
+        *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
+    }
     if (warp == 0) umma_commit_if(el, &s.fin);
 }
 
@@ -666,6 +728,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P)
         reinterpret_cast<uint4*>(s.tlo)[i] = make_uint4(0u, 0u, 0u, 0u);
         reinterpret_cast<uint4*>(s.amat)[i] = make_uint4(0u, 0u, 0u, 0u);
     }
+    for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
     if (warp == 0) tmem_alloc(&s.tm, 512);
     fence_async_smem();
     tc_fence_before_sync();

@@ -73,12 +73,6 @@ __host__ __device__ inline size_t flush_smem_bytes(int L, int maxd, bool kda) {
 }
 
 // ---- warp-level tensor-core helpers (mma.sync path) ----
-__device__ __forceinline__ void mma_h_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                            uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 // (ldmatrix_x4_trans: lq_quant.cu, compiled ahead of this file in the same translation unit)
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], const void* smem_row) {
     const uint32_t addr = uint32_t(__cvta_generic_to_shared(smem_row));
