@@ -17,6 +17,7 @@
 // a power of two of its own, from bounds that hold whatever the inputs: |k^| <= 1, 0 <= beta <= 1 and decays <= 1 make the rule a
 // contraction, |r_t|, |u_t| / 2, |S| <= |S_0| + sum |v_t| =: B per row.  T is bounded by 1 for the same reason.  The products that
 // only reach the bf16 outputs (S q, A u) take one piece, 2^-12.
+#include <cuda.h>
 #include <stddef.h>
 
 #include "lq_tc.cuh"
@@ -65,20 +66,20 @@ struct alignas(16) PrepSmem {                                            // of o
 struct alignas(16) ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
-    unsigned char thi[2][8192], tlo[2][8192], amat[2][8192];
-    uint16_t v[2][CT][VD], o[CT][VD];                        // bf16 values, and outputs on their way out
+    unsigned char thi[2][8192], tlo[2][8192], amat[2][8192], v[2][16384];          // v: bf16, two blocks of 64 values by 64 rows
+    uint16_t o[CT][VD];                                      // outputs on their way out
     PrepSmem prep[2];
     ChunkScalars sc[2];
     float2 part[2][CK_MAIN];
-    uint64_t tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, fin;
+    uint64_t raw_full[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, fin;
     uint32_t tm;
     int dead;
 };
 
 static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
-                  offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 16 == 0 && offsetof(ChunkSmem, o) % 16 == 0 &&
+                  offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
                   offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(PrepSmem, tt) % 16 == 0 &&
-                  offsetof(PrepSmem, Gk) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, tile_full) % 8 == 0,
+                  offsetof(PrepSmem, Gk) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
               "vector accesses and swizzled tiles");
 
 // Waits like warp_wait_bounded; once one wait of the CTA has run out, all later ones of every warp return at once, so that the CTA
@@ -90,9 +91,6 @@ __device__ __forceinline__ void ck_wait(ChunkSmem& s, uint64_t* bar, uint32_t pa
     }
     s.dead = 1;
     atomicOr(&g_status, ST_CONSUMER_TIMEOUT);
-}
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 // exponent e with b 2^e in [2^13, 2^14), within what fp32 scaling can carry
@@ -120,32 +118,17 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float decay_between(float2 to, float2 from) { return ex2((to.x - from.x) + (to.y - from.y)); }
 __device__ __forceinline__ void prep_bar(int grp) { named_bar(2 + grp, CK_PREP); }
 
-// k and q rows of a chunk, as they come, into the places of the tile where their f16 form goes (zeros behind the chunk's last token),
-// and the rows of v; every thread converts what it has copied
-__device__ __forceinline__ void ck_fetch(unsigned char* tile, uint16_t* vbuf, const RuleParams& P, int hk, int hv, int64_t t0, int len, int w,
-                                         int lane) {
-    const int c = lane & 15, t1 = 32 * (w & 1) + (lane >> 4), tv = 2 * w + (lane >> 4);   // token of the thread's first piece
-    const uint16_t* src = P.mixed + (t0 + t1) * P.mixed_stride + ((w < 2 ? P.H : 0) + hk) * KD + 8 * c;
-    const uint16_t* vsrc = P.mixed + (t0 + tv) * P.mixed_stride + 2 * P.H * KD + hv * VD + 8 * c;
-    unsigned char* dst = tile + (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128;
-    uint16_t* vdst = vbuf + tv * VD + 8 * c;
-    const int64_t step = 2 * P.mixed_stride, vstep = 8 * P.mixed_stride;
-    if (len == CT) {
+// k, q and v rows of a chunk, as they come: boxes of 64 rows by 64 elements in the 128-byte swizzle, k and q where their f16 form goes.
+// Rows behind the chunk's last token belong to other sequences (or lie behind the tensor: zeros).
+constexpr uint32_t CK_RAW_BYTES = 6 * 8192;
+__device__ __forceinline__ void ck_fetch(ChunkSmem& s, const CUtensorMap* rows, int grp, int xk, int xq, int xv, int t0) {
+    mbar_arrive_expect_tx(&s.raw_full[grp], CK_RAW_BYTES);
 #pragma unroll
-        for (int i = 0; i < 16; ++i, src += step) cp_async16(dst + 256 * i + (((c & 7) ^ ((2 * i + (lane >> 4)) & 7)) << 4), src, 16u);
-#pragma unroll
-        for (int i = 0; i < 8; ++i, vsrc += vstep) cp_async16(vdst + 8 * i * VD, vsrc, 16u);
-    } else {
-        for (int i = 0; i < 16; ++i, src += step) {
-            const bool in = t1 + 2 * i < len;
-            cp_async16(dst + 256 * i + (((c & 7) ^ ((2 * i + (lane >> 4)) & 7)) << 4), in ? src : P.mixed, in ? 16u : 0u);
-        }
-        for (int i = 0; i < 8; ++i, vsrc += vstep) {
-            const bool in = tv + 8 * i < len;
-            cp_async16(vdst + 8 * i * VD, in ? vsrc : P.mixed, in ? 16u : 0u);
-        }
+    for (int b = 0; b < 2; ++b) {
+        tma_load_2d(s.tile[grp] + 16384 * b, rows, xk + 64 * b, t0, &s.raw_full[grp]);
+        tma_load_2d(s.tile[grp] + 16384 * b + 8192, rows, xq + 64 * b, t0, &s.raw_full[grp]);
+        tma_load_2d(s.v[grp] + 8192 * b, rows, xv + 64 * b, t0, &s.raw_full[grp]);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
 }
 // Sum of eight values over the sixteen lanes that share lane >> 4, eight shuffles: every exchange halves what a lane keeps.  Lane l
 // returns the total of value 4 (l >> 3 & 1) + 2 (l >> 2 & 1) + (l >> 1 & 1).
@@ -165,16 +148,23 @@ __device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
     float s = (up ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, up ? b[0] : b[1], 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
-__device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w, int lane) {
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+// Rows of k (warps 0 and 1) and q to f16, in place: a lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
+__device__ __forceinline__ void ck_convert(unsigned char* tile, unsigned char* v, float* rs, int len, int w, int lane) {
     const int c = lane & 15;
-    tile += (c >> 3) * 16384;
+    tile += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
+    if (len < CT) {                                          // rows of other sequences
+        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 16; ++i)
+            if (32 * (w & 1) + 2 * i + (lane >> 4) >= len) *reinterpret_cast<uint4*>(tile + 256 * i) = zero;
+        for (int i = lane + 32 * w; i < 1024; i += CK_PREP)
+            if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(v + 16 * i) = zero;
+    }
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
         uint4 x[8];
         float ss[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7));
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 2048 * hf + 256 * i);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 f0 = bf16x2_to_f2(x[i].x), f1 = bf16x2_to_f2(x[i].y), f2 = bf16x2_to_f2(x[i].z), f3 = bf16x2_to_f2(x[i].w);
@@ -198,7 +188,7 @@ __device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w
                 const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), make_float2(mi, mi));
                 h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(tile + ck_off(32 * w + 16 * hf + 2 * i + (lane >> 4), c & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(tile + 2048 * hf + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
 }
@@ -401,7 +391,7 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
     }
 }
 
-__device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
+__device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const CUtensorMap* rows, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
                                         int grp, int w, int lane) {
     const uint32_t el = elect_one();
     const int pt = 32 * w + lane;
@@ -416,10 +406,14 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, int h
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
         if (w == 3) ck_gates(ps, graw, n, ea, dtb, lane);
-        if (c >= 2) ck_wait(s, &s.main_done[grp], ph ^ 1u);
-        ck_fetch(tile, &s.v[grp][0][0], P, hk, hv, at, n, w, lane);
+        if (w == 0) {
+            if (c >= 2) ck_wait(s, &s.main_done[grp], ph ^ 1u);
+            if (el) ck_fetch(s, rows, grp, (P.H + hk) * KD, hk * KD, 2 * P.H * KD + hv * VD, int(at));
+            __syncwarp();
+        }
         if (w == 3 && c + 2 < nchunk) ck_load_gates(P, hv, at + 2 * CT, int(left - 2 * CT < CT ? left - 2 * CT : CT), lane, graw);
-        ck_convert(tile, w < 2 ? ps.kr : ps.qr, w, lane);
+        ck_wait(s, &s.raw_full[grp], ph);
+        ck_convert(tile, s.v[grp], w < 2 ? ps.kr : ps.qr, n, w, lane);
         fence_async_smem();
         tc_fence_before_sync();                              // (this group's last Gram matrix has been read)
         prep_bar(grp);
@@ -465,22 +459,22 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, int h
 }
 
 // ---- main warps -----------------------------------------------------------------------------------------------------------
-// outputs of a chunk from shared memory to global, by all main threads
-__device__ __forceinline__ void ck_store(const uint16_t* ob, const RuleParams& P, int hv, int64_t at, int len, int tid) {
-    const int r = tid >> 4, c = tid & 15;
-    uint16_t* op = P.o + ((at + r) * P.HV + hv) * VD + 8 * c;
-    const int64_t step = int64_t(16) * P.HV * VD;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (r + 16 * i < len) *reinterpret_cast<uint4*>(op) = *reinterpret_cast<const uint4*>(ob + (r + 16 * i) * VD + 8 * c);
-        op += step;
+// outputs of a chunk from shared memory to global: one bulk store, or row by row where the chunk is not full
+__device__ __forceinline__ void ck_store(const uint16_t (&ob)[CT][VD], const RuleParams& P, const CUtensorMap* outs, int hv, int64_t at, int len,
+                                         int tid, int warp, uint32_t el) {
+    if (len == CT) {
+        if (warp == 4 && el) tma_store_2d(outs, ob, hv * VD, int(at));
+        __syncwarp();
+    } else {
+        for (int r = tid >> 4; r < len; r += CK_MAIN / 16)
+            *reinterpret_cast<uint4*>(P.o + ((at + r) * P.HV + hv) * VD + 8 * (tid & 15)) = *reinterpret_cast<const uint4*>(&ob[r][8 * (tid & 15)]);
     }
 }
 __device__ __forceinline__ float2 f2_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // Chunk c's outputs are finished while S k of chunk c + 1 is under way, and leave for memory while T r of it is.
-__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
+__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const CUtensorMap* outs, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
     const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
     const uint32_t el = elect_one();
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
@@ -503,11 +497,13 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         float va = 0.f;
         if (c < nchunk) {
             ck_wait(s, &s.tile_full[buf], ph);
-            const uint16_t* vp = &s.v[buf][32 * h][v];
+            const unsigned char* vp = s.v[buf] + (v >> 6) * 8192 + 32 * h * 128 + 2 * (v & 7);
+            const int vc = (v >> 3) & 7;
             __nv_bfloat162 sum = __floats2bfloat162_rn(0.f, 0.f);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                vv[i] = uint32_t(vp[2 * i * VD]) | (uint32_t(vp[(2 * i + 1) * VD]) << 16);
+                vv[i] = uint32_t(*reinterpret_cast<const uint16_t*>(vp + 2 * i * 128 + ((vc ^ (2 * i & 7)) << 4))) |
+                        uint32_t(*reinterpret_cast<const uint16_t*>(vp + (2 * i + 1) * 128 + ((vc ^ ((2 * i + 1) & 7)) << 4))) << 16;
                 const uint32_t a = vv[i] & 0x7fff7fffu;
                 sum = __hadd2(sum, *reinterpret_cast<const __nv_bfloat162*>(&a));
             }
@@ -536,6 +532,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             for (int i = 4; i < 32; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
             n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
             s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
+            if (warp == 4) bulk_wait_read();                 // (the outputs two chunks ago have left their buffer)
             tc_fence_before_sync();
             named_bar(1, CK_MAIN);
             const float2 other = s.part[buf][tid ^ 128];
@@ -576,6 +573,10 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             umma_commit_if(el, &s.qs_full);
         }
         __syncwarp();
+        if (c == nchunk) {                                   // (no norm here: wait for the buffer of the outputs alone)
+            if (warp == 4) bulk_wait_read();
+            named_bar(1, CK_MAIN);
+        }
         if (c > 0) {                                         // outputs of the chunk before
             ck_wait(s, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
             tc_fence_after_sync();
@@ -589,11 +590,12 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                 op[2 * i * VD] = uint16_t(b);
                 op[(2 * i + 1) * VD] = uint16_t(b >> 16);
             }
+            fence_async_smem();
             tc_fence_before_sync();
         }
         if (c == nchunk) {
             named_bar(1, CK_MAIN);
-            ck_store(&s.o[0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
+            ck_store(s.o, P, outs, hv, t0 + int64_t(c - 1) * CT, plen, tid, warp, el);
             break;
         }
         ck_wait(s, &s.ks_full, uint32_t(c) & 1u);
@@ -629,7 +631,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             umma_commit_if(el, &s.y_full);
         }
         __syncwarp();
-        if (c > 0) ck_store(&s.o[0][0], P, hv, t0 + int64_t(c - 1) * CT, plen, tid);
+        if (c > 0) ck_store(s.o, P, outs, hv, t0 + int64_t(c - 1) * CT, plen, tid, warp, el);
         ck_wait(s, &s.qs_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {
@@ -689,15 +691,18 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
     }
     if (warp == 0) umma_commit_if(el, &s.fin);
+    if (warp == 4) bulk_wait_all();
 }
 
-__global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P) {
+__global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P, const __grid_constant__ CUtensorMap rows,
+                                                                   const __grid_constant__ CUtensorMap outs) {
     extern __shared__ __align__(128) unsigned char rule_smem[];
     ChunkSmem& s = *reinterpret_cast<ChunkSmem*>(rule_smem + ((1024u - (smem_u32(rule_smem) & 1023u)) & 1023u));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
+            mbar_init(&s.raw_full[i], 1);
             mbar_init(&s.tile_full[i], 1);
             mbar_init(&s.ta_full[i], 1);
             mbar_init(&s.main_done[i], CK_MAIN / 32);
@@ -739,10 +744,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P)
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
     if (uw >= CK_MAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
-        ck_prep(s, P, hk, hv, t0, len, nchunk, tm, (uw >> 2) & 1, uw & 3, lane);
+        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw >> 2) & 1, uw & 3, lane);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_MAIN_REGS));
-        ck_main(s, P, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
+        ck_main(s, P, &outs, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
     }
     ck_wait(s, &s.fin, 0);                                   // no tensor-core instruction is left
     tc_fence_before_sync();
@@ -768,12 +773,32 @@ static int launch_recurrent(const RuleParams& P, cudaStream_t st) {
     if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
     return finish_launch();
 }
+// Tensor map of a bf16 matrix [rows][cols] for boxes of 64 rows.
+static int encode_rows(CUtensorMap* m, const void* base, int64_t rows, int64_t cols, int64_t stride, uint32_t box, CUtensorMapSwizzle swizzle) {
+    using Encode = decltype(&cuTensorMapEncodeTiled);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess) f = nullptr;
+        return reinterpret_cast<Encode>(f);
+    }();
+    if (!encode) return LQ_ERR_LAUNCH;
+    const cuuint64_t dims[2] = {cuuint64_t(cols), cuuint64_t(rows)}, strides[1] = {cuuint64_t(stride) * 2};
+    const cuuint32_t boxes[2] = {box, CT}, ones[2] = {1, 1};
+    const CUresult e = encode(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return e == CUDA_SUCCESS ? LQ_OK : LQ_ERR_LAUNCH;
+}
 static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     constexpr size_t smem = sizeof(ChunkSmem) + 1024;
     static_assert(smem <= 227 * 1024, "the working set of a CTA");
-    int rc = ensure_smem((const void*)rule_chunk_kernel, smem);
+    if (P.T > 0x7fffffff) return LQ_ERR_RANGE;               // (coordinates of the tensor maps)
+    CUtensorMap rows, outs;
+    int rc = encode_rows(&rows, P.mixed, P.T, 2 * int64_t(P.H) * KD + int64_t(P.HV) * VD, P.mixed_stride, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (!rc) rc = encode_rows(&outs, P.o, P.T, int64_t(P.HV) * VD, int64_t(P.HV) * VD, VD, CU_TENSOR_MAP_SWIZZLE_NONE);
+    if (!rc) rc = ensure_smem((const void*)rule_chunk_kernel, smem);
     if (rc) return rc;
-    const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(P.N) * unsigned(P.HV), CK_THREADS, smem, st, P);
+    const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(P.N) * unsigned(P.HV), CK_THREADS, smem, st, P, rows, outs);
     if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
     return finish_launch();
 }
