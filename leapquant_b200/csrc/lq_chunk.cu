@@ -28,16 +28,19 @@ constexpr int RULE_SHORT = 8;                                // mean length from
 constexpr int CT = 64;                                       // tokens of a chunk
 // T and A lie within [-1, 1]; times 2^13 their small entries keep eleven bits down to 2^-27 as well
 constexpr float MAT_UP = 8192.f, MAT_DOWN = 1.f / 8192.f;
-// two warpgroups of main warps and two of prep warps; the main warps hold the state and take registers over from the others:
-// 256 * 168 + 256 * 88 = 512 * 128 = 65 536
-constexpr int CK_MAIN = 256, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP;
-constexpr int CK_MAIN_REGS = 168, CK_PREP_REGS = 88;
+#ifndef CK_MG
+#define CK_MG 2
+#endif
+constexpr int MG = CK_MG;                                    // threads that share a row of the state, each with
+constexpr int SP = 64 / MG, TP = 32 / MG;                    // SP pairs of its columns and TP pairs of a chunk's tokens
+constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP;
 
-// tensor memory: 512 columns.  D takes the place of X | XQ once both have been read, AU that of Y, and the operand of A u that of the
-// state's heads once S q is through.  G: Gram matrix of the even and of the odd chunks.
-constexpr uint32_t TM_SHI = 0, TM_SLO = 64, TM_X = 128, TM_XQ = 192, TM_D = 128, TM_PHI = 256, TM_PLO = 288, TM_Y = 320, TM_AU = 320,
-                   TM_UOP = 0;
-__host__ __device__ constexpr uint32_t tm_gram(int buf) { return buf ? 384u : 448u; }
+// Tensor memory, 512 columns.  D takes the place of X | XQ once both have been read.  The operand of A u takes that of S's heads once S q
+// is through.  Two regions of 64 change roles with every chunk: one has S's remainders and, after S k, the outputs (e^G S q^ put there,
+// A u added by the tensor cores), the other has u = T r -- and under the next chunk, whose remainders go there, the outputs stay.
+constexpr uint32_t TM_SHI = 0, TM_UOP = 0, TM_X = 128, TM_XQ = 192, TM_D = 128, TM_PHI = 256, TM_PLO = 288;
+__device__ __forceinline__ uint32_t tm_slo(int buf) { return buf ? 320u : 64u; }                    // and the outputs of the chunk
+__device__ __forceinline__ uint32_t tm_gram(int buf) { return buf ? 384u : 448u; }                  // of the even and of the odd chunks
 
 // f16 operands, fp32 accumulator; B with the reduction contiguous (K-major) or, for S += u k^T, the 128 key columns (MN-major)
 __host__ __device__ constexpr uint32_t ck_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24); }
@@ -52,7 +55,7 @@ __device__ __forceinline__ uint32_t ck_off(int row, int c) { return uint32_t(row
 struct alignas(16) ChunkScalars {                                        // of one chunk, by token
     float c1[CT];                                            // -beta e^{G_t} kr_t: takes S k to what is added to beta v
     float beta[CT];
-    float c2[CT];                                            // e^{G_t} qr_t
+    float c2[CT];                                            // e^{G_t} qr_t 2^13, the scale of A u
     float c3[CT];                                            // e^{G_C - G_t} kr_t 2^-13 (u comes with the 2^13 of T)
     float decay;                                             // e^{G_C}
     int len;                                                 // tokens of the chunk, 1 .. 64
@@ -60,7 +63,8 @@ struct alignas(16) ChunkScalars {                                        // of o
 struct alignas(16) PrepSmem {                                            // of one prep group
     float L[CT][CT + 4];                                     // times 2^13, like everything that becomes f16 on the way to T
     float tt[2][32][36];                                     // transposed inverses of the two diagonal blocks of 32, times 2^13
-    float2 G[CT], Gk[CT];                                    // log2 of the decay from the chunk's start, head and remainder; Gk: over kr
+    float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
+    float gh[CT], gl[CT];                                    // the two apart, minus log2 kr, negated: what is added to a later token's
     float kr[CT], qr[CT], ws[32], beta[CT];                  // ws: kr_s times the decay from s to token 31, for s < 32
 };
 struct alignas(16) ChunkSmem {
@@ -79,18 +83,26 @@ struct alignas(16) ChunkSmem {
 static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
                   offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
                   offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(PrepSmem, tt) % 16 == 0 &&
-                  offsetof(PrepSmem, Gk) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
+                  offsetof(PrepSmem, gh) % 16 == 0 && offsetof(PrepSmem, gl) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
               "vector accesses and swizzled tiles");
 
 // Waits like warp_wait_bounded; once one wait of the CTA has run out, all later ones of every warp return at once, so that the CTA
 // runs to its end (on rubbish) instead of waiting that long again and again.
 __device__ __forceinline__ void ck_wait(ChunkSmem& s, uint64_t* bar, uint32_t parity) {
-    for (uint32_t it = 0; it < WAIT_LIMIT; ++it) {
-        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return;
+#pragma unroll 1
+    for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
+        if (it == WAIT_LIMIT) s.dead = 1;
         if (it >= 64 && __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s.dead) != 0)) return;
     }
-    s.dead = 1;
-    atomicOr(&g_status, ST_CONSUMER_TIMEOUT);
+}
+// the same for waits that are long as a rule: sleeps between the tests, whose issue slots the working warps need
+__device__ __forceinline__ void ck_wait_long(ChunkSmem& s, uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
+        if (it == WAIT_LIMIT / 16) s.dead = 1;
+        if (it >= 64 && __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s.dead) != 0)) return;
+        __nanosleep(64);
+    }
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
 // exponent e with b 2^e in [2^13, 2^14), within what fp32 scaling can carry
@@ -99,6 +111,8 @@ __device__ __forceinline__ int scale_exponent(float b) {
     return e < -100 ? -100 : e > 100 ? 100 : e;
 }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ float2 f2_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 // two fp32 values as an f16 head, the leading eleven bits, and an f16 remainder: 22 bits
 __device__ __forceinline__ void split_h2(float2 x, uint32_t& hi, uint32_t& lo) {
     const float2 f = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u), __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
@@ -130,22 +144,25 @@ __device__ __forceinline__ void ck_fetch(ChunkSmem& s, const CUtensorMap* rows, 
         tma_load_2d(s.v[grp] + 8192 * b, rows, xv + 64 * b, t0, &s.raw_full[grp]);
     }
 }
-// Sum of eight values over the sixteen lanes that share lane >> 4, eight shuffles: every exchange halves what a lane keeps.  Lane l
-// returns the total of value 4 (l >> 3 & 1) + 2 (l >> 2 & 1) + (l >> 1 & 1).
+// the same rows into L2
+__device__ __forceinline__ void ck_prefetch(const CUtensorMap* rows, int xk, int xq, int xv, int t0) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+        tma_prefetch_2d(rows, xk + 64 * b, t0);
+        tma_prefetch_2d(rows, xq + 64 * b, t0);
+        tma_prefetch_2d(rows, xv + 64 * b, t0);
+    }
+}
+// Sum of eight values over the sixteen lanes that share lane >> 4: every exchange halves what a lane keeps.  Lane l returns the total of
+// value (l >> 1) & 7.
 __device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
+    const bool u8 = lane & 8, u4 = lane & 4, u2 = lane & 2;
     float a[4], b[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool up = lane & 8;
-        a[i] = (up ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[4 + i], 8);
-    }
+    for (int i = 0; i < 4; ++i) a[i] = (u8 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, u8 ? v[i] : v[4 + i], 8);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const bool up = lane & 4;
-        b[i] = (up ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, up ? a[i] : a[2 + i], 4);
-    }
-    const bool up = lane & 2;
-    float s = (up ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, up ? b[0] : b[1], 2);
+    for (int i = 0; i < 2; ++i) b[i] = (u4 ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, u4 ? a[i] : a[2 + i], 4);
+    float s = (u2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, u2 ? b[0] : b[1], 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
 // Rows of k (warps 0 and 1) and q to f16, in place: a lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
@@ -154,62 +171,64 @@ __device__ __forceinline__ void ck_convert(unsigned char* tile, unsigned char* v
     tile += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
     if (len < CT) {                                          // rows of other sequences
         const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
         for (int i = 0; i < 16; ++i)
             if (32 * (w & 1) + 2 * i + (lane >> 4) >= len) *reinterpret_cast<uint4*>(tile + 256 * i) = zero;
+#pragma unroll 1
         for (int i = lane + 32 * w; i < 1024; i += CK_PREP)
             if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(v + 16 * i) = zero;
     }
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll 1
+    for (int p = 0; p < 2; ++p) {
         uint4 x[8];
         float ss[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 2048 * hf + 256 * i);
+        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 2048 * p + 256 * i);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 f0 = bf16x2_to_f2(x[i].x), f1 = bf16x2_to_f2(x[i].y), f2 = bf16x2_to_f2(x[i].z), f3 = bf16x2_to_f2(x[i].w);
-            const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2));
-            ss[i] = (a.x + a.y) + (b.x + b.y);
+            const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2)), c2 = __fadd2_rn(a, b);
+            ss[i] = c2.x + c2.y;
         }
-        const float sum = fold8(ss, lane);                   // of piece (lane >> 1) & 7 with its three bits as fold8 says
+        const float sum = fold8(ss, lane);
         // the row times 2^-e has a norm in [1, 2); a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
         int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
         e = e < -60 ? -60 : e;
         const float m = sum <= 3.4e38f ? pow2f(-e) : 0.f;
-        const int mine = ((lane >> 3) & 1) * 4 + ((lane >> 2) & 1) * 2 + ((lane >> 1) & 1);
-        if (!(lane & 1)) rs[32 * (w & 1) + 16 * hf + 2 * mine + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
+        if (!(lane & 1)) rs[32 * (w & 1) + 16 * p + 2 * ((lane >> 1) & 7) + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | ((i >> 2) << 3) | (((i >> 1) & 1) << 2) | ((i & 1) << 1));
+            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | (i << 1));
             const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
             uint32_t h[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), make_float2(mi, mi));
+                const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), both(mi));
                 h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(tile + 2048 * hf + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(tile + 2048 * p + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
 }
-// raw gates of the tokens 2 l and 2 l + 1 of a chunk: a | b << 16
-__device__ __forceinline__ void ck_load_gates(const RuleParams& P, int hv, int64_t t0, int len, int lane, uint32_t (&g)[2]) {
+// decays and beta of the chunk, by one warp: lane l has the tokens 2 l and 2 l + 1; sums in fp64
+__device__ __forceinline__ void ck_gates(PrepSmem& s, const RuleParams& P, int hv, int64_t t0, int len, float ea, float dtb, int lane) {
+    double g[2];
+    float ar[2], br[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int t = 2 * lane + i;
-        g[i] = t < len ? uint32_t(__ldg(P.a + (t0 + t) * P.a_stride + hv)) | uint32_t(__ldg(P.b + (t0 + t) * P.b_stride + hv)) << 16 : 0u;
+        const int64_t t = t0 + (2 * lane + i < len ? 2 * lane + i : 0);
+        ar[i] = bf16_to_f(__ldg(P.a + t * P.a_stride + hv));
+        br[i] = bf16_to_f(__ldg(P.b + t * P.b_stride + hv));
     }
-}
-// decays and beta of the chunk, by one warp; sums in fp64
-__device__ __forceinline__ void ck_gates(PrepSmem& s, const uint32_t (&raw)[2], int len, float ea, float dtb, int lane) {
-    double g[2];
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
         const int t = 2 * lane + i;
         // a decay of 2^-200 leaves nothing in fp32; bounded, the differences stay finite
-        const float x = -ea * softplus_full(bf16lo(raw[i]) + dtb) * 1.4426950408889634f;
-        g[i] = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
-        s.beta[t] = t < len ? sigmoidf_(bf16hi(raw[i])) : 0.f;
+        const float x = -ea * softplus_full((i ? ar[1] : ar[0]) + dtb) * 1.4426950408889634f;
+        const double d = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
+        if (i) g[1] = d;
+        else g[0] = d;
+        s.beta[t] = t < len ? sigmoidf_(i ? br[1] : br[0]) : 0.f;
     }
     double sum = g[0] + g[1];
 #pragma unroll
@@ -223,6 +242,18 @@ __device__ __forceinline__ void ck_gates(PrepSmem& s, const uint32_t (&raw)[2], 
     s.G[2 * lane + 1] = make_float2(h1, float(sum - double(h1)));
 }
 
+// eight columns of a row of A or L to their places
+__device__ __forceinline__ void ck_put8(PrepSmem& s, unsigned char* amat, bool isq, int t, int c8, const float2 (&y)[4]) {
+    if (isq) {
+        uint32_t h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = h2_bits(__floats2half2_rn(y[j].x, y[j].y));
+        *reinterpret_cast<uint4*>(amat + ck_off(t, c8)) = make_uint4(h[0], h[1], h[2], h[3]);
+    } else {
+        *reinterpret_cast<float4*>(&s.L[t][8 * c8]) = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+        *reinterpret_cast<float4*>(&s.L[t][8 * c8 + 4]) = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
+    }
+}
 // Gram rows -> L (fp32, k rows) and A (f16 operand, q rows); a thread has a row.  Inside a diagonal block of 32 tokens the decay is
 // taken pair by pair; from the first block to the second in two steps over token 31, neither of which exceeds 1.
 __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32_t gram, int w, int lane) {
@@ -232,47 +263,35 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
     const float rowf = (isq ? s.qr[t] : s.kr[t] * s.beta[t]) * MAT_UP;
     gram += uint32_t(32 * w) << 16;
     if (blk == 1) {
-        uint32_t g[32];
-        tmem_ld_32(gram, g);
         const float f = rowf * decay_between(Gt, s.G[31]);
+#pragma unroll 1
+        for (int c8 = 0; c8 < 4; ++c8) {
+            uint32_t g[8];
+            float2 y[4];
+            tmem_ld_8(gram + 8 * c8, g);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float4 ws = *reinterpret_cast<const float4*>(&s.ws[4 * c]);
-            const float2 a = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(g[4 * c]), __uint_as_float(g[4 * c + 1])), make_float2(f, f)), make_float2(ws.x, ws.y));
-            const float2 b = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(g[4 * c + 2]), __uint_as_float(g[4 * c + 3])), make_float2(f, f)), make_float2(ws.z, ws.w));
-            if (isq) {
-                g[2 * c] = h2_bits(__floats2half2_rn(a.x, a.y));
-                g[2 * c + 1] = h2_bits(__floats2half2_rn(b.x, b.y));
-            } else {
-                *reinterpret_cast<float4*>(&s.L[t][4 * c]) = make_float4(a.x, a.y, b.x, b.y);
-            }
+            for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j], g[2 * j + 1]), both(f)), *reinterpret_cast<const float2*>(&s.ws[8 * c8 + 2 * j]));
+            ck_put8(s, amat, isq, t, c8, y);
         }
-        if (isq)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) *reinterpret_cast<uint4*>(amat + ck_off(t, c)) = make_uint4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
     }
-    uint32_t g[32];
-    tmem_ld_32(gram + 32 * blk, g);
-    const int last = isq ? lane : lane - 1;                  // last column of the block that counts
+    const int last = isq ? lane : lane - 1;                  // last column of the diagonal block that counts
+#pragma unroll 1
+    for (int c8 = 0; c8 < 4; ++c8) {
+        uint32_t g[8];
+        float2 y[4];
+        tmem_ld_8(gram + 32 * blk + 8 * c8, g);
 #pragma unroll
-    for (int c = 0; c < 32; c += 2) {
-        const float4 from = *reinterpret_cast<const float4*>(&s.Gk[32 * blk + c]);
-        const float2 d = __fmul2_rn(make_float2(rowf, rowf), make_float2(decay_between(Gt, make_float2(from.x, from.y)), decay_between(Gt, make_float2(from.z, from.w))));
-        const float2 y = __fmul2_rn(make_float2(__uint_as_float(g[c]), __uint_as_float(g[c + 1])), d);
-        g[c] = c <= last ? __float_as_uint(y.x) : 0u;
-        g[c + 1] = c < last ? __float_as_uint(y.y) : 0u;
-    }
-    if (isq) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            uint32_t h[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) h[j] = h2_bits(__floats2half2_rn(__uint_as_float(g[8 * c + 2 * j]), __uint_as_float(g[8 * c + 2 * j + 1])));
-            *reinterpret_cast<uint4*>(amat + ck_off(t, 4 * blk + c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int j = 0; j < 4; j += 2) {
+            const int c = 8 * c8 + 2 * j;
+            const float4 fh = *reinterpret_cast<const float4*>(&s.gh[32 * blk + c]), fl = *reinterpret_cast<const float4*>(&s.gl[32 * blk + c]);
+            const float2 d0 = __fadd2_rn(__fadd2_rn(both(Gt.x), make_float2(fh.x, fh.y)), __fadd2_rn(both(Gt.y), make_float2(fl.x, fl.y)));
+            const float2 d1 = __fadd2_rn(__fadd2_rn(both(Gt.x), make_float2(fh.z, fh.w)), __fadd2_rn(both(Gt.y), make_float2(fl.z, fl.w)));
+            const float2 z0 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j], g[2 * j + 1]), both(rowf)), make_float2(ex2(d0.x), ex2(d0.y)));
+            const float2 z1 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j + 2], g[2 * j + 3]), both(rowf)), make_float2(ex2(d1.x), ex2(d1.y)));
+            y[j] = make_float2(c <= last ? z0.x : 0.f, c < last ? z0.y : 0.f);
+            y[j + 1] = make_float2(c + 2 <= last ? z1.x : 0.f, c + 2 < last ? z1.y : 0.f);
         }
-    } else {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(&s.L[t][32 * blk + 4 * c]) = make_uint4(g[4 * c], g[4 * c + 1], g[4 * c + 2], g[4 * c + 3]);
+        ck_put8(s, amat, isq, t, 4 * blk + c8, y);
     }
 }
 struct Pieces { uint32_t hi, lo; };
@@ -354,33 +373,31 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
     prep_bar(grp);
     {
         const int n0 = 16 * (w & 1), i0 = 16 * (w >> 1);     // sixteen columns of T11, sixteen rows of T22
-        float X[4][4] = {};
-        Pieces a[4];
+        Pieces a1[2][4];
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            if (ks == 0 && n0) continue;                     // T11 is lower triangular
+        for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a[r] = pieces(lds2(&s.tt[0][n0 + gid + 8 * (r & 1)][16 * ks + 2 * tig + 8 * (r >> 1)]));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float* l = &s.L[32 + 8 * j + gid][16 * ks + 2 * tig];
-                mma_pieces(X[j], a, pieces(lds2(l)), pieces(lds2(l + 8)));
-            }
-        }
+            for (int r = 0; r < 4; ++r) a1[ks][r] = pieces(lds2(&s.tt[0][n0 + gid + 8 * (r & 1)][16 * ks + 2 * tig + 8 * (r >> 1)]));
         float d[2][4] = {};
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            if (ks == 1 && !i0) continue;                    // so is T22
+        for (int k2 = 0; k2 < 32; k2 += 16) {                // sixteen rows of L21 T11
+            if (k2 > i0) break;                              // T22 is lower triangular
+            Pieces b[2][2], a2[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a[r] = pieces(t_pair(s.tt[1], i0 + gid + 8 * (r & 1), 16 * ks + 2 * tig + 8 * (r >> 1)));
+            for (int j = 0; j < 2; ++j) {
+                float X[4] = {};
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                Pieces b[2];
+                for (int ks = 0; ks < 2; ++ks) {
+                    const float* l = &s.L[32 + k2 + 8 * j + gid][16 * ks + 2 * tig];
+                    mma_pieces(X, a1[ks], pieces(lds2(l)), pieces(lds2(l + 8)));
+                }
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    b[j] = pieces(__fmul2_rn(make_float2(X[2 * ks + j][2 * q], X[2 * ks + j][2 * q + 1]), make_float2(0x1p-16f, 0x1p-16f)));
-                mma_pieces(d[q], a, b[0], b[1]);
+                for (int q = 0; q < 2; ++q) b[q][j] = pieces(__fmul2_rn(make_float2(X[2 * q], X[2 * q + 1]), make_float2(0x1p-16f, 0x1p-16f)));
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a2[r] = pieces(t_pair(s.tt[1], i0 + gid + 8 * (r & 1), k2 + 2 * tig + 8 * (r >> 1)));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) mma_pieces(d[q], a2, b[q][0], b[q][1]);
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q)
@@ -399,20 +416,22 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
     ChunkScalars& q = s.sc[grp];
     unsigned char* tile = s.tile[grp];
     const float ea = expf(P.A_log[hv]), dtb = P.dt_bias[hv];
-    uint32_t graw[2] = {0u, 0u};
-    if (w == 3 && grp < nchunk) ck_load_gates(P, hv, t0 + grp * CT, int(len - grp * CT < CT ? len - grp * CT : CT), lane, graw);
+#pragma unroll 1
     for (int c = grp; c < nchunk; c += 2) {
         const uint32_t ph = uint32_t(c >> 1) & 1u;
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
-        if (w == 3) ck_gates(ps, graw, n, ea, dtb, lane);
+        if (w == 3) ck_gates(ps, P, hv, at, n, ea, dtb, lane);
         if (w == 0) {
-            if (c >= 2) ck_wait(s, &s.main_done[grp], ph ^ 1u);
-            if (el) ck_fetch(s, rows, grp, (P.H + hk) * KD, hk * KD, 2 * P.H * KD + hv * VD, int(at));
+            if (c >= 2) ck_wait_long(s, &s.main_done[grp], ph ^ 1u);
+            if (el) {
+                const int xk = (P.H + hk) * KD, xq = hk * KD, xv = 2 * P.H * KD + hv * VD;
+                ck_fetch(s, rows, grp, xk, xq, xv, int(at));
+                if (c + 2 < nchunk) ck_prefetch(rows, xk, xq, xv, int(at) + 2 * CT);
+            }
             __syncwarp();
         }
-        if (w == 3 && c + 2 < nchunk) ck_load_gates(P, hv, at + 2 * CT, int(left - 2 * CT < CT ? left - 2 * CT : CT), lane, graw);
-        ck_wait(s, &s.raw_full[grp], ph);
+        ck_wait_long(s, &s.raw_full[grp], ph);
         ck_convert(tile, s.v[grp], w < 2 ? ps.kr : ps.qr, n, w, lane);
         fence_async_smem();
         tc_fence_before_sync();                              // (this group's last Gram matrix has been read)
@@ -420,7 +439,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         if (w == 0) {
             tc_fence_after_sync();
             const uint64_t d0 = ck_desc(smem_u32(tile), 16);
-#pragma unroll
+#pragma unroll 2
             for (int ks = 0; ks < 8; ++ks) {
                 const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
                 umma_f16_ss(el, tm + tm_gram(grp), d, d, ck_idesc(64, false), ks > 0);
@@ -428,19 +447,24 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
             umma_commit_if(el, &s.g_full[grp]);
         }
         __syncwarp();
-        if (pt < 64) {
-            const float2 G = ps.G[pt], Gc = ps.G[CT - 1];
-            const float e = ex2(G.x + G.y), kr = ps.kr[pt], b = ps.beta[pt];
-            q.c1[pt] = -(b * e * kr);
-            q.beta[pt] = b;
-            q.c2[pt] = e * ps.qr[pt];
-            q.c3[pt] = decay_between(Gc, G) * kr * MAT_DOWN;
-            ps.Gk[pt] = make_float2(G.x, G.y - log2f(kr));
-            if (pt < 32) ps.ws[pt] = decay_between(ps.G[31], G) * kr;
-            if (pt == 0) {
+        const int tk = pt & 63;
+        const float2 G = ps.G[tk];
+        if (w >= 2) {                                        // for the main warps, and for the Gram rows
+            const float2 Gc = ps.G[CT - 1];
+            const float e = ex2(G.x + G.y), kr = ps.kr[tk], b = ps.beta[tk];
+            q.c1[tk] = -(b * e * kr);
+            q.beta[tk] = b;
+            q.c2[tk] = e * ps.qr[tk] * MAT_UP;
+            q.c3[tk] = decay_between(Gc, G) * kr * MAT_DOWN;
+            if (tk == 0) {
                 q.decay = ex2(Gc.x + Gc.y);
                 q.len = n;
             }
+        } else {
+            const float kr = ps.kr[tk];
+            ps.gh[tk] = -G.x;
+            ps.gl[tk] = log2f(kr) - G.y;
+            if (tk < 32) ps.ws[tk] = decay_between(ps.G[31], G) * kr;
         }
         prep_bar(grp);
         if (pt == 0) mbar_arrive(&s.tile_full[grp]);
@@ -466,58 +490,65 @@ __device__ __forceinline__ void ck_store(const uint16_t (&ob)[CT][VD], const Rul
         if (warp == 4 && el) tma_store_2d(outs, ob, hv * VD, int(at));
         __syncwarp();
     } else {
+#pragma unroll 1
         for (int r = tid >> 4; r < len; r += CK_MAIN / 16)
             *reinterpret_cast<uint4*>(P.o + ((at + r) * P.HV + hv) * VD + 8 * (tid & 15)) = *reinterpret_cast<const uint4*>(&ob[r][8 * (tid & 15)]);
     }
 }
-__device__ __forceinline__ float2 f2_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-
+// two neighbouring tokens' values (2 i and 2 i + 1 of eight) of a value dimension, in the swizzle of their tile
+__device__ __forceinline__ uint32_t v_pair(const unsigned char* p, int vc, int i) {
+    return uint32_t(*reinterpret_cast<const uint16_t*>(p + 2 * i * 128 + ((vc ^ (2 * i)) << 4))) |
+           uint32_t(*reinterpret_cast<const uint16_t*>(p + (2 * i + 1) * 128 + ((vc ^ (2 * i + 1)) << 4))) << 16;
+}
+__device__ __forceinline__ float2 v_two(const unsigned char* p, int vc, int i) {
+    return make_float2(bf16_to_f(*reinterpret_cast<const uint16_t*>(p + 2 * i * 128 + ((vc ^ (2 * i)) << 4))),
+                       bf16_to_f(*reinterpret_cast<const uint16_t*>(p + (2 * i + 1) * 128 + ((vc ^ (2 * i + 1)) << 4))));
+}
 // Chunk c's outputs are finished while S k of chunk c + 1 is under way, and leave for memory while T r of it is.
 __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const CUtensorMap* outs, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
     const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
     const uint32_t el = elect_one();
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
-    float2 S[32];                                            // S[v][64 h ..] times 2^e
-    float* Srow = Sg + v * KD + 64 * h;
+    float2 S[SP];                                            // S[v][2 SP h ..] times 2^e
+    float* Srow = Sg + v * KD + 2 * SP * h;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < SP / 2; ++i) {
         const float4 x = keep ? *reinterpret_cast<const float4*>(Srow + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
         S[2 * i] = make_float2(x.x, x.y);
         S[2 * i + 1] = make_float2(x.z, x.w);
     }
     int e = 0, plen = 0;
-    float decay = 0.f, of = 0.f;                             // of the chunk before: its decay, 2^-e scale of its outputs
-    float2 o[16];                                            // e^G S q^ of the chunk before, times 2^e
+    float decay = 0.f, of = 0.f;                             // of the chunk before: its decay, and what its outputs are multiplied with
+    const int vc = (v >> 3) & 7, voff = (v >> 6) * 8192 + 2 * TP * h * 128 + 2 * (v & 7);
+#pragma unroll 1
     for (int c = 0; c <= nchunk; ++c) {
         const int buf = c & 1;
-        const uint32_t ph = uint32_t(c >> 1) & 1u;
+        const uint32_t ph = uint32_t(c >> 1) & 1u, slo = tm_slo(buf), tmy = tm_slo(buf ^ 1);
         const ChunkScalars& q = s.sc[buf];
-        uint32_t vv[16];
+        const unsigned char* vp = s.v[buf] + voff;
         float va = 0.f;
         if (c < nchunk) {
             ck_wait(s, &s.tile_full[buf], ph);
-            const unsigned char* vp = s.v[buf] + (v >> 6) * 8192 + 32 * h * 128 + 2 * (v & 7);
-            const int vc = (v >> 3) & 7;
             __nv_bfloat162 sum = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll 1
+            for (int i0 = 0; i0 < TP; i0 += 4) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                vv[i] = uint32_t(*reinterpret_cast<const uint16_t*>(vp + 2 * i * 128 + ((vc ^ (2 * i & 7)) << 4))) |
-                        uint32_t(*reinterpret_cast<const uint16_t*>(vp + (2 * i + 1) * 128 + ((vc ^ ((2 * i + 1) & 7)) << 4))) << 16;
-                const uint32_t a = vv[i] & 0x7fff7fffu;
-                sum = __hadd2(sum, *reinterpret_cast<const __nv_bfloat162*>(&a));
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t a = v_pair(vp + 256 * i0, vc, i) & 0x7fff7fffu;
+                    sum = __hadd2(sum, *reinterpret_cast<const __nv_bfloat162*>(&a));
+                }
             }
-            va = (__low2float(sum) + __high2float(sum)) * 1.0625f;       // sixteen roundings to 8 bits: not below the sum of |v|
+            va = (__low2float(sum) + __high2float(sum)) * 1.0625f;       // a few roundings to 8 bits: not below the sum of |v|
         }
         if (c > 0) {                                         // the state behind the chunk before
             ck_wait(s, &s.d_full, uint32_t(c - 1) & 1u);
             tc_fence_after_sync();
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                uint32_t r[32];
-                tmem_ld_32(row + TM_D + 64 * h + 32 * p, r);
+            for (int p = 0; p < SP / 8; ++p) {
+                uint32_t r[16];
+                tmem_ld_16(row + TM_D + 2 * SP * h + 16 * p, r);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) S[16 * p + i] = __ffma2_rn(S[16 * p + i], both(decay), f2_of(r[2 * i], r[2 * i + 1]));
+                for (int i = 0; i < 8; ++i) S[8 * p + i] = __ffma2_rn(S[8 * p + i], both(decay), f2_of(r[2 * i], r[2 * i + 1]));
             }
             // every product of that chunk is through, and its scalars and values have been read: its buffers are free
             if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
@@ -529,66 +560,79 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
 #pragma unroll
             for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
 #pragma unroll
-            for (int i = 4; i < 32; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
+            for (int i = 4; i < SP; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
             n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
             s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
             if (warp == 4) bulk_wait_read();                 // (the outputs two chunks ago have left their buffer)
             tc_fence_before_sync();
             named_bar(1, CK_MAIN);
-            const float2 other = s.part[buf][tid ^ 128];
-            const float bound = sqrtf(n2[0].x + n2[0].y + other.x) * pow2f(-e) + (va + other.y);
-            const int en = scale_exponent(bound), de = en - e;
-            const float2 up = both(pow2f(de < -126 ? -126 : de > 127 ? 127 : de));
-            e = en;
+            float sum2 = n2[0].x + n2[0].y, sumv = va;
+#pragma unroll
+            for (int g = 1; g < MG; ++g) {
+                const float2 other = s.part[buf][tid ^ (128 * g)];
+                sum2 += other.x;
+                sumv += other.y;
+            }
+            const float bound = sqrtf(sum2) * pow2f(-e) + sumv;
+            // (kept while the bound stays between 2^10 and 2^14)
+            const int en = scale_exponent(bound);
+            int de = en - e;
+            if (de >= 0 && de <= 3) de = 0;
+            if (__any_sync(0xffffffffu, de != 0)) {
+                const float2 up = both(pow2f(de < -126 ? -126 : de > 127 ? 127 : de));
+                e += de;
+#pragma unroll
+                for (int i = 0; i < SP; ++i) S[i] = __fmul2_rn(S[i], up);
+            }
             tc_fence_after_sync();
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-                uint32_t hi[16], lo[16];
+            for (int p = 0; p < SP / 8; ++p) {
+                uint32_t hi[8], lo[8];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    S[16 * p + i] = __fmul2_rn(S[16 * p + i], up);
-                    split_h2(S[16 * p + i], hi[i], lo[i]);
+                for (int i = 0; i < 8; ++i) {
+                    split_h2(S[8 * p + i], hi[i], lo[i]);
                 }
-                tmem_st_16(row + TM_SHI + 32 * h + 16 * p, hi);
-                tmem_st_16(row + TM_SLO + 32 * h + 16 * p, lo);
+                tmem_st_8(row + TM_SHI + SP * h + 8 * p, hi);
+                tmem_st_8(row + slo + SP * h + 8 * p, lo);
             }
             tmem_st_wait();
-            tc_fence_before_sync();
-            named_bar(1, CK_MAIN);
+        } else if (warp == 4) {
+            bulk_wait_read();
         }
+        tc_fence_before_sync();
+        named_bar(1, CK_MAIN);
         const uint32_t ti = smem_u32(s.tile[buf]);
         if (warp == 0 && c < nchunk) {                       // S k^T, then S q^T
             tc_fence_after_sync();
             const uint64_t d0 = ck_desc(ti, 16);
-#pragma unroll
+#pragma unroll 2
             for (int ks = 0; ks < 8; ++ks) {
                 const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
                 umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
-                umma_f16_ts(el, tm + TM_X, tm + TM_SLO + 8 * ks, d, ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + TM_X, tm + slo + 8 * ks, d, ck_idesc(64, false), 1u);
             }
             umma_commit_if(el, &s.ks_full);
-#pragma unroll
+#pragma unroll 2
             for (int ks = 0; ks < 8; ++ks)
                 umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, d0 + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
             umma_commit_if(el, &s.qs_full);
         }
         __syncwarp();
-        if (c == nchunk) {                                   // (no norm here: wait for the buffer of the outputs alone)
-            if (warp == 4) bulk_wait_read();
-            named_bar(1, CK_MAIN);
-        }
         if (c > 0) {                                         // outputs of the chunk before
             ck_wait(s, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
             tc_fence_after_sync();
-            uint32_t x[32];
-            tmem_ld_32(row + TM_AU + 32 * h, x);
-            uint16_t* op = &s.o[32 * h][v];
+#pragma unroll 1
+            for (int p = 0; p < TP / 8; ++p) {
+                uint32_t x[16];
+                tmem_ld_16(row + tmy + 2 * TP * h + 16 * p, x);
+                uint16_t* op = &s.o[2 * TP * h + 16 * p][v];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 y = __fmul2_rn(__ffma2_rn(f2_of(x[2 * i], x[2 * i + 1]), both(MAT_DOWN), o[i]), both(of));
-                const uint32_t b = f2_to_bf16x2(y.x, y.y);
-                op[2 * i * VD] = uint16_t(b);
-                op[(2 * i + 1) * VD] = uint16_t(b >> 16);
+                for (int i = 0; i < 8; ++i) {
+                    const float2 y = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), both(of));
+                    const uint32_t b = f2_to_bf16x2(y.x, y.y);
+                    op[2 * i * VD] = uint16_t(b);
+                    op[(2 * i + 1) * VD] = uint16_t(b >> 16);
+                }
             }
             fence_async_smem();
             tc_fence_before_sync();
@@ -601,19 +645,24 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
         ck_wait(s, &s.ks_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {                                                    // r = beta (v - e^G S k^), times 2^e
-            uint32_t x[32], hi[16], lo[16];
-            tmem_ld_32(row + TM_X + 32 * h, x);
             const float2 up = both(pow2f(e));
+#pragma unroll 1
+            for (int p = 0; p < TP / 8; ++p) {
+                uint32_t x[16], hi[8], lo[8];
+                tmem_ld_16(row + TM_X + 2 * TP * h + 16 * p, x);
+                const float *c1 = &q.c1[2 * TP * h + 16 * p], *be = &q.beta[2 * TP * h + 16 * p];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float4 c1 = *reinterpret_cast<const float4*>(&q.c1[32 * h + 2 * i]), be = *reinterpret_cast<const float4*>(&q.beta[32 * h + 2 * i]);
-                const float2 v0 = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(vv[i]), up), make_float2(be.x, be.y));
-                const float2 v1 = __fmul2_rn(__fmul2_rn(bf16x2_to_f2(vv[i + 1]), up), make_float2(be.z, be.w));
-                split_h2(__ffma2_rn(make_float2(c1.x, c1.y), f2_of(x[2 * i], x[2 * i + 1]), v0), hi[i], lo[i]);
-                split_h2(__ffma2_rn(make_float2(c1.z, c1.w), f2_of(x[2 * i + 2], x[2 * i + 3]), v1), hi[i + 1], lo[i + 1]);
+                for (int i = 0; i < 8; i += 2) {
+                    const float4 cc = *reinterpret_cast<const float4*>(c1 + 2 * i), bb = *reinterpret_cast<const float4*>(be + 2 * i);
+                    const unsigned char* vi = vp + 2048 * p + 1024 * (i >> 2);
+                    const float2 v0 = __fmul2_rn(__fmul2_rn(v_two(vi, vc, i & 3), up), make_float2(bb.x, bb.y));
+                    const float2 v1 = __fmul2_rn(__fmul2_rn(v_two(vi, vc, (i & 3) + 1), up), make_float2(bb.z, bb.w));
+                    split_h2(__ffma2_rn(make_float2(cc.x, cc.y), f2_of(x[2 * i], x[2 * i + 1]), v0), hi[i], lo[i]);
+                    split_h2(__ffma2_rn(make_float2(cc.z, cc.w), f2_of(x[2 * i + 2], x[2 * i + 3]), v1), hi[i + 1], lo[i + 1]);
+                }
+                tmem_st_8(row + TM_PHI + TP * h + 8 * p, hi);
+                tmem_st_8(row + TM_PLO + TP * h + 8 * p, lo);
             }
-            tmem_st_16(row + TM_PHI + 16 * h, hi);
-            tmem_st_16(row + TM_PLO + 16 * h, lo);
             tmem_st_wait();
         }
         tc_fence_before_sync();
@@ -622,11 +671,11 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
             ck_wait(s, &s.ta_full[buf], ph);
             tc_fence_after_sync();
             const uint64_t th = ck_desc(smem_u32(s.thi[buf]), 16), tl = ck_desc(smem_u32(s.tlo[buf]), 16);
-#pragma unroll
+#pragma unroll 1
             for (int ks = 0; ks < 4; ++ks) {
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
-                umma_f16_ts(el, tm + TM_Y, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + tmy, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
+                umma_f16_ts(el, tm + tmy, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
+                umma_f16_ts(el, tm + tmy, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
             }
             umma_commit_if(el, &s.y_full);
         }
@@ -634,48 +683,57 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
         if (c > 0) ck_store(s.o, P, outs, hv, t0 + int64_t(c - 1) * CT, plen, tid, warp, el);
         ck_wait(s, &s.qs_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
-        {
-            uint32_t x[32];
-            tmem_ld_32(row + TM_XQ + 32 * h, x);
+#pragma unroll 1
+        for (int p = 0; p < TP / 8; ++p) {                   // e^G S q^, for A u to be added to
+            uint32_t x[16];
+            tmem_ld_16(row + TM_XQ + 2 * TP * h + 16 * p, x);
+            const float* c2 = &q.c2[2 * TP * h + 16 * p];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float4 c2 = *reinterpret_cast<const float4*>(&q.c2[32 * h + 2 * i]);
-                o[i] = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), make_float2(c2.x, c2.y));
-                o[i + 1] = __fmul2_rn(f2_of(x[2 * i + 2], x[2 * i + 3]), make_float2(c2.z, c2.w));
+            for (int i = 0; i < 8; i += 2) {
+                const float4 cc = *reinterpret_cast<const float4*>(c2 + 2 * i);
+                const float2 a = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), make_float2(cc.x, cc.y));
+                const float2 b = __fmul2_rn(f2_of(x[2 * i + 2], x[2 * i + 3]), make_float2(cc.z, cc.w));
+                x[2 * i] = __float_as_uint(a.x);
+                x[2 * i + 1] = __float_as_uint(a.y);
+                x[2 * i + 2] = __float_as_uint(b.x);
+                x[2 * i + 3] = __float_as_uint(b.y);
             }
+            tmem_st_16(row + slo + 2 * TP * h + 16 * p, x);
         }
         decay = q.decay;
         plen = q.len;
-        of = P.scale * pow2f(-e);
+        of = P.scale * pow2f(-e) * MAT_DOWN;
         ck_wait(s, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
-        {                                                    // u for A u (one piece), u e^{G_C - G} kr for the state (two)
-            uint32_t y[32], un[16], hi[16], lo[16];
-            tmem_ld_32(row + TM_Y + 32 * h, y);
+#pragma unroll 1
+        for (int p = 0; p < TP / 8; ++p) {                   // u for A u (one piece), u e^{G_C - G} kr for the state (two)
+            uint32_t y[16], un[8], hi[8], lo[8];
+            tmem_ld_16(row + tmy + 2 * TP * h + 16 * p, y);
+            const float* c3 = &q.c3[2 * TP * h + 16 * p];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                const float4 c3 = *reinterpret_cast<const float4*>(&q.c3[32 * h + 2 * i]);
+            for (int i = 0; i < 8; i += 2) {
+                const float4 cc = *reinterpret_cast<const float4*>(c3 + 2 * i);
                 const float2 u0 = f2_of(y[2 * i], y[2 * i + 1]), u1 = f2_of(y[2 * i + 2], y[2 * i + 3]);
                 const float2 d0 = __fmul2_rn(u0, both(MAT_DOWN)), d1 = __fmul2_rn(u1, both(MAT_DOWN));
                 un[i] = h2_bits(__floats2half2_rn(d0.x, d0.y));
                 un[i + 1] = h2_bits(__floats2half2_rn(d1.x, d1.y));
-                split_h2(__fmul2_rn(u0, make_float2(c3.x, c3.y)), hi[i], lo[i]);
-                split_h2(__fmul2_rn(u1, make_float2(c3.z, c3.w)), hi[i + 1], lo[i + 1]);
+                split_h2(__fmul2_rn(u0, make_float2(cc.x, cc.y)), hi[i], lo[i]);
+                split_h2(__fmul2_rn(u1, make_float2(cc.z, cc.w)), hi[i + 1], lo[i + 1]);
             }
-            tmem_st_16(row + TM_UOP + 16 * h, un);
-            tmem_st_16(row + TM_PHI + 16 * h, hi);
-            tmem_st_16(row + TM_PLO + 16 * h, lo);
-            tmem_st_wait();
+            tmem_st_8(row + TM_UOP + TP * h + 8 * p, un);
+            tmem_st_8(row + TM_PHI + TP * h + 8 * p, hi);
+            tmem_st_8(row + TM_PLO + TP * h + 8 * p, lo);
         }
+        tmem_st_wait();
         tc_fence_before_sync();
         named_bar(1, CK_MAIN);
         if (warp == 0) {                                     // A u, then the chunk's part of the state
             tc_fence_after_sync();
             const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16), kt = ck_desc(ti, 16384);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, tm + TM_AU, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), ks > 0);
+#pragma unroll 1
+            for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, tm + slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);
             umma_commit_if(el, &s.au_full[buf]);
-#pragma unroll
+#pragma unroll 1
             for (int ks = 0; ks < 4; ++ks) {
                 umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
                 umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
@@ -686,7 +744,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
     }
     const float2 down = both(pow2f(-e));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < SP / 2; ++i) {
         const float2 a = __fmul2_rn(S[2 * i], down), b = __fmul2_rn(S[2 * i + 1], down);
         *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
     }
@@ -724,15 +782,18 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     if (len == 0) return;
     const int slot = P.idx[n];
     if (slot <= 0 || slot >= P.NS || !first_of_slot(P.idx, n, slot, lane)) {       // padding: zeros, and no state
+#pragma unroll 1
         for (int64_t i = tid; i < len * (VD / 8); i += CK_THREADS)
             *reinterpret_cast<uint4*>(P.o + ((t0 + i / (VD / 8)) * P.HV + hv) * VD + 8 * (i % (VD / 8))) = make_uint4(0u, 0u, 0u, 0u);
         return;
     }
+#pragma unroll 1
     for (int i = tid; i < 2 * 8192 / 16; i += CK_THREADS) {                        // the upper right blocks of T and A stay zero
         reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);
         reinterpret_cast<uint4*>(s.tlo)[i] = make_uint4(0u, 0u, 0u, 0u);
         reinterpret_cast<uint4*>(s.amat)[i] = make_uint4(0u, 0u, 0u, 0u);
     }
+#pragma unroll 1
     for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
     if (warp == 0) tmem_alloc(&s.tm, 512);
     fence_async_smem();
@@ -743,16 +804,17 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     const int nchunk = int((len + CT - 1) / CT);
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
     if (uw >= CK_MAIN / 32) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
-        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw >> 2) & 1, uw & 3, lane);
+        if (MG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane);
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_MAIN_REGS));
+        if (MG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         ck_main(s, P, &outs, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
     }
     ck_wait(s, &s.fin, 0);                                   // no tensor-core instruction is left
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tm, 512);
+    if (tid == 0 && s.dead) atomicOr(&g_status, ST_CONSUMER_TIMEOUT);
 }
 
 static int rule_check(const lq_dims* d, const RuleParams& P) {
