@@ -33,7 +33,11 @@ constexpr float MAT_UP = 8192.f, MAT_DOWN = 1.f / 8192.f;
 #endif
 constexpr int MG = CK_MG;                                    // threads that share a row of the state, each with
 constexpr int SP = 64 / MG, TP = 32 / MG;                    // SP pairs of its columns and TP pairs of a chunk's tokens
-constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP;
+constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP + 32;
+// Registers: 17 warps get 96 each (five of them share a quarter of the SM).  The main warps take over what the prep warps give up,
+// 256 * 128 + 256 * 64 + 32 * 96 = 544 * 96; the launch looks that the kernel was built so, or they would wait for good.
+constexpr int CK_REGS = 96, CK_MAIN_REGS = 128, CK_PREP_REGS = 64;
+static_assert(CK_MAIN * CK_MAIN_REGS + 2 * CK_PREP * CK_PREP_REGS + 32 * CK_REGS <= CK_THREADS * CK_REGS, "register split");
 
 // Tensor memory, 512 columns.  D takes the place of X | XQ once both have been read.  The operand of A u takes that of S's heads once S q
 // is through.  Two regions of 64 change roles with every chunk: one has S's remainders and, after S k, the outputs (e^G S q^ put there,
@@ -60,11 +64,11 @@ struct alignas(16) ChunkScalars {                                        // of o
     float decay;                                             // e^{G_C}
     int len;                                                 // tokens of the chunk, 1 .. 64
 };
-struct alignas(16) PrepSmem {                                            // of one prep group
-    float L[CT][CT + 4];                                     // times 2^13, like everything that becomes f16 on the way to T
-    float tt[2][32][36];                                     // transposed inverses of the two diagonal blocks of 32, times 2^13
+struct alignas(16) PrepSmem {                                // of one prep group
+    float L[CT][CT + 4];                                     // times 2^13, like all that becomes f16 on the way to T
+    float tt[2][32][36];                                     // T^T of the two diagonal blocks of 32, times 2^13
     float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
-    float gh[CT], gl[CT];                                    // the two apart, minus log2 kr, negated: what is added to a later token's
+    float gh[CT], gl[CT];                                    // the two apart and negated
     float kr[CT], qr[CT], ws[32], beta[CT];                  // ws: kr_s times the decay from s to token 31, for s < 32
 };
 struct alignas(16) ChunkSmem {
@@ -74,34 +78,31 @@ struct alignas(16) ChunkSmem {
     uint16_t o[CT][VD];                                      // outputs on their way out
     PrepSmem prep[2];
     ChunkScalars sc[2];
-    float2 part[2][CK_MAIN];
-    uint64_t raw_full[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, fin;
+    uint16_t vsum[2][8][VD];                                 // bf16 sums of |v| of a value dimension, over every eighth token each
+    float part[2][CK_MAIN];
+    uint64_t raw_full[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
     uint32_t tm;
-    int dead;
+    int dead;                                                // a wait has run out
 };
 
 static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
                   offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
-                  offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(PrepSmem, tt) % 16 == 0 &&
+                  offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(ChunkSmem, vsum) % 16 == 0 &&
                   offsetof(PrepSmem, gh) % 16 == 0 && offsetof(PrepSmem, gl) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
               "vector accesses and swizzled tiles");
 
-// Waits like warp_wait_bounded; once one wait of the CTA has run out, all later ones of every warp return at once, so that the CTA
-// runs to its end (on rubbish) instead of waiting that long again and again.
-__device__ __forceinline__ void ck_wait(ChunkSmem& s, uint64_t* bar, uint32_t parity) {
+// Waits like warp_wait_bounded.  Once a wait of a warp has run out, its later ones test once and go on: the CTA runs to its end, on
+// rubbish, and reports.  SLEEP: waits that are long as a rule leave the issue slots to the warps that work.
+template <bool SLEEP = false>
+__device__ __forceinline__ void ck_wait(int& patience, uint64_t* bar, uint32_t parity) {
+    int left = patience;
 #pragma unroll 1
-    for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
-        if (it == WAIT_LIMIT) s.dead = 1;
-        if (it >= 64 && __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s.dead) != 0)) return;
-    }
-}
-// the same for waits that are long as a rule: sleeps between the tests, whose issue slots the working warps need
-__device__ __forceinline__ void ck_wait_long(ChunkSmem& s, uint64_t* bar, uint32_t parity) {
-#pragma unroll 1
-    for (uint32_t it = 0; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++it) {
-        if (it == WAIT_LIMIT / 16) s.dead = 1;
-        if (it >= 64 && __any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s.dead) != 0)) return;
-        __nanosleep(64);
+    while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        if (--left < 0) {
+            patience = 0;
+            break;
+        }
+        if (SLEEP) __nanosleep(64);
     }
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
@@ -110,14 +111,16 @@ __device__ __forceinline__ int scale_exponent(float b) {
     const int e = 140 - int((__float_as_uint(b) >> 23) & 255u);
     return e < -100 ? -100 : e > 100 ? 100 : e;
 }
+__device__ __forceinline__ uint32_t b2_bits(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ float2 f2_of(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-// two fp32 values as an f16 head, the leading eleven bits, and an f16 remainder: 22 bits
+// two fp32 values as an f16 head and an f16 remainder: 22 bits.  (Two conversions there and one back, 6.5 cycles a pair; a head cut out
+// with AND keeps the integer pipe busy for 9.)
 __device__ __forceinline__ void split_h2(float2 x, uint32_t& hi, uint32_t& lo) {
-    const float2 f = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffffe000u), __uint_as_float(__float_as_uint(x.y) & 0xffffe000u));
-    hi = h2_bits(__floats2half2_rn(f.x, f.y));
-    const float2 r = __fadd2_rn(x, make_float2(-f.x, -f.y));
+    const __half2 h = __floats2half2_rn(x.x, x.y);
+    const float2 f = __half22float2(h), r = __fadd2_rn(x, make_float2(-f.x, -f.y));
+    hi = h2_bits(h);
     lo = h2_bits(__floats2half2_rn(r.x, r.y));
 }
 
@@ -144,61 +147,64 @@ __device__ __forceinline__ void ck_fetch(ChunkSmem& s, const CUtensorMap* rows, 
         tma_load_2d(s.v[grp] + 8192 * b, rows, xv + 64 * b, t0, &s.raw_full[grp]);
     }
 }
-// the same rows into L2
-__device__ __forceinline__ void ck_prefetch(const CUtensorMap* rows, int xk, int xq, int xv, int t0) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-        tma_prefetch_2d(rows, xk + 64 * b, t0);
-        tma_prefetch_2d(rows, xq + 64 * b, t0);
-        tma_prefetch_2d(rows, xv + 64 * b, t0);
-    }
-}
-// Sum of eight values over the sixteen lanes that share lane >> 4: every exchange halves what a lane keeps.  Lane l returns the total of
-// value (l >> 1) & 7.
-__device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
-    const bool u8 = lane & 8, u4 = lane & 4, u2 = lane & 2;
-    float a[4], b[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = (u8 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, u8 ? v[i] : v[4 + i], 8);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) b[i] = (u4 ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, u4 ? a[i] : a[2 + i], 4);
-    float s = (u2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, u2 ? b[0] : b[1], 2);
+// Sum of four values over the sixteen lanes that share lane >> 4: every exchange halves what a lane keeps.  Lane l returns the total of
+// value (l >> 2) & 3.
+__device__ __forceinline__ float fold4(const float (&v)[4], int lane) {
+    const bool u8 = lane & 8, u4 = lane & 4;
+    const float a = (u8 ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, u8 ? v[0] : v[2], 8);
+    const float b = (u8 ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, u8 ? v[1] : v[3], 8);
+    float s = (u4 ? b : a) + __shfl_xor_sync(0xffffffffu, u4 ? a : b, 4);
+    s += __shfl_xor_sync(0xffffffffu, s, 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
+// Sums of |v| over the tokens g, g + 8, ... of a chunk (g: this half of a warp), for a bound: bf16 will do, rounded up by the reader.  A
+// lane reads one 16-byte piece of the rows, the same eight values in all of them, since the swizzle goes by the row's number mod 8.
+__device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)[8][VD], int w, int lane) {
+    const int g = 2 * w + (lane >> 4), c = lane & 15;
+    v += (c >> 3) * 8192 + g * 128 + (c & 7) * 16;
+    __nv_bfloat162 sum[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j] = __floats2bfloat162_rn(0.f, 0.f);
+#pragma unroll 2
+    for (int i = 0; i < 8; ++i) {
+        const uint4 x = *reinterpret_cast<const uint4*>(v + 1024 * i);
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum[j] = __hadd2(sum[j], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&xw[j])));
+    }
+    *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3]));
+}
+// rows behind the chunk's last token, which belong to other sequences, become zeros
+__device__ __forceinline__ void ck_clear(unsigned char* tile, unsigned char* v, int len, int pt) {
+#pragma unroll 1
+    for (int i = pt; i < 6 * 512; i += CK_PREP)              // pieces of 16 bytes: six blocks of 64 rows
+        if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(i < 4 * 512 ? tile + 16 * i : v + 16 * (i - 4 * 512)) = make_uint4(0u, 0u, 0u, 0u);
+}
 // Rows of k (warps 0 and 1) and q to f16, in place: a lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
-__device__ __forceinline__ void ck_convert(unsigned char* tile, unsigned char* v, float* rs, int len, int w, int lane) {
+__device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w, int lane) {
     const int c = lane & 15;
     tile += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
-    if (len < CT) {                                          // rows of other sequences
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
-        for (int i = 0; i < 16; ++i)
-            if (32 * (w & 1) + 2 * i + (lane >> 4) >= len) *reinterpret_cast<uint4*>(tile + 256 * i) = zero;
-#pragma unroll 1
-        for (int i = lane + 32 * w; i < 1024; i += CK_PREP)
-            if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(v + 16 * i) = zero;
-    }
-#pragma unroll 1
-    for (int p = 0; p < 2; ++p) {
-        uint4 x[8];
-        float ss[8];
+    for (int p = 0; p < 4; ++p) {
+        uint4 x[4];
+        float ss[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 2048 * p + 256 * i);
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 1024 * p + 256 * i);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 4; ++i) {
             const float2 f0 = bf16x2_to_f2(x[i].x), f1 = bf16x2_to_f2(x[i].y), f2 = bf16x2_to_f2(x[i].z), f3 = bf16x2_to_f2(x[i].w);
             const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2)), c2 = __fadd2_rn(a, b);
             ss[i] = c2.x + c2.y;
         }
-        const float sum = fold8(ss, lane);
+        const float sum = fold4(ss, lane);
         // the row times 2^-e has a norm in [1, 2); a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
         int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
         e = e < -60 ? -60 : e;
         const float m = sum <= 3.4e38f ? pow2f(-e) : 0.f;
-        if (!(lane & 1)) rs[32 * (w & 1) + 16 * p + 2 * ((lane >> 1) & 7) + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
+        if (!(lane & 3)) rs[32 * (w & 1) + 8 * p + 2 * ((lane >> 2) & 3) + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | (i << 1));
+        for (int i = 0; i < 4; ++i) {
+            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | (i << 2));
             const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
             uint32_t h[4];
 #pragma unroll
@@ -206,29 +212,34 @@ __device__ __forceinline__ void ck_convert(unsigned char* tile, unsigned char* v
                 const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), both(mi));
                 h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(tile + 2048 * p + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(tile + 1024 * p + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
 }
+// log2(1 + e^x): with z = e^-|x| and r = z / (2 + z) <= 1/3, log(1 + z) = 2 (r + r^3/3 + r^5/5 + ...), the next term below 2^-24 of it
+__device__ __forceinline__ float softplus_log2(float x) {
+    const float z = ex2(-1.4426950408889634f * fabsf(x)), r = __fdividef(z, 2.0f + z), q = r * r;
+    float p = 1.0f / 15.0f;
+    p = fmaf(p, q, 1.0f / 13.0f);
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    p = fmaf(p, q, 1.0f);
+    return fmaf(2.0f * 1.4426950408889634f * r, p, x > 0.f ? x * 1.4426950408889634f : 0.f);
+}
 // decays and beta of the chunk, by one warp: lane l has the tokens 2 l and 2 l + 1; sums in fp64
-__device__ __forceinline__ void ck_gates(PrepSmem& s, const RuleParams& P, int hv, int64_t t0, int len, float ea, float dtb, int lane) {
+__device__ __forceinline__ void ck_gates(PrepSmem& s, const uint16_t* a, int64_t a_step, const uint16_t* b, int64_t b_step, int len, float ea,
+                                         float dtb, int lane) {
     double g[2];
-    float ar[2], br[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int64_t t = t0 + (2 * lane + i < len ? 2 * lane + i : 0);
-        ar[i] = bf16_to_f(__ldg(P.a + t * P.a_stride + hv));
-        br[i] = bf16_to_f(__ldg(P.b + t * P.b_stride + hv));
-    }
-#pragma unroll 1
-    for (int i = 0; i < 2; ++i) {
-        const int t = 2 * lane + i;
+        const int t = 2 * lane + i, u = t < len ? t : 0;
+        const float x = -ea * softplus_log2(bf16_to_f(__ldg(a + u * a_step)) + dtb), y = bf16_to_f(__ldg(b + u * b_step));
         // a decay of 2^-200 leaves nothing in fp32; bounded, the differences stay finite
-        const float x = -ea * softplus_full((i ? ar[1] : ar[0]) + dtb) * 1.4426950408889634f;
-        const double d = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
-        if (i) g[1] = d;
-        else g[0] = d;
-        s.beta[t] = t < len ? sigmoidf_(i ? br[1] : br[0]) : 0.f;
+        g[i] = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
+        s.beta[t] = t < len ? __fdividef(1.0f, 1.0f + ex2(-1.4426950408889634f * y)) : 0.f;
     }
     double sum = g[0] + g[1];
 #pragma unroll
@@ -286,8 +297,9 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
             const float4 fh = *reinterpret_cast<const float4*>(&s.gh[32 * blk + c]), fl = *reinterpret_cast<const float4*>(&s.gl[32 * blk + c]);
             const float2 d0 = __fadd2_rn(__fadd2_rn(both(Gt.x), make_float2(fh.x, fh.y)), __fadd2_rn(both(Gt.y), make_float2(fl.x, fl.y)));
             const float2 d1 = __fadd2_rn(__fadd2_rn(both(Gt.x), make_float2(fh.z, fh.w)), __fadd2_rn(both(Gt.y), make_float2(fl.z, fl.w)));
-            const float2 z0 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j], g[2 * j + 1]), both(rowf)), make_float2(ex2(d0.x), ex2(d0.y)));
-            const float2 z1 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j + 2], g[2 * j + 3]), both(rowf)), make_float2(ex2(d1.x), ex2(d1.y)));
+            const float4 kr = *reinterpret_cast<const float4*>(&s.kr[32 * blk + c]);
+            const float2 z0 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j], g[2 * j + 1]), __fmul2_rn(both(rowf), make_float2(kr.x, kr.y))), make_float2(ex2(d0.x), ex2(d0.y)));
+            const float2 z1 = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j + 2], g[2 * j + 3]), __fmul2_rn(both(rowf), make_float2(kr.z, kr.w))), make_float2(ex2(d1.x), ex2(d1.y)));
             y[j] = make_float2(c <= last ? z0.x : 0.f, c < last ? z0.y : 0.f);
             y[j + 1] = make_float2(c + 2 <= last ? z1.x : 0.f, c + 2 < last ? z1.y : 0.f);
         }
@@ -306,110 +318,103 @@ __device__ __forceinline__ void mma_pieces(float (&d)[4], const Pieces (&a)[4], 
     mma_h_16816(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.lo, b1.lo);
     mma_h_16816(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.hi, b1.hi);
 }
-__device__ __forceinline__ float2 lds2(const float* p) { return *reinterpret_cast<const float2*>(p); }
-// two neighbours of a row of T, which is kept transposed
-__device__ __forceinline__ float2 t_pair(const float (&tt)[32][36], int i, int n) { return make_float2(tt[n][i], tt[n + 1][i]); }
 __device__ __forceinline__ void put_t(unsigned char* thi, unsigned char* tlo, int t, int c, Pieces p) {
     const uint32_t off = ck_off(t, c >> 3) + 2 * (c & 7);
     *reinterpret_cast<uint32_t*>(thi + off) = p.hi;
     *reinterpret_cast<uint32_t*>(tlo + off) = p.lo;
 }
-// T = (I + L)^-1 in blocks: 16 x 16 by substitution (warp w has diagonal block w, a lane a column), then twice the lower left block
-// -T22 (L21 T11) of a square twice as large, on mma.sync.  The first product is taken transposed, (L21 T11)^T = T11^T L21^T: its
-// accumulators are then the B operand of the second as they are.  Scales: L and T times 2^13, their product back to 2^10 (a sum of 32).
+// T = (I + L)^-1 in blocks: 16 x 16 by substitution (warp w has diagonal block w, a lane a column of T, which is a row of T^T), then twice
+// the lower left block -T22 (L21 T11) of a square twice as large, on mma.sync.  The first product is taken transposed, (L21 T11)^T =
+// T11^T L21^T: its accumulators are then the B operand of the second as they are.  Scales: L and T times 2^13, their product back to
+// 2^10 (a sum of 32).  Loops rather than straight code: an SM's instruction cache holds 32 KB, and beyond that every instruction of the
+// kernel costs 2.7 cycles.
 __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsigned char* tlo, int grp, int w, int lane) {
     const int gid = lane >> 2, tig = lane & 3;
     {
         const int o = 16 * w, c = lane & 15;
-        float x[16];
+        float* tt = &s.tt[w >> 1][(o & 16) + c][o & 16];     // this column of T
+#pragma unroll 1
+        for (int b = 0; b < 16; b += 4) {
+            const float* l = &s.L[o + b][o];
+            float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+            for (int m = 0; m < b; m += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(tt + m);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float a = 0.f, b = 0.f;
-#pragma unroll
-            for (int m = 0; m < i; m += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(&s.L[o + i][o + m]);
-                a = fmaf(l.x, x[m], a);
-                if (m + 1 < i) b = fmaf(l.y, x[m + 1], b);
-                if (m + 2 < i) a = fmaf(l.z, x[m + 2], a);
-                if (m + 3 < i) b = fmaf(l.w, x[m + 3], b);
-            }
-            x[i] = fmaf(a + b, -MAT_DOWN, c == i ? MAT_UP : 0.f);
-        }
-        if (lane < 16)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<float4*>(&s.tt[w >> 1][(o & 16) + c][(o & 16) + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-    }
-    prep_bar(grp);
-    {
-        const int sq = w >> 1, nt = w & 1, o = 32 * sq;      // the square of 32, and which eight of its first sixteen columns
-        const float (&tt)[32][36] = s.tt[sq];
-        float X[2][4] = {};
-        Pieces a[4], wb[2];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = pieces(lds2(&tt[gid + 8 * (r & 1)][2 * tig + 8 * (r >> 1)]));
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float* l = &s.L[o + 16 + 8 * j + gid][o + 2 * tig];
-            mma_pieces(X[j], a, pieces(lds2(l)), pieces(lds2(l + 8)));
-            const float2 y = nt ? make_float2(X[j][2], X[j][3]) : make_float2(X[j][0], X[j][1]);
-            wb[j] = pieces(__fmul2_rn(y, make_float2(0x1p-16f, 0x1p-16f)));
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) a[r] = pieces(t_pair(tt, 16 + gid + 8 * (r & 1), 16 + 2 * tig + 8 * (r >> 1)));
-        float d[4] = {};
-        mma_pieces(d, a, wb[0], wb[1]);
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int i = gid + 8 * r, n = 8 * nt + 2 * tig;
-            const float2 y = __fmul2_rn(make_float2(d[2 * r], d[2 * r + 1]), make_float2(-0x1p-10f, -0x1p-10f));
-            put_t(thi, tlo, o + 16 + i, o + n, pieces(y));
-            put_t(thi, tlo, o + 16 + i, o + 16 + n, nt ? a[2 + r] : a[r]);
-            put_t(thi, tlo, o + i, o + n, pieces(t_pair(tt, i, n)));
-            s.tt[sq][n][16 + i] = y.x;
-            s.tt[sq][n + 1][16 + i] = y.y;
-        }
-    }
-    prep_bar(grp);
-    {
-        const int n0 = 16 * (w & 1), i0 = 16 * (w >> 1);     // sixteen columns of T11, sixteen rows of T22
-        Pieces a1[2][4];
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) a1[ks][r] = pieces(lds2(&s.tt[0][n0 + gid + 8 * (r & 1)][16 * ks + 2 * tig + 8 * (r >> 1)]));
-        float d[2][4] = {};
-#pragma unroll
-        for (int k2 = 0; k2 < 32; k2 += 16) {                // sixteen rows of L21 T11
-            if (k2 > i0) break;                              // T22 is lower triangular
-            Pieces b[2][2], a2[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                float X[4] = {};
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    const float* l = &s.L[32 + k2 + 8 * j + gid][16 * ks + 2 * tig];
-                    mma_pieces(X, a1[ks], pieces(lds2(l)), pieces(lds2(l + 8)));
+                for (int r = 0; r < 4; ++r) {
+                    const float4 y = *reinterpret_cast<const float4*>(l + r * (CT + 4) + m);
+                    a[r] = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, a[r]))));
                 }
+            }
+            const float l10 = l[CT + 4 + b];
+            const float2 l2 = *reinterpret_cast<const float2*>(l + 2 * (CT + 4) + b);
+            const float4 l3 = *reinterpret_cast<const float4*>(l + 3 * (CT + 4) + b);
+            float4 x;
+            x.x = fmaf(a[0], -MAT_DOWN, c == b ? MAT_UP : 0.f);
+            x.y = fmaf(fmaf(l10, x.x, a[1]), -MAT_DOWN, c == b + 1 ? MAT_UP : 0.f);
+            x.z = fmaf(fmaf(l2.x, x.x, fmaf(l2.y, x.y, a[2])), -MAT_DOWN, c == b + 2 ? MAT_UP : 0.f);
+            x.w = fmaf(fmaf(l3.x, x.x, fmaf(l3.y, x.y, fmaf(l3.z, x.z, a[3]))), -MAT_DOWN, c == b + 3 ? MAT_UP : 0.f);
+            *reinterpret_cast<float4*>(tt + b) = x;          // (both halves of the warp: the same)
+        }
+        __syncwarp();
+        const float* d = &s.tt[w >> 1][(o & 16) + 2 * tig][(o & 16) + gid];
 #pragma unroll
-                for (int q = 0; q < 2; ++q) b[q][j] = pieces(__fmul2_rn(make_float2(X[2 * q], X[2 * q + 1]), make_float2(0x1p-16f, 0x1p-16f)));
+        for (int r = 0; r < 4; ++r) {
+            const int i = 8 * (r & 1), n = 8 * (r >> 1);
+            put_t(thi, tlo, o + gid + i, o + 2 * tig + n, pieces(make_float2(d[n * 36 + i], d[n * 36 + 36 + i])));
+        }
+    }
+#pragma unroll 1
+    for (int h = 16; h <= 32; h += 16) {
+        prep_bar(grp);
+        // of the square of 2 h at o: sixteen columns from n0 on, sixteen rows from i0 on (h = 16: two warps do the same)
+        const int o = h == 16 ? 32 * (w >> 1) : 0, n0 = h == 16 ? 0 : 16 * (w & 1), i0 = h == 16 ? 0 : 16 * (w >> 1);
+        float* t11 = &s.tt[h == 16 ? w >> 1 : 0][0][0];      // T^T of the two diagonal blocks, rows of 36
+        const float* t22 = h == 16 ? t11 + 16 * 36 + 16 : &s.tt[1][0][0];
+        const float* l21 = &s.L[o + h + gid][o + 2 * tig];
+        float d[2][4] = {};
+#pragma unroll 1
+        for (int k2 = 0; k2 <= i0; k2 += 16) {               // sixteen rows of L21 T11; T22 is lower triangular
+            float X[2][4] = {};
+            Pieces a[4], b[2][2];
+#pragma unroll 1
+            for (int ks = n0; ks < h; ks += 16) {            // so is T11
+                const float* ta = t11 + (n0 + gid) * 36 + ks + 2 * tig;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a[r] = pieces(*reinterpret_cast<const float2*>(ta + (r & 1) * 8 * 36 + (r >> 1) * 8));
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float* l = l21 + (k2 + 8 * j) * (CT + 4) + ks;
+                    mma_pieces(X[j], a, pieces(*reinterpret_cast<const float2*>(l)), pieces(*reinterpret_cast<const float2*>(l + 8)));
+                }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) a2[r] = pieces(t_pair(s.tt[1], i0 + gid + 8 * (r & 1), k2 + 2 * tig + 8 * (r >> 1)));
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) mma_pieces(d[q], a2, b[q][0], b[q][1]);
+                for (int j = 0; j < 2; ++j) b[q][j] = pieces(__fmul2_rn(make_float2(X[j][2 * q], X[j][2 * q + 1]), both(0x1p-16f)));
+            const float* tb = t22 + (k2 + 2 * tig) * 36 + i0 + gid;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) a[r] = pieces(make_float2(tb[(r >> 1) * 8 * 36 + (r & 1) * 8], tb[(r >> 1) * 8 * 36 + 36 + (r & 1) * 8]));
+#pragma unroll
+            for (int q = 0; q < 2; ++q) mma_pieces(d[q], a, b[q][0], b[q][1]);
         }
 #pragma unroll
         for (int q = 0; q < 2; ++q)
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
-                put_t(thi, tlo, 32 + i0 + gid + 8 * r, n0 + 8 * q + 2 * tig,
-                      pieces(__fmul2_rn(make_float2(d[q][2 * r], d[q][2 * r + 1]), make_float2(-0x1p-10f, -0x1p-10f))));
+            for (int r = 0; r < 2; ++r) {
+                const int i = i0 + gid + 8 * r, n = n0 + 8 * q + 2 * tig;
+                const float2 y = __fmul2_rn(make_float2(d[q][2 * r], d[q][2 * r + 1]), both(-0x1p-10f));
+                put_t(thi, tlo, o + h + i, o + n, pieces(y));
+                if (h == 16) {
+                    t11[n * 36 + 16 + i] = y.x;
+                    t11[n * 36 + 36 + 16 + i] = y.y;
+                }
+            }
     }
 }
 
 __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const CUtensorMap* rows, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
-                                        int grp, int w, int lane) {
+                                        int grp, int w, int lane, int& patience) {
     const uint32_t el = elect_one();
     const int pt = 32 * w + lane;
     PrepSmem& ps = s.prep[grp];
@@ -421,25 +426,26 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         const uint32_t ph = uint32_t(c >> 1) & 1u;
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
-        if (w == 3) ck_gates(ps, P, hv, at, n, ea, dtb, lane);
+        if (w == 3) ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
         if (w == 0) {
-            if (c >= 2) ck_wait_long(s, &s.main_done[grp], ph ^ 1u);
-            if (el) {
-                const int xk = (P.H + hk) * KD, xq = hk * KD, xv = 2 * P.H * KD + hv * VD;
-                ck_fetch(s, rows, grp, xk, xq, xv, int(at));
-                if (c + 2 < nchunk) ck_prefetch(rows, xk, xq, xv, int(at) + 2 * CT);
-            }
+            if (c >= 2) ck_wait<true>(patience, &s.main_done[grp], ph ^ 1u);
+            if (el) ck_fetch(s, rows, grp, (P.H + hk) * KD, hk * KD, 2 * P.H * KD + hv * VD, int(at));
             __syncwarp();
         }
-        ck_wait_long(s, &s.raw_full[grp], ph);
-        ck_convert(tile, s.v[grp], w < 2 ? ps.kr : ps.qr, n, w, lane);
+        ck_wait<true>(patience, &s.raw_full[grp], ph);
+        if (n < CT) {
+            ck_clear(tile, s.v[grp], n, pt);
+            prep_bar(grp);
+        }
+        ck_vsum(s.v[grp], s.vsum[grp], w, lane);
+        ck_convert(tile, w < 2 ? ps.kr : ps.qr, w, lane);
         fence_async_smem();
         tc_fence_before_sync();                              // (this group's last Gram matrix has been read)
         prep_bar(grp);
         if (w == 0) {
             tc_fence_after_sync();
             const uint64_t d0 = ck_desc(smem_u32(tile), 16);
-#pragma unroll 2
+#pragma unroll 1
             for (int ks = 0; ks < 8; ++ks) {
                 const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
                 umma_f16_ss(el, tm + tm_gram(grp), d, d, ck_idesc(64, false), ks > 0);
@@ -447,10 +453,9 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
             umma_commit_if(el, &s.g_full[grp]);
         }
         __syncwarp();
-        const int tk = pt & 63;
-        const float2 G = ps.G[tk];
-        if (w >= 2) {                                        // for the main warps, and for the Gram rows
-            const float2 Gc = ps.G[CT - 1];
+        if (w >= 2) {                                        // scalars for the main warps, which may then begin
+            const int tk = pt - 64;
+            const float2 G = ps.G[tk], Gc = ps.G[CT - 1];
             const float e = ex2(G.x + G.y), kr = ps.kr[tk], b = ps.beta[tk];
             q.c1[tk] = -(b * e * kr);
             q.beta[tk] = b;
@@ -460,16 +465,18 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
                 q.decay = ex2(Gc.x + Gc.y);
                 q.len = n;
             }
-        } else {
-            const float kr = ps.kr[tk];
-            ps.gh[tk] = -G.x;
-            ps.gl[tk] = log2f(kr) - G.y;
-            if (tk < 32) ps.ws[tk] = decay_between(ps.G[31], G) * kr;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.tile_full[grp]);
+        } else if (w == 1) {                                 // and for the Gram rows
+            const float2 g0 = ps.G[lane], g1 = ps.G[lane + 32];
+            ps.gh[lane] = -g0.x;
+            ps.gl[lane] = -g0.y;
+            ps.gh[lane + 32] = -g1.x;
+            ps.gl[lane + 32] = -g1.y;
+            ps.ws[lane] = decay_between(ps.G[31], g0) * ps.kr[lane];
         }
         prep_bar(grp);
-        if (pt == 0) mbar_arrive(&s.tile_full[grp]);
-        __syncwarp();
-        ck_wait(s, &s.g_full[grp], ph);
+        ck_wait(patience, &s.g_full[grp], ph);
         tc_fence_after_sync();
         ck_gram(ps, s.amat[grp], tm + tm_gram(grp), w, lane);
         prep_bar(grp);
@@ -483,31 +490,28 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
 }
 
 // ---- main warps -----------------------------------------------------------------------------------------------------------
-// outputs of a chunk from shared memory to global: one bulk store, or row by row where the chunk is not full
-__device__ __forceinline__ void ck_store(const uint16_t (&ob)[CT][VD], const RuleParams& P, const CUtensorMap* outs, int hv, int64_t at, int len,
-                                         int tid, int warp, uint32_t el) {
-    if (len == CT) {
-        if (warp == 4 && el) tma_store_2d(outs, ob, hv * VD, int(at));
-        __syncwarp();
-    } else {
-#pragma unroll 1
-        for (int r = tid >> 4; r < len; r += CK_MAIN / 16)
-            *reinterpret_cast<uint4*>(P.o + ((at + r) * P.HV + hv) * VD + 8 * (tid & 15)) = *reinterpret_cast<const uint4*>(&ob[r][8 * (tid & 15)]);
-    }
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 // two neighbouring tokens' values (2 i and 2 i + 1 of eight) of a value dimension, in the swizzle of their tile
-__device__ __forceinline__ uint32_t v_pair(const unsigned char* p, int vc, int i) {
-    return uint32_t(*reinterpret_cast<const uint16_t*>(p + 2 * i * 128 + ((vc ^ (2 * i)) << 4))) |
-           uint32_t(*reinterpret_cast<const uint16_t*>(p + (2 * i + 1) * 128 + ((vc ^ (2 * i + 1)) << 4))) << 16;
-}
 __device__ __forceinline__ float2 v_two(const unsigned char* p, int vc, int i) {
     return make_float2(bf16_to_f(*reinterpret_cast<const uint16_t*>(p + 2 * i * 128 + ((vc ^ (2 * i)) << 4))),
                        bf16_to_f(*reinterpret_cast<const uint16_t*>(p + (2 * i + 1) * 128 + ((vc ^ (2 * i + 1)) << 4))));
 }
+// a warp has written its part of an operand in tensor memory
+__device__ __forceinline__ void ck_ready(uint64_t* bar, int lane) {
+    tmem_st_wait();
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+    __syncwarp();
+}
 // Chunk c's outputs are finished while S k of chunk c + 1 is under way, and leave for memory while T r of it is.
-__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const CUtensorMap* outs, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid) {
+__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid,
+                                        int& patience) {
     const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
-    const uint32_t el = elect_one();
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
     float2 S[SP];                                            // S[v][2 SP h ..] times 2^e
     float* Srow = Sg + v * KD + 2 * SP * h;
@@ -528,20 +532,13 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
         const unsigned char* vp = s.v[buf] + voff;
         float va = 0.f;
         if (c < nchunk) {
-            ck_wait(s, &s.tile_full[buf], ph);
-            __nv_bfloat162 sum = __floats2bfloat162_rn(0.f, 0.f);
-#pragma unroll 1
-            for (int i0 = 0; i0 < TP; i0 += 4) {
+            ck_wait(patience, &s.tile_full[buf], ph);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t a = v_pair(vp + 256 * i0, vc, i) & 0x7fff7fffu;
-                    sum = __hadd2(sum, *reinterpret_cast<const __nv_bfloat162*>(&a));
-                }
-            }
-            va = (__low2float(sum) + __high2float(sum)) * 1.0625f;       // a few roundings to 8 bits: not below the sum of |v|
+            for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[buf][g][v]);
+            va *= 1.125f;                                    // (sums in bf16: not below the true one)
         }
         if (c > 0) {                                         // the state behind the chunk before
-            ck_wait(s, &s.d_full, uint32_t(c - 1) & 1u);
+            ck_wait(patience, &s.d_full, uint32_t(c - 1) & 1u);
             tc_fence_after_sync();
 #pragma unroll
             for (int p = 0; p < SP / 8; ++p) {
@@ -562,18 +559,13 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
 #pragma unroll
             for (int i = 4; i < SP; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
             n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
-            s.part[buf][tid] = make_float2(n2[0].x + n2[0].y, va);
-            if (warp == 4) bulk_wait_read();                 // (the outputs two chunks ago have left their buffer)
-            tc_fence_before_sync();
-            named_bar(1, CK_MAIN);
-            float sum2 = n2[0].x + n2[0].y, sumv = va;
+            const float mine = n2[0].x + n2[0].y;
+            s.part[buf][tid] = mine;
+            named_bar(4 + (warp & 3), 32 * MG);              // the warps that share these rows
+            float sum2 = mine;
 #pragma unroll
-            for (int g = 1; g < MG; ++g) {
-                const float2 other = s.part[buf][tid ^ (128 * g)];
-                sum2 += other.x;
-                sumv += other.y;
-            }
-            const float bound = sqrtf(sum2) * pow2f(-e) + sumv;
+            for (int g = 1; g < MG; ++g) sum2 += s.part[buf][tid ^ (128 * g)];
+            const float bound = fmaf(sqrt_approx(sum2), pow2f(-e), va);
             // (kept while the bound stays between 2^10 and 2^14)
             const int en = scale_exponent(bound);
             int de = en - e;
@@ -584,7 +576,6 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
 #pragma unroll
                 for (int i = 0; i < SP; ++i) S[i] = __fmul2_rn(S[i], up);
             }
-            tc_fence_after_sync();
 #pragma unroll
             for (int p = 0; p < SP / 8; ++p) {
                 uint32_t hi[8], lo[8];
@@ -595,39 +586,18 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
                 tmem_st_8(row + TM_SHI + SP * h + 8 * p, hi);
                 tmem_st_8(row + slo + SP * h + 8 * p, lo);
             }
-            tmem_st_wait();
-        } else if (warp == 4) {
-            bulk_wait_read();
+            ck_ready(&s.s_ready, lane);
         }
-        tc_fence_before_sync();
-        named_bar(1, CK_MAIN);
-        const uint32_t ti = smem_u32(s.tile[buf]);
-        if (warp == 0 && c < nchunk) {                       // S k^T, then S q^T
-            tc_fence_after_sync();
-            const uint64_t d0 = ck_desc(ti, 16);
-#pragma unroll 2
-            for (int ks = 0; ks < 8; ++ks) {
-                const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-                umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
-                umma_f16_ts(el, tm + TM_X, tm + slo + 8 * ks, d, ck_idesc(64, false), 1u);
-            }
-            umma_commit_if(el, &s.ks_full);
-#pragma unroll 2
-            for (int ks = 0; ks < 8; ++ks)
-                umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, d0 + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
-            umma_commit_if(el, &s.qs_full);
-        }
-        __syncwarp();
         if (c > 0) {                                         // outputs of the chunk before
-            ck_wait(s, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
+            ck_wait(patience, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
             tc_fence_after_sync();
 #pragma unroll 1
-            for (int p = 0; p < TP / 8; ++p) {
-                uint32_t x[16];
-                tmem_ld_16(row + tmy + 2 * TP * h + 16 * p, x);
-                uint16_t* op = &s.o[2 * TP * h + 16 * p][v];
+            for (int p = 0; p < TP / 4; ++p) {
+                uint32_t x[8];
+                tmem_ld_8(row + tmy + 2 * TP * h + 8 * p, x);
+                uint16_t* op = &s.o[2 * TP * h + 8 * p][v];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     const float2 y = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), both(of));
                     const uint32_t b = f2_to_bf16x2(y.x, y.y);
                     op[2 * i * VD] = uint16_t(b);
@@ -635,62 +605,46 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
                 }
             }
             fence_async_smem();
-            tc_fence_before_sync();
         }
         if (c == nchunk) {
             named_bar(1, CK_MAIN);
-            ck_store(s.o, P, outs, hv, t0 + int64_t(c - 1) * CT, plen, tid, warp, el);
+#pragma unroll 1
+            for (int r = tid >> 4; r < plen; r += CK_MAIN / 16)
+                *reinterpret_cast<uint4*>(P.o + ((t0 + int64_t(c - 1) * CT + r) * P.HV + hv) * VD + 8 * (tid & 15)) =
+                    *reinterpret_cast<const uint4*>(&s.o[r][8 * (tid & 15)]);
             break;
         }
-        ck_wait(s, &s.ks_full, uint32_t(c) & 1u);
+        ck_wait(patience, &s.ks_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {                                                    // r = beta (v - e^G S k^), times 2^e
             const float2 up = both(pow2f(e));
 #pragma unroll 1
-            for (int p = 0; p < TP / 8; ++p) {
-                uint32_t x[16], hi[8], lo[8];
-                tmem_ld_16(row + TM_X + 2 * TP * h + 16 * p, x);
-                const float *c1 = &q.c1[2 * TP * h + 16 * p], *be = &q.beta[2 * TP * h + 16 * p];
+            for (int p = 0; p < TP / 4; ++p) {
+                uint32_t x[8], hi[4], lo[4];
+                tmem_ld_8(row + TM_X + 2 * TP * h + 8 * p, x);
+                const float *c1 = &q.c1[2 * TP * h + 8 * p], *be = &q.beta[2 * TP * h + 8 * p];
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
+                for (int i = 0; i < 4; i += 2) {
                     const float4 cc = *reinterpret_cast<const float4*>(c1 + 2 * i), bb = *reinterpret_cast<const float4*>(be + 2 * i);
-                    const unsigned char* vi = vp + 2048 * p + 1024 * (i >> 2);
-                    const float2 v0 = __fmul2_rn(__fmul2_rn(v_two(vi, vc, i & 3), up), make_float2(bb.x, bb.y));
-                    const float2 v1 = __fmul2_rn(__fmul2_rn(v_two(vi, vc, (i & 3) + 1), up), make_float2(bb.z, bb.w));
+                    const float2 v0 = __fmul2_rn(v_two(vp + 1024 * p, vc, i), __fmul2_rn(up, make_float2(bb.x, bb.y)));
+                    const float2 v1 = __fmul2_rn(v_two(vp + 1024 * p, vc, i + 1), __fmul2_rn(up, make_float2(bb.z, bb.w)));
                     split_h2(__ffma2_rn(make_float2(cc.x, cc.y), f2_of(x[2 * i], x[2 * i + 1]), v0), hi[i], lo[i]);
                     split_h2(__ffma2_rn(make_float2(cc.z, cc.w), f2_of(x[2 * i + 2], x[2 * i + 3]), v1), hi[i + 1], lo[i + 1]);
                 }
-                tmem_st_8(row + TM_PHI + TP * h + 8 * p, hi);
-                tmem_st_8(row + TM_PLO + TP * h + 8 * p, lo);
+                tmem_st_4(row + TM_PHI + TP * h + 4 * p, hi);
+                tmem_st_4(row + TM_PLO + TP * h + 4 * p, lo);
             }
-            tmem_st_wait();
+            ck_ready(&s.r_ready, lane);
         }
-        tc_fence_before_sync();
-        named_bar(1, CK_MAIN);
-        if (warp == 0) {                                     // u = T r
-            ck_wait(s, &s.ta_full[buf], ph);
-            tc_fence_after_sync();
-            const uint64_t th = ck_desc(smem_u32(s.thi[buf]), 16), tl = ck_desc(smem_u32(s.tlo[buf]), 16);
-#pragma unroll 1
-            for (int ks = 0; ks < 4; ++ks) {
-                umma_f16_ts(el, tm + tmy, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
-                umma_f16_ts(el, tm + tmy, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
-                umma_f16_ts(el, tm + tmy, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
-            }
-            umma_commit_if(el, &s.y_full);
-        }
-        __syncwarp();
-        if (c > 0) ck_store(s.o, P, outs, hv, t0 + int64_t(c - 1) * CT, plen, tid, warp, el);
-        ck_wait(s, &s.qs_full, uint32_t(c) & 1u);
+        ck_wait(patience, &s.qs_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
 #pragma unroll 1
-        for (int p = 0; p < TP / 8; ++p) {                   // e^G S q^, for A u to be added to
-            uint32_t x[16];
-            tmem_ld_16(row + TM_XQ + 2 * TP * h + 16 * p, x);
-            const float* c2 = &q.c2[2 * TP * h + 16 * p];
+        for (int p = 0; p < TP / 4; ++p) {                   // e^G S q^, for A u to be added to
+            uint32_t x[8];
+            tmem_ld_8(row + TM_XQ + 2 * TP * h + 8 * p, x);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float4 cc = *reinterpret_cast<const float4*>(c2 + 2 * i);
+            for (int i = 0; i < 4; i += 2) {
+                const float4 cc = *reinterpret_cast<const float4*>(&q.c2[2 * TP * h + 8 * p + 2 * i]);
                 const float2 a = __fmul2_rn(f2_of(x[2 * i], x[2 * i + 1]), make_float2(cc.x, cc.y));
                 const float2 b = __fmul2_rn(f2_of(x[2 * i + 2], x[2 * i + 3]), make_float2(cc.z, cc.w));
                 x[2 * i] = __float_as_uint(a.x);
@@ -698,21 +652,20 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
                 x[2 * i + 2] = __float_as_uint(b.x);
                 x[2 * i + 3] = __float_as_uint(b.y);
             }
-            tmem_st_16(row + slo + 2 * TP * h + 16 * p, x);
+            tmem_st_8(row + slo + 2 * TP * h + 8 * p, x);
         }
         decay = q.decay;
         plen = q.len;
         of = P.scale * pow2f(-e) * MAT_DOWN;
-        ck_wait(s, &s.y_full, uint32_t(c) & 1u);
+        ck_wait(patience, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
 #pragma unroll 1
-        for (int p = 0; p < TP / 8; ++p) {                   // u for A u (one piece), u e^{G_C - G} kr for the state (two)
-            uint32_t y[16], un[8], hi[8], lo[8];
-            tmem_ld_16(row + tmy + 2 * TP * h + 16 * p, y);
-            const float* c3 = &q.c3[2 * TP * h + 16 * p];
+        for (int p = 0; p < TP / 4; ++p) {                   // u for A u (one piece), u e^{G_C - G} kr for the state (two)
+            uint32_t y[8], un[4], hi[4], lo[4];
+            tmem_ld_8(row + tmy + 2 * TP * h + 8 * p, y);
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                const float4 cc = *reinterpret_cast<const float4*>(c3 + 2 * i);
+            for (int i = 0; i < 4; i += 2) {
+                const float4 cc = *reinterpret_cast<const float4*>(&q.c3[2 * TP * h + 8 * p + 2 * i]);
                 const float2 u0 = f2_of(y[2 * i], y[2 * i + 1]), u1 = f2_of(y[2 * i + 2], y[2 * i + 3]);
                 const float2 d0 = __fmul2_rn(u0, both(MAT_DOWN)), d1 = __fmul2_rn(u1, both(MAT_DOWN));
                 un[i] = h2_bits(__floats2half2_rn(d0.x, d0.y));
@@ -720,27 +673,11 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
                 split_h2(__fmul2_rn(u0, make_float2(cc.x, cc.y)), hi[i], lo[i]);
                 split_h2(__fmul2_rn(u1, make_float2(cc.z, cc.w)), hi[i + 1], lo[i + 1]);
             }
-            tmem_st_8(row + TM_UOP + TP * h + 8 * p, un);
-            tmem_st_8(row + TM_PHI + TP * h + 8 * p, hi);
-            tmem_st_8(row + TM_PLO + TP * h + 8 * p, lo);
+            tmem_st_4(row + TM_UOP + TP * h + 4 * p, un);
+            tmem_st_4(row + TM_PHI + TP * h + 4 * p, hi);
+            tmem_st_4(row + TM_PLO + TP * h + 4 * p, lo);
         }
-        tmem_st_wait();
-        tc_fence_before_sync();
-        named_bar(1, CK_MAIN);
-        if (warp == 0) {                                     // A u, then the chunk's part of the state
-            tc_fence_after_sync();
-            const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16), kt = ck_desc(ti, 16384);
-#pragma unroll 1
-            for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, tm + slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);
-            umma_commit_if(el, &s.au_full[buf]);
-#pragma unroll 1
-            for (int ks = 0; ks < 4; ++ks) {
-                umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
-                umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
-            }
-            umma_commit_if(el, &s.d_full);
-        }
-        __syncwarp();
+        ck_ready(&s.u_ready, lane);
     }
     const float2 down = both(pow2f(-e));
 #pragma unroll
@@ -748,8 +685,62 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, const
         const float2 a = __fmul2_rn(S[2 * i], down), b = __fmul2_rn(S[2 * i + 1], down);
         *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
     }
-    if (warp == 0) umma_commit_if(el, &s.fin);
-    if (warp == 4) bulk_wait_all();
+}
+
+// The tensor-core instructions of the main chain, and the bulk stores of the outputs, by a warp of their own: whoever issues waits while
+// the tensor cores are busy.
+__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* outs, int hv, int t0, int nchunk, uint32_t tm, int& patience) {
+    const uint32_t el = elect_one();
+#pragma unroll 1
+    for (int c = 0; c < nchunk; ++c) {
+        const int buf = c & 1;
+        const uint32_t ph = uint32_t(c >> 1) & 1u, pc = uint32_t(c) & 1u, slo = tm + tm_slo(buf), tmy = tm + tm_slo(buf ^ 1);
+        const uint64_t kq = ck_desc(smem_u32(s.tile[buf]), 16), kt = ck_desc(smem_u32(s.tile[buf]), 16384);
+        ck_wait(patience, &s.tile_full[buf], ph);
+        ck_wait(patience, &s.s_ready, pc);
+        tc_fence_after_sync();
+#pragma unroll 1
+        for (int ks = 0; ks < 8; ++ks) {                     // S k^T
+            const uint64_t d = kq + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
+            umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
+            umma_f16_ts(el, tm + TM_X, slo + 8 * ks, d, ck_idesc(64, false), 1u);
+        }
+        umma_commit_if(el, &s.ks_full);
+#pragma unroll 1
+        for (int ks = 0; ks < 8; ++ks)                       // S q^T
+            umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, kq + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
+        umma_commit_if(el, &s.qs_full);
+        ck_wait(patience, &s.ta_full[buf], ph);
+        ck_wait(patience, &s.r_ready, pc);
+        tc_fence_after_sync();
+        const uint64_t th = ck_desc(smem_u32(s.thi[buf]), 16), tl = ck_desc(smem_u32(s.tlo[buf]), 16);
+#pragma unroll 1
+        for (int ks = 0; ks < 4; ++ks) {                     // u = T r
+            umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
+            umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
+            umma_f16_ts(el, tmy, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
+        }
+        umma_commit_if(el, &s.y_full);
+        if (el && c > 0) tma_store_2d(outs, s.o, hv * VD, t0 + (c - 1) * CT);      // outputs of the chunk before, a full one
+        __syncwarp();
+        ck_wait(patience, &s.u_ready, pc);
+        tc_fence_after_sync();
+        const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16);
+#pragma unroll 1
+        for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);       // A u
+        if (el) bulk_wait_read();                            // au_full says that the outputs' buffer is free, too
+        __syncwarp();
+        umma_commit_if(el, &s.au_full[buf]);
+#pragma unroll 1
+        for (int ks = 0; ks < 4; ++ks) {                     // the chunk's part of the state
+            umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
+            umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
+        }
+        umma_commit_if(el, &s.d_full);
+    }
+    umma_commit_if(el, &s.fin);
+    if (el) bulk_wait_all();
+    __syncwarp();
 }
 
 __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P, const __grid_constant__ CUtensorMap rows,
@@ -761,7 +752,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.raw_full[i], 1);
-            mbar_init(&s.tile_full[i], 1);
+            mbar_init(&s.tile_full[i], 2);
             mbar_init(&s.ta_full[i], 1);
             mbar_init(&s.main_done[i], CK_MAIN / 32);
             mbar_init(&s.au_full[i], 1);
@@ -771,6 +762,9 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
         mbar_init(&s.qs_full, 1);
         mbar_init(&s.y_full, 1);
         mbar_init(&s.d_full, 1);
+        mbar_init(&s.s_ready, CK_MAIN / 32);
+        mbar_init(&s.r_ready, CK_MAIN / 32);
+        mbar_init(&s.u_ready, CK_MAIN / 32);
         mbar_init(&s.fin, 3);
         s.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -803,14 +797,19 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     const uint32_t tm = s.tm;
     const int nchunk = int((len + CT - 1) / CT);
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
-    if (uw >= CK_MAIN / 32) {
-        if (MG == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane);
+    int patience = WAIT_LIMIT;
+    if (uw == CK_THREADS / 32 - 1) {
+        ck_issue(s, &outs, hv, int(t0), nchunk, tm, patience);
+    } else if (uw >= CK_MAIN / 32) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
+        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane, patience);
     } else {
-        if (MG == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-        ck_main(s, P, &outs, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid);
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_MAIN_REGS));
+        ck_main(s, P, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid,
+                patience);
     }
-    ck_wait(s, &s.fin, 0);                                   // no tensor-core instruction is left
+    ck_wait(patience, &s.fin, 0);                            // no tensor-core instruction is left
+    if (patience == 0) s.dead = 1;
     tc_fence_before_sync();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tm, 512);
@@ -859,6 +858,11 @@ static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     int rc = encode_rows(&rows, P.mixed, P.T, 2 * int64_t(P.H) * KD + int64_t(P.HV) * VD, P.mixed_stride, 64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = encode_rows(&outs, P.o, P.T, int64_t(P.HV) * VD, int64_t(P.HV) * VD, VD, CU_TENSOR_MAP_SWIZZLE_NONE);
     if (!rc) rc = ensure_smem((const void*)rule_chunk_kernel, smem);
+    static const int regs = [] {
+        cudaFuncAttributes at;
+        return cudaFuncGetAttributes(&at, rule_chunk_kernel) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (!rc && regs != CK_REGS) return LQ_ERR_LAUNCH;        // the register split of the warps would not add up
     if (rc) return rc;
     const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(P.N) * unsigned(P.HV), CK_THREADS, smem, st, P, rows, outs);
     if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
