@@ -48,6 +48,7 @@ __device__ __forceinline__ uint32_t tm_gram(int buf) { return buf ? 384u : 448u;
 
 // f16 operands, fp32 accumulator; B with the reduction contiguous (K-major) or, for S += u k^T, the 128 key columns (MN-major)
 __host__ __device__ constexpr uint32_t ck_idesc(int n, bool b_mn) { return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (uint32_t(n >> 3) << 17) | ((128u >> 4) << 24); }
+constexpr uint32_t CK_IDESC_BF16 = (1u << 7) | (1u << 10);    // both operands bf16
 // Descriptor of rows of 128 bytes in the 128-byte swizzle, eight rows (1 KB) after one another; `lbo`: bytes between blocks of 64
 // elements of a MN-major operand (not used by a K-major one, which is advanced by hand).
 __device__ __forceinline__ uint64_t ck_desc(uint32_t addr, uint32_t lbo) {
@@ -69,23 +70,25 @@ struct alignas(16) PrepSmem {                                // of one prep grou
     float tt[2][32][36];                                     // T^T of the two diagonal blocks of 32, times 2^13
     float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
     float gh[CT], gl[CT];                                    // the two apart and negated
-    float kr[CT], qr[CT], ws[32], beta[CT];                  // ws: kr_s times the decay from s to token 31, for s < 32
+    float kr[CT], qr[CT], ws[32], beta[CT];                  // 1 / |k|, 1 / |q|; ws: kr_s times the decay from s to token 31, for s < 32
+    float down[2 * CT];                                      // powers of two that take the rows of k and q to f16
 };
 struct alignas(16) ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
-    unsigned char thi[2][8192], tlo[2][8192], amat[2][8192], v[2][16384];          // v: bf16, two blocks of 64 values by 64 rows
+    unsigned char raw[32768];                                // the same as it comes, bf16
+    unsigned char thi[8192], tlo[8192], amat[2][8192], v[16384];                   // v: bf16, two blocks of 64 values by 64 rows
     uint16_t o[CT][VD];                                      // outputs on their way out
     PrepSmem prep[2];
     ChunkScalars sc[2];
-    uint16_t vsum[2][8][VD];                                 // bf16 sums of |v| of a value dimension, over every eighth token each
+    uint16_t vsum[8][VD];                                    // bf16 sums of |v| of a value dimension, over every eighth token each
     float part[2][CK_MAIN];
-    uint64_t raw_full[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
+    uint64_t raw_full[2], v_full[2], v_ready[2], raw_free, tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
     uint32_t tm;
     int dead;                                                // a wait has run out
 };
 
-static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
+static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, raw) % 1024 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
                   offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
                   offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(ChunkSmem, vsum) % 16 == 0 &&
                   offsetof(PrepSmem, gh) % 16 == 0 && offsetof(PrepSmem, gl) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
@@ -135,26 +138,31 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ float decay_between(float2 to, float2 from) { return ex2((to.x - from.x) + (to.y - from.y)); }
 __device__ __forceinline__ void prep_bar(int grp) { named_bar(2 + grp, CK_PREP); }
 
-// k, q and v rows of a chunk, as they come: boxes of 64 rows by 64 elements in the 128-byte swizzle, k and q where their f16 form goes.
-// Rows behind the chunk's last token belong to other sequences (or lie behind the tensor: zeros).
-constexpr uint32_t CK_RAW_BYTES = 6 * 8192;
-__device__ __forceinline__ void ck_fetch(ChunkSmem& s, const CUtensorMap* rows, int grp, int xk, int xq, int xv, int t0) {
-    mbar_arrive_expect_tx(&s.raw_full[grp], CK_RAW_BYTES);
+// k and q rows of a chunk, or its rows of v, as they come: boxes of 64 rows by 64 elements in the 128-byte swizzle.  Rows behind the
+// chunk's last token belong to other sequences (or lie behind the tensor: zeros).
+__device__ __forceinline__ void ck_fetch_kq(ChunkSmem& s, const CUtensorMap* rows, int xk, int xq, int t0, uint64_t* full) {
+    mbar_arrive_expect_tx(full, 4 * 8192);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-        tma_load_2d(s.tile[grp] + 16384 * b, rows, xk + 64 * b, t0, &s.raw_full[grp]);
-        tma_load_2d(s.tile[grp] + 16384 * b + 8192, rows, xq + 64 * b, t0, &s.raw_full[grp]);
-        tma_load_2d(s.v[grp] + 8192 * b, rows, xv + 64 * b, t0, &s.raw_full[grp]);
+        tma_load_2d(s.raw + 16384 * b, rows, xk + 64 * b, t0, full);
+        tma_load_2d(s.raw + 16384 * b + 8192, rows, xq + 64 * b, t0, full);
     }
 }
-// Sum of four values over the sixteen lanes that share lane >> 4: every exchange halves what a lane keeps.  Lane l returns the total of
-// value (l >> 2) & 3.
-__device__ __forceinline__ float fold4(const float (&v)[4], int lane) {
-    const bool u8 = lane & 8, u4 = lane & 4;
-    const float a = (u8 ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, u8 ? v[0] : v[2], 8);
-    const float b = (u8 ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, u8 ? v[1] : v[3], 8);
-    float s = (u4 ? b : a) + __shfl_xor_sync(0xffffffffu, u4 ? a : b, 4);
-    s += __shfl_xor_sync(0xffffffffu, s, 2);
+__device__ __forceinline__ void ck_fetch_v(ChunkSmem& s, const CUtensorMap* rows, int xv, int t0, uint64_t* full) {
+    mbar_arrive_expect_tx(full, 2 * 8192);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) tma_load_2d(s.v + 8192 * b, rows, xv + 64 * b, t0, full);
+}
+// Sum of eight values over the sixteen lanes that share lane >> 4: every exchange halves what a lane keeps.  Lane l returns the total of
+// value (l >> 1) & 7.
+__device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
+    const bool u8 = lane & 8, u4 = lane & 4, u2 = lane & 2;
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = (u8 ? v[4 + i] : v[i]) + __shfl_xor_sync(0xffffffffu, u8 ? v[i] : v[4 + i], 8);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = (u4 ? a[2 + i] : a[i]) + __shfl_xor_sync(0xffffffffu, u4 ? a[i] : a[2 + i], 4);
+    float s = (u2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, u2 ? b[0] : b[1], 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
 // Sums of |v| over the tokens g, g + 8, ... of a chunk (g: this half of a warp), for a bound: bf16 will do, rounded up by the reader.  A
@@ -174,45 +182,61 @@ __device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)
     }
     *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3]));
 }
-// rows behind the chunk's last token, which belong to other sequences, become zeros
-__device__ __forceinline__ void ck_clear(unsigned char* tile, unsigned char* v, int len, int pt) {
+// rows behind the chunk's last token, which belong to other sequences, become zeros; pieces of 16 bytes, blocks of 64 rows
+__device__ __forceinline__ void ck_clear(unsigned char* p, int blocks, int len, int pt, int threads) {
 #pragma unroll 1
-    for (int i = pt; i < 6 * 512; i += CK_PREP)              // pieces of 16 bytes: six blocks of 64 rows
-        if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(i < 4 * 512 ? tile + 16 * i : v + 16 * (i - 4 * 512)) = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = pt; i < blocks * 512; i += threads)
+        if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(p + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
 }
-// Rows of k (warps 0 and 1) and q to f16, in place: a lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
-__device__ __forceinline__ void ck_convert(unsigned char* tile, float* rs, int w, int lane) {
+// Norms of the rows of k (warps 0 and 1) and q.  A lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
+__device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* down, int w, int lane) {
     const int c = lane & 15;
-    tile += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
+    raw += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
 #pragma unroll 1
-    for (int p = 0; p < 4; ++p) {
-        uint4 x[4];
-        float ss[4];
+    for (int p = 0; p < 2; ++p) {
+        float ss[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const uint4*>(tile + 1024 * p + 256 * i);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f0 = bf16x2_to_f2(x[i].x), f1 = bf16x2_to_f2(x[i].y), f2 = bf16x2_to_f2(x[i].z), f3 = bf16x2_to_f2(x[i].w);
+        for (int i = 0; i < 8; ++i) {
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + 2048 * p + 256 * i);
+            const float2 f0 = bf16x2_to_f2(x.x), f1 = bf16x2_to_f2(x.y), f2 = bf16x2_to_f2(x.z), f3 = bf16x2_to_f2(x.w);
             const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2)), c2 = __fadd2_rn(a, b);
             ss[i] = c2.x + c2.y;
         }
-        const float sum = fold4(ss, lane);
-        // the row times 2^-e has a norm in [1, 2); a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
+        const float sum = fold8(ss, lane);
+        // a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
+        if (__any_sync(0xffffffffu, sum > 3.4e38f)) {
+#pragma unroll 1
+            for (int i = 0; i < 8; ++i)
+                if (__shfl_sync(0xffffffffu, sum, (lane & 16) | (i << 1)) > 3.4e38f) *reinterpret_cast<uint4*>(raw + 2048 * p + 256 * i) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        // the row times 2^-e has a norm in [1, 2)
         int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
         e = e < -60 ? -60 : e;
-        const float m = sum <= 3.4e38f ? pow2f(-e) : 0.f;
-        if (!(lane & 3)) rs[32 * (w & 1) + 8 * p + 2 * ((lane >> 2) & 3) + (lane >> 4)] = rsqrtf(sum + 1e-6f) * pow2f(e);
+        if (!(lane & 1)) {
+            const int r = 16 * p + 2 * ((lane >> 1) & 7) + (lane >> 4);
+            rs[32 * (w & 1) + r] = rsqrtf(sum + 1e-6f);
+            down[32 * w + r] = pow2f(-e);
+        }
+    }
+}
+// rows of k and q as f16
+__device__ __forceinline__ void ck_convert(const unsigned char* raw, unsigned char* tile, const float* down, int w, int lane) {
+    const int c = lane & 15, at = (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
+    down += 32 * w + (lane >> 4);
+#pragma unroll 1
+    for (int p = 0; p < 4; ++p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float mi = __shfl_sync(0xffffffffu, m, (lane & 16) | (i << 2));
-            const uint32_t xw[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            const uint4 x = *reinterpret_cast<const uint4*>(raw + at + 1024 * p + 256 * i);
+            const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
+            const float m = down[8 * p + 2 * i];
             uint32_t h[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), both(mi));
+                const float2 y = __fmul2_rn(bf16x2_to_f2(xw[j]), both(m));
                 h[j] = h2_bits(__floats2half2_rn(y.x, y.y));
             }
-            *reinterpret_cast<uint4*>(tile + 1024 * p + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(tile + at + 1024 * p + 256 * i) = make_uint4(h[0], h[1], h[2], h[3]);
         }
     }
 }
@@ -328,16 +352,17 @@ __device__ __forceinline__ void put_t(unsigned char* thi, unsigned char* tlo, in
 // T11^T L21^T: its accumulators are then the B operand of the second as they are.  Scales: L and T times 2^13, their product back to
 // 2^10 (a sum of 32).  Loops rather than straight code: an SM's instruction cache holds 32 KB, and beyond that every instruction of the
 // kernel costs 2.7 cycles.
-__device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsigned char* tlo, int grp, int w, int lane) {
+__device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsigned char* tlo, uint64_t* t_free, uint32_t t_parity, int& patience,
+                                          int grp, int w, int lane) {
     const int gid = lane >> 2, tig = lane & 3;
     {
         const int o = 16 * w, c = lane & 15;
         float* tt = &s.tt[w >> 1][(o & 16) + c][o & 16];     // this column of T
-#pragma unroll 1
+#pragma unroll
         for (int b = 0; b < 16; b += 4) {
             const float* l = &s.L[o + b][o];
             float a[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
+#pragma unroll
             for (int m = 0; m < b; m += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(tt + m);
 #pragma unroll
@@ -357,6 +382,7 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
             *reinterpret_cast<float4*>(tt + b) = x;          // (both halves of the warp: the same)
         }
         __syncwarp();
+        if (t_free) ck_wait(patience, t_free, t_parity);     // the T of the chunk before has been used
         const float* d = &s.tt[w >> 1][(o & 16) + 2 * tig][(o & 16) + gid];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -419,47 +445,52 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
     const int pt = 32 * w + lane;
     PrepSmem& ps = s.prep[grp];
     ChunkScalars& q = s.sc[grp];
-    unsigned char* tile = s.tile[grp];
     const float ea = expf(P.A_log[hv]), dtb = P.dt_bias[hv];
 #pragma unroll 1
     for (int c = grp; c < nchunk; c += 2) {
-        const uint32_t ph = uint32_t(c >> 1) & 1u;
+        const uint32_t ph = uint32_t(c >> 1) & 1u, pc = uint32_t(c) & 1u;
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
-        if (w == 3) ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
         if (w == 0) {
-            if (c >= 2) ck_wait<true>(patience, &s.main_done[grp], ph ^ 1u);
-            if (el) ck_fetch(s, rows, grp, (P.H + hk) * KD, hk * KD, 2 * P.H * KD + hv * VD, int(at));
+            if (c > 0) ck_wait<true>(patience, &s.raw_free, pc ^ 1u);
+            if (el) ck_fetch_kq(s, rows, (P.H + hk) * KD, hk * KD, int(at), &s.raw_full[grp]);
             __syncwarp();
+        } else if (w == 3) {
+            ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
         }
         ck_wait<true>(patience, &s.raw_full[grp], ph);
         if (n < CT) {
-            ck_clear(tile, s.v[grp], n, pt);
+            ck_clear(s.raw, 4, n, pt, CK_PREP);
             prep_bar(grp);
         }
-        ck_vsum(s.v[grp], s.vsum[grp], w, lane);
-        ck_convert(tile, w < 2 ? ps.kr : ps.qr, w, lane);
+        ck_norms(s.raw, w < 2 ? ps.kr : ps.qr, ps.down, w, lane);
         fence_async_smem();
-        tc_fence_before_sync();                              // (this group's last Gram matrix has been read)
         prep_bar(grp);
-        if (w == 0) {
+        if (w == 0) {                                        // K K^T and Q K^T of the rows as they are
             tc_fence_after_sync();
-            const uint64_t d0 = ck_desc(smem_u32(tile), 16);
-#pragma unroll 1
+            const uint64_t d0 = ck_desc(smem_u32(s.raw), 16);
+#pragma unroll 4
             for (int ks = 0; ks < 8; ++ks) {
                 const uint64_t d = d0 + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
-                umma_f16_ss(el, tm + tm_gram(grp), d, d, ck_idesc(64, false), ks > 0);
+                umma_f16_ss(el, tm + tm_gram(grp), d, d, ck_idesc(64, false) | CK_IDESC_BF16, ks > 0);
             }
             umma_commit_if(el, &s.g_full[grp]);
+            __syncwarp();
         }
+        if (c >= 2) ck_wait<true>(patience, &s.main_done[grp], ph ^ 1u);
+        ck_convert(s.raw, s.tile[grp], ps.down, w, lane);
+        ck_wait(patience, &s.g_full[grp], ph);               // (the rows as they are have been read, and the matrix is there)
+        if (lane == 0) mbar_arrive(&s.raw_free);
         __syncwarp();
+        fence_async_smem();
+        prep_bar(grp);
         if (w >= 2) {                                        // scalars for the main warps, which may then begin
             const int tk = pt - 64;
             const float2 G = ps.G[tk], Gc = ps.G[CT - 1];
-            const float e = ex2(G.x + G.y), kr = ps.kr[tk], b = ps.beta[tk];
+            const float e = ex2(G.x + G.y), kr = __fdividef(ps.kr[tk], ps.down[tk]), b = ps.beta[tk];
             q.c1[tk] = -(b * e * kr);
             q.beta[tk] = b;
-            q.c2[tk] = e * ps.qr[tk] * MAT_UP;
+            q.c2[tk] = e * __fdividef(ps.qr[tk], ps.down[CT + tk]) * MAT_UP;
             q.c3[tk] = decay_between(Gc, G) * kr * MAT_DOWN;
             if (tk == 0) {
                 q.decay = ex2(Gc.x + Gc.y);
@@ -476,11 +507,11 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
             ps.ws[lane] = decay_between(ps.G[31], g0) * ps.kr[lane];
         }
         prep_bar(grp);
-        ck_wait(patience, &s.g_full[grp], ph);
         tc_fence_after_sync();
         ck_gram(ps, s.amat[grp], tm + tm_gram(grp), w, lane);
+        tc_fence_before_sync();                              // (the matrix has been read)
         prep_bar(grp);
-        ck_invert(ps, s.thi[grp], s.tlo[grp], grp, w, lane);
+        ck_invert(ps, s.thi, s.tlo, c > 0 ? &s.y_full : nullptr, pc ^ 1u, patience, grp, w, lane);
         fence_async_smem();
         prep_bar(grp);
         if (pt == 0) mbar_arrive(&s.ta_full[grp]);
@@ -529,12 +560,13 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         const int buf = c & 1;
         const uint32_t ph = uint32_t(c >> 1) & 1u, slo = tm_slo(buf), tmy = tm_slo(buf ^ 1);
         const ChunkScalars& q = s.sc[buf];
-        const unsigned char* vp = s.v[buf] + voff;
+        const unsigned char* vp = s.v + voff;
         float va = 0.f;
         if (c < nchunk) {
             ck_wait(patience, &s.tile_full[buf], ph);
+            ck_wait(patience, &s.v_ready[buf], ph);
 #pragma unroll
-            for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[buf][g][v]);
+            for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[g][v]);
             va *= 1.125f;                                    // (sums in bf16: not below the true one)
         }
         if (c > 0) {                                         // the state behind the chunk before
@@ -547,7 +579,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 #pragma unroll
                 for (int i = 0; i < 8; ++i) S[8 * p + i] = __ffma2_rn(S[8 * p + i], both(decay), f2_of(r[2 * i], r[2 * i + 1]));
             }
-            // every product of that chunk is through, and its scalars and values have been read: its buffers are free
+            // every product of that chunk is through, and its scalars have been read: its buffers are free
             if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
             __syncwarp();
         }
@@ -591,7 +623,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         if (c > 0) {                                         // outputs of the chunk before
             ck_wait(patience, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
             tc_fence_after_sync();
-#pragma unroll 1
+#pragma unroll 2
             for (int p = 0; p < TP / 4; ++p) {
                 uint32_t x[8];
                 tmem_ld_8(row + tmy + 2 * TP * h + 8 * p, x);
@@ -614,11 +646,12 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                     *reinterpret_cast<const uint4*>(&s.o[r][8 * (tid & 15)]);
             break;
         }
+        ck_wait(patience, &s.v_full[buf], ph);
         ck_wait(patience, &s.ks_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
         {                                                    // r = beta (v - e^G S k^), times 2^e
             const float2 up = both(pow2f(e));
-#pragma unroll 1
+#pragma unroll 2
             for (int p = 0; p < TP / 4; ++p) {
                 uint32_t x[8], hi[4], lo[4];
                 tmem_ld_8(row + TM_X + 2 * TP * h + 8 * p, x);
@@ -638,7 +671,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         }
         ck_wait(patience, &s.qs_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
-#pragma unroll 1
+#pragma unroll 2
         for (int p = 0; p < TP / 4; ++p) {                   // e^G S q^, for A u to be added to
             uint32_t x[8];
             tmem_ld_8(row + TM_XQ + 2 * TP * h + 8 * p, x);
@@ -659,7 +692,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         of = P.scale * pow2f(-e) * MAT_DOWN;
         ck_wait(patience, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
-#pragma unroll 1
+#pragma unroll 2
         for (int p = 0; p < TP / 4; ++p) {                   // u for A u (one piece), u e^{G_C - G} kr for the state (two)
             uint32_t y[8], un[4], hi[4], lo[4];
             tmem_ld_8(row + tmy + 2 * TP * h + 8 * p, y);
@@ -689,8 +722,26 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 
 // The tensor-core instructions of the main chain, and the bulk stores of the outputs, by a warp of their own: whoever issues waits while
 // the tensor cores are busy.
-__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* outs, int hv, int t0, int nchunk, uint32_t tm, int& patience) {
+// the values of chunk c are there: rows behind the chunk's end cleared, and the sums for the bounds
+__device__ __forceinline__ void ck_values(ChunkSmem& s, int c, int64_t len, int& patience) {
+    const int lane = threadIdx.x & 31, buf = c & 1;
+    const int64_t left = len - int64_t(c) * CT;
+    ck_wait(patience, &s.v_full[buf], uint32_t(c >> 1) & 1u);
+    if (left < CT) {
+        ck_clear(s.v, 2, int(left), lane, 32);
+        __syncwarp();
+    }
+#pragma unroll 1
+    for (int w = 0; w < 4; ++w) ck_vsum(s.v, s.vsum, w, lane);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.v_ready[buf]);
+    __syncwarp();
+}
+__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, const CUtensorMap* outs, int xv, int hv, int t0, int64_t len, int nchunk, uint32_t tm, int& patience) {
     const uint32_t el = elect_one();
+    if (el) ck_fetch_v(s, rows, xv, t0, &s.v_full[0]);
+    __syncwarp();
+    ck_values(s, 0, len, patience);
 #pragma unroll 1
     for (int c = 0; c < nchunk; ++c) {
         const int buf = c & 1;
@@ -699,44 +750,46 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* outs, 
         ck_wait(patience, &s.tile_full[buf], ph);
         ck_wait(patience, &s.s_ready, pc);
         tc_fence_after_sync();
-#pragma unroll 1
+#pragma unroll 4
         for (int ks = 0; ks < 8; ++ks) {                     // S k^T
             const uint64_t d = kq + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
             umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
             umma_f16_ts(el, tm + TM_X, slo + 8 * ks, d, ck_idesc(64, false), 1u);
         }
         umma_commit_if(el, &s.ks_full);
-#pragma unroll 1
+#pragma unroll 4
         for (int ks = 0; ks < 8; ++ks)                       // S q^T
             umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, kq + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
         umma_commit_if(el, &s.qs_full);
         ck_wait(patience, &s.ta_full[buf], ph);
         ck_wait(patience, &s.r_ready, pc);
         tc_fence_after_sync();
-        const uint64_t th = ck_desc(smem_u32(s.thi[buf]), 16), tl = ck_desc(smem_u32(s.tlo[buf]), 16);
-#pragma unroll 1
+        const uint64_t th = ck_desc(smem_u32(s.thi), 16), tl = ck_desc(smem_u32(s.tlo), 16);
+#pragma unroll
         for (int ks = 0; ks < 4; ++ks) {                     // u = T r
             umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
             umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
             umma_f16_ts(el, tmy, tm + TM_PLO + 8 * ks, th + 2 * ks, ck_idesc(64, false), 1u);
         }
         umma_commit_if(el, &s.y_full);
+        if (el && c + 1 < nchunk) ck_fetch_v(s, rows, xv, t0 + (c + 1) * CT, &s.v_full[buf ^ 1]);        // (r is there: v has been read)
         if (el && c > 0) tma_store_2d(outs, s.o, hv * VD, t0 + (c - 1) * CT);      // outputs of the chunk before, a full one
         __syncwarp();
         ck_wait(patience, &s.u_ready, pc);
         tc_fence_after_sync();
         const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16);
-#pragma unroll 1
+#pragma unroll
         for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);       // A u
         if (el) bulk_wait_read();                            // au_full says that the outputs' buffer is free, too
         __syncwarp();
         umma_commit_if(el, &s.au_full[buf]);
-#pragma unroll 1
+#pragma unroll
         for (int ks = 0; ks < 4; ++ks) {                     // the chunk's part of the state
             umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
             umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
         }
         umma_commit_if(el, &s.d_full);
+        if (c + 1 < nchunk) ck_values(s, c + 1, len, patience);
     }
     umma_commit_if(el, &s.fin);
     if (el) bulk_wait_all();
@@ -752,12 +805,15 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.raw_full[i], 1);
+            mbar_init(&s.v_full[i], 1);
+            mbar_init(&s.v_ready[i], 1);
             mbar_init(&s.tile_full[i], 2);
             mbar_init(&s.ta_full[i], 1);
             mbar_init(&s.main_done[i], CK_MAIN / 32);
             mbar_init(&s.au_full[i], 1);
             mbar_init(&s.g_full[i], 1);
         }
+        mbar_init(&s.raw_free, CK_PREP / 32);
         mbar_init(&s.ks_full, 1);
         mbar_init(&s.qs_full, 1);
         mbar_init(&s.y_full, 1);
@@ -782,11 +838,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
         return;
     }
 #pragma unroll 1
-    for (int i = tid; i < 2 * 8192 / 16; i += CK_THREADS) {                        // the upper right blocks of T and A stay zero
-        reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);
-        reinterpret_cast<uint4*>(s.tlo)[i] = make_uint4(0u, 0u, 0u, 0u);
-        reinterpret_cast<uint4*>(s.amat)[i] = make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int i = tid; i < 4 * 8192 / 16; i += CK_THREADS) reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);   // the upper right
+                                                                                    // blocks of T (head, remainder) and both A stay zero
 #pragma unroll 1
     for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
     if (warp == 0) tmem_alloc(&s.tm, 512);
@@ -799,7 +852,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
     int patience = WAIT_LIMIT;
     if (uw == CK_THREADS / 32 - 1) {
-        ck_issue(s, &outs, hv, int(t0), nchunk, tm, patience);
+        ck_issue(s, &rows, &outs, 2 * P.H * KD + hv * VD, hv, int(t0), len, nchunk, tm, patience);
     } else if (uw >= CK_MAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
         ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane, patience);
