@@ -24,14 +24,15 @@
 
 namespace lq {
 
-constexpr int RULE_SHORT = 8;                                // mean length from which lq_gdn_prefill works in chunks
+// Sequences of fewer tokens are run token by token, longer ones in chunks.  A chunk costs a CTA 18 us however many tokens it has, the
+// recurrence about 0.8 us a token once every SM has heads: 12 tokens of 64 sequences of 32 heads 155 against 261 us, 24 tokens 297 against 263;
+// one sequence, 16 tokens 15.1 against 19.2 us, 24 tokens 19.8 against 18.9.
+constexpr int RULE_SHORT = 20;
+constexpr int RANKED = 128;                                  // batches up to which CTAs take the longest sequences first
 constexpr int CT = 64;                                       // tokens of a chunk
 // T and A lie within [-1, 1]; times 2^13 their small entries keep eleven bits down to 2^-27 as well
 constexpr float MAT_UP = 8192.f, MAT_DOWN = 1.f / 8192.f;
-#ifndef CK_MG
-#define CK_MG 2
-#endif
-constexpr int MG = CK_MG;                                    // threads that share a row of the state, each with
+constexpr int MG = 2;                                        // threads that share a row of the state, each with
 constexpr int SP = 64 / MG, TP = 32 / MG;                    // SP pairs of its columns and TP pairs of a chunk's tokens
 constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_PREP + 32;
 // Registers: 17 warps get 96 each (five of them share a quarter of the SM).  The main warps take over what the prep warps give up,
@@ -83,9 +84,11 @@ struct alignas(16) ChunkSmem {
     ChunkScalars sc[2];
     uint16_t vsum[8][VD];                                    // bf16 sums of |v| of a value dimension, over every eighth token each
     float part[2][CK_MAIN];
-    uint64_t raw_full[2], v_full[2], v_ready[2], raw_free, tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
+    uint64_t raw_full[2], v_full[2], v_ready[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
     uint32_t tm;
     int dead;                                                // a wait has run out
+    int seq;                                                 // this CTA's sequence
+    int len[RANKED];
 };
 
 static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, raw) % 1024 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
@@ -95,8 +98,7 @@ static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && of
               "vector accesses and swizzled tiles");
 
 // Waits like warp_wait_bounded.  Once a wait of a warp has run out, its later ones test once and go on: the CTA runs to its end, on
-// rubbish, and reports.  SLEEP: waits that are long as a rule leave the issue slots to the warps that work.
-template <bool SLEEP = false>
+// rubbish, and reports.
 __device__ __forceinline__ void ck_wait(int& patience, uint64_t* bar, uint32_t parity) {
     int left = patience;
 #pragma unroll 1
@@ -105,7 +107,6 @@ __device__ __forceinline__ void ck_wait(int& patience, uint64_t* bar, uint32_t p
             patience = 0;
             break;
         }
-        if (SLEEP) __nanosleep(64);
     }
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
@@ -336,7 +337,6 @@ __device__ __forceinline__ Pieces pieces(float2 x) {
     split_h2(x, p.hi, p.lo);
     return p;
 }
-// D += A B for one m16n8k16 tile of operands in two pieces
 __device__ __forceinline__ void mma_pieces(float (&d)[4], const Pieces (&a)[4], const Pieces& b0, const Pieces& b1) {
     mma_h_16816(d, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b0.hi, b1.hi);
     mma_h_16816(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b0.lo, b1.lo);
@@ -439,6 +439,20 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
     }
 }
 
+// The values of chunk c are there: rows behind the chunk's end cleared, and the sums for the bounds.
+__device__ __forceinline__ void ck_values(ChunkSmem& s, int c, int64_t len, int grp, int w, int lane, int& patience) {
+    const int buf = c & 1, pt = 32 * w + lane;
+    const int64_t left = len - int64_t(c) * CT;
+    ck_wait(patience, &s.v_full[buf], uint32_t(c >> 1) & 1u);
+    if (left < CT) {
+        ck_clear(s.v, 2, int(left), pt, CK_PREP);
+        prep_bar(grp);
+    }
+    ck_vsum(s.v, s.vsum, w, lane);
+    prep_bar(grp);
+    if (pt == 0) mbar_arrive(&s.v_ready[buf]);
+    __syncwarp();
+}
 __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const CUtensorMap* rows, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
                                         int grp, int w, int lane, int& patience) {
     const uint32_t el = elect_one();
@@ -446,19 +460,17 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
     PrepSmem& ps = s.prep[grp];
     ChunkScalars& q = s.sc[grp];
     const float ea = expf(P.A_log[hv]), dtb = P.dt_bias[hv];
+    if (grp == 0 && w == 0 && el) ck_fetch_kq(s, rows, (P.H + hk) * KD, hk * KD, int(t0), &s.raw_full[0]);
+    __syncwarp();
 #pragma unroll 1
     for (int c = grp; c < nchunk; c += 2) {
         const uint32_t ph = uint32_t(c >> 1) & 1u, pc = uint32_t(c) & 1u;
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
-        if (w == 0) {
-            if (c > 0) ck_wait<true>(patience, &s.raw_free, pc ^ 1u);
-            if (el) ck_fetch_kq(s, rows, (P.H + hk) * KD, hk * KD, int(at), &s.raw_full[grp]);
-            __syncwarp();
-        } else if (w == 3) {
+        if (w == 3)
             ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
-        }
-        ck_wait<true>(patience, &s.raw_full[grp], ph);
+        ck_wait(patience, &s.raw_full[grp], ph);
+        if (c != 1) ck_values(s, c == 0 ? 0 : c - 1, len, grp, w, lane, patience);     // of the chunk before: the other group has its hands full
         if (n < CT) {
             ck_clear(s.raw, 4, n, pt, CK_PREP);
             prep_bar(grp);
@@ -477,13 +489,18 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
             umma_commit_if(el, &s.g_full[grp]);
             __syncwarp();
         }
-        if (c >= 2) ck_wait<true>(patience, &s.main_done[grp], ph ^ 1u);
+        if (c >= 2) ck_wait(patience, &s.main_done[grp], ph ^ 1u);
         ck_convert(s.raw, s.tile[grp], ps.down, w, lane);
         ck_wait(patience, &s.g_full[grp], ph);               // (the rows as they are have been read, and the matrix is there)
-        if (lane == 0) mbar_arrive(&s.raw_free);
-        __syncwarp();
         fence_async_smem();
         prep_bar(grp);
+        if (w == 0 && el && c + 1 < nchunk) {                // the next chunk, for the other group, into the buffer that is free now
+            ck_fetch_kq(s, rows, (P.H + hk) * KD, hk * KD, int(at) + CT, &s.raw_full[grp ^ 1]);
+            if (c + 2 < nchunk)
+#pragma unroll 1
+                for (int b = 0; b < 4; ++b) tma_prefetch_2d(rows, ((b & 2 ? P.H : 0) + hk) * KD + 64 * (b & 1), int(at) + 2 * CT);
+        }
+        __syncwarp();
         if (w >= 2) {                                        // scalars for the main warps, which may then begin
             const int tk = pt - 64;
             const float2 G = ps.G[tk], Gc = ps.G[CT - 1];
@@ -517,6 +534,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         if (pt == 0) mbar_arrive(&s.ta_full[grp]);
         __syncwarp();
     }
+    if (nchunk > 1 && (nchunk & 1) == grp) ck_values(s, nchunk - 1, len, grp, w, lane, patience);
     if (w == 0) umma_commit_if(el, &s.fin);
 }
 
@@ -722,26 +740,10 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 
 // The tensor-core instructions of the main chain, and the bulk stores of the outputs, by a warp of their own: whoever issues waits while
 // the tensor cores are busy.
-// the values of chunk c are there: rows behind the chunk's end cleared, and the sums for the bounds
-__device__ __forceinline__ void ck_values(ChunkSmem& s, int c, int64_t len, int& patience) {
-    const int lane = threadIdx.x & 31, buf = c & 1;
-    const int64_t left = len - int64_t(c) * CT;
-    ck_wait(patience, &s.v_full[buf], uint32_t(c >> 1) & 1u);
-    if (left < CT) {
-        ck_clear(s.v, 2, int(left), lane, 32);
-        __syncwarp();
-    }
-#pragma unroll 1
-    for (int w = 0; w < 4; ++w) ck_vsum(s.v, s.vsum, w, lane);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&s.v_ready[buf]);
-    __syncwarp();
-}
-__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, const CUtensorMap* outs, int xv, int hv, int t0, int64_t len, int nchunk, uint32_t tm, int& patience) {
+__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, const CUtensorMap* outs, int xv, int hv, int t0, int nchunk, uint32_t tm, int& patience) {
     const uint32_t el = elect_one();
     if (el) ck_fetch_v(s, rows, xv, t0, &s.v_full[0]);
     __syncwarp();
-    ck_values(s, 0, len, patience);
 #pragma unroll 1
     for (int c = 0; c < nchunk; ++c) {
         const int buf = c & 1;
@@ -750,14 +752,14 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
         ck_wait(patience, &s.tile_full[buf], ph);
         ck_wait(patience, &s.s_ready, pc);
         tc_fence_after_sync();
-#pragma unroll 4
+#pragma unroll 2
         for (int ks = 0; ks < 8; ++ks) {                     // S k^T
             const uint64_t d = kq + uint64_t(((ks >> 2) * 16384 + (ks & 3) * 32) >> 4);
             umma_f16_ts(el, tm + TM_X, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
             umma_f16_ts(el, tm + TM_X, slo + 8 * ks, d, ck_idesc(64, false), 1u);
         }
         umma_commit_if(el, &s.ks_full);
-#pragma unroll 4
+#pragma unroll 2
         for (int ks = 0; ks < 8; ++ks)                       // S q^T
             umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, kq + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
         umma_commit_if(el, &s.qs_full);
@@ -765,7 +767,7 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
         ck_wait(patience, &s.r_ready, pc);
         tc_fence_after_sync();
         const uint64_t th = ck_desc(smem_u32(s.thi), 16), tl = ck_desc(smem_u32(s.tlo), 16);
-#pragma unroll
+#pragma unroll 2
         for (int ks = 0; ks < 4; ++ks) {                     // u = T r
             umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, th + 2 * ks, ck_idesc(64, false), ks > 0);
             umma_f16_ts(el, tmy, tm + TM_PHI + 8 * ks, tl + 2 * ks, ck_idesc(64, false), 1u);
@@ -773,27 +775,69 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
         }
         umma_commit_if(el, &s.y_full);
         if (el && c + 1 < nchunk) ck_fetch_v(s, rows, xv, t0 + (c + 1) * CT, &s.v_full[buf ^ 1]);        // (r is there: v has been read)
+        if (el && c + 2 < nchunk) {                          // the buffer allows no earlier copy, but what it will copy can be in L2
+            tma_prefetch_2d(rows, xv, t0 + (c + 2) * CT);
+            tma_prefetch_2d(rows, xv + 64, t0 + (c + 2) * CT);
+        }
         if (el && c > 0) tma_store_2d(outs, s.o, hv * VD, t0 + (c - 1) * CT);      // outputs of the chunk before, a full one
         __syncwarp();
         ck_wait(patience, &s.u_ready, pc);
         tc_fence_after_sync();
         const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16);
-#pragma unroll
+#pragma unroll 2
         for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);       // A u
         if (el) bulk_wait_read();                            // au_full says that the outputs' buffer is free, too
         __syncwarp();
         umma_commit_if(el, &s.au_full[buf]);
-#pragma unroll
+#pragma unroll 2
         for (int ks = 0; ks < 4; ++ks) {                     // the chunk's part of the state
             umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
             umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
         }
         umma_commit_if(el, &s.d_full);
-        if (c + 1 < nchunk) ck_values(s, c + 1, len, patience);
     }
     umma_commit_if(el, &s.fin);
     if (el) bulk_wait_all();
     __syncwarp();
+}
+
+// Sequence of rank r among those that are not left to the recurrence, the longest first (by their order in batches of more than RANKED, where
+// ranking would take longer than it saves); -1 if there are not that many.
+__device__ __forceinline__ int ck_sequence(ChunkSmem& s, const RuleParams& P, int r, int tid) {
+    int64_t t0, len;
+    if (tid == 0) s.seq = -1;
+    if (P.N <= RANKED) {
+        if (tid < P.N) {
+            rule_span(P, tid, t0, len);
+            s.len[tid] = int(len);
+        }
+        __syncthreads();
+        if (tid < P.N && s.len[tid] >= P.shorter) {
+            const int mine = s.len[tid];
+            int rank = 0;
+            for (int m = 0; m < P.N; ++m) rank += s.len[m] > mine || (s.len[m] == mine && m < tid);
+            if (rank == r) s.seq = tid;
+        }
+    } else {
+        __syncthreads();
+        if (tid < 32) {
+#pragma unroll 1
+            for (int base = 0; base < P.N; base += 32) {
+                bool in = false;
+                if (base + tid < P.N) {
+                    rule_span(P, base + tid, t0, len);
+                    in = len >= P.shorter;
+                }
+                const unsigned got = __ballot_sync(0xffffffffu, in);
+                const int before = __popc(got & ((1u << tid) - 1));
+                if (in && before == r) s.seq = base + tid;
+                r -= __popc(got);
+                if (r < 0) break;
+            }
+        }
+    }
+    __syncthreads();
+    return s.seq;
 }
 
 __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P, const __grid_constant__ CUtensorMap rows,
@@ -813,7 +857,6 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
             mbar_init(&s.au_full[i], 1);
             mbar_init(&s.g_full[i], 1);
         }
-        mbar_init(&s.raw_free, CK_PREP / 32);
         mbar_init(&s.ks_full, 1);
         mbar_init(&s.qs_full, 1);
         mbar_init(&s.y_full, 1);
@@ -826,10 +869,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    const int n = blockIdx.x / P.HV, hv = blockIdx.x % P.HV, hk = hv / (P.HV / P.H);
+    const int n = ck_sequence(s, P, int(blockIdx.x) / P.HV, tid), hv = blockIdx.x % P.HV, hk = hv / (P.HV / P.H);
+    if (n < 0) return;
     int64_t t0, len;
     rule_span(P, n, t0, len);
-    if (len == 0) return;
     const int slot = P.idx[n];
     if (slot <= 0 || slot >= P.NS || !first_of_slot(P.idx, n, slot, lane)) {       // padding: zeros, and no state
 #pragma unroll 1
@@ -852,7 +895,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
     int patience = WAIT_LIMIT;
     if (uw == CK_THREADS / 32 - 1) {
-        ck_issue(s, &rows, &outs, 2 * P.H * KD + hv * VD, hv, int(t0), len, nchunk, tm, patience);
+        ck_issue(s, &rows, &outs, 2 * P.H * KD + hv * VD, hv, int(t0), nchunk, tm, patience);
     } else if (uw >= CK_MAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
         ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane, patience);
@@ -917,7 +960,9 @@ static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     }();
     if (!rc && regs != CK_REGS) return LQ_ERR_LAUNCH;        // the register split of the warps would not add up
     if (rc) return rc;
-    const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(P.N) * unsigned(P.HV), CK_THREADS, smem, st, P, rows, outs);
+    // no more than T / P.shorter sequences can be that long
+    const int64_t most = P.T / P.shorter < P.N ? P.T / P.shorter : P.N;
+    const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(most) * unsigned(P.HV), CK_THREADS, smem, st, P, rows, outs);
     if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
     return finish_launch();
 }
@@ -929,6 +974,7 @@ static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, i
     P.ssm = ssm; P.SS = d->SS; P.mixed = (const uint16_t*)mixed; P.mixed_stride = mixed_stride; P.a = (const uint16_t*)a;
     P.b = (const uint16_t*)b; P.a_stride = a_stride; P.b_stride = b_stride; P.A_log = A_log; P.dt_bias = dt_bias; P.cu = cu;
     P.idx = idx; P.has_initial = has_initial; P.o = (uint16_t*)o; P.NS = d->NS; P.H = d->H; P.HV = d->HV; P.N = N; P.T = T;
+    P.shorter = T + 1;
     P.scale = scale > 0.f ? scale : 1.0f / sqrtf(float(KD));
     return P;
 }
@@ -941,14 +987,22 @@ extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, i
                               void* stream) {
     using namespace lq;
     if (!d) return LQ_ERR_NULL;
-    const RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
+    RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
                                      T, scale);
     const int rc = rule_check(d, P);
     if (rc || N == 0 || T == 0) return rc;
     if (!cu) return LQ_ERR_NULL;
+    // The lengths are on the device: a batch gets both kernels, and each of its sequences is run by one of them.
     const int impl = g_rule_impl.load(std::memory_order_relaxed);
-    const bool tokens = impl == 1 || (impl == 0 && T < int64_t(RULE_SHORT) * N);
-    return tokens ? launch_recurrent(P, static_cast<cudaStream_t>(stream)) : launch_chunk(P, static_cast<cudaStream_t>(stream));
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    P.shorter = impl == 1 ? T + 1 : impl == 2 ? 1 : RULE_SHORT;
+    if (T < P.shorter) return launch_recurrent(P, st);
+    if (N == 1) P.shorter = 1;                               // one kernel for one sequence
+    if (P.shorter > 1) {
+        const int rc2 = launch_recurrent(P, st);
+        if (rc2) return rc2;
+    }
+    return launch_chunk(P, st);
 }
 
 extern "C" int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,

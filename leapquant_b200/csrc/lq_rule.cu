@@ -25,6 +25,7 @@ struct RuleParams {
     int32_t NS, H, HV, N;
     int64_t T;
     float scale;
+    int64_t shorter;                  // rule_recurrent_kernel takes the sequences with fewer tokens, rule_chunk_kernel the others
 };
 
 // log(1 + e^x) to fp32 precision for every x: 1 + e^x alone would cut e^x off at 2^-24, and a layer that starts with steps of a
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(32 * RW_WARPS) rule_recurrent_kernel(RuleParam
     const int v0 = (part * RW_WARPS + warp) * RW_ROWS;
     int64_t t0, len;
     rule_span(P, n, t0, len);
-    if (len == 0) return;
+    if (len == 0 || len >= P.shorter) return;
     const int slot = P.idx[n];
     const bool ours = slot > 0 && slot < P.NS;
     const int c = 4 * (lane & 7), r8 = lane >> 3;

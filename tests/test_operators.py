@@ -163,6 +163,19 @@ def test_prefill_strides(kw, impl):
     clean()
 
 
+@gpu
+@pytest.mark.parametrize("lens", [[18], [20], [1, 30, 5, 64, 19, 20, 21, 0, 100, 1], [(7 * i) % 45 for i in range(150)], [3] * 140 + [70]],
+                         ids=["18", "20", "mixed", "150", "141"])
+def test_prefill_batches_of_short_and_long_sequences(lens):
+    """What a caller gets by default: each sequence in the form that suits its length, in batches that are ranked by it and larger ones."""
+    n = len(lens)
+    slots = [(i * 7) % n + 1 if n % 7 else i + 1 for i in range(n)]
+    S, S64, o, o64, size = run_rule(1, 2, lens, slots, n + 1, seed=n, fresh=[i % 3 == 0 for i in range(n)])
+    check_rule(S, S64, o, o64, size, max(lens))
+    assert bool((o[sum(lens):] == 7.0).all())
+    clean()
+
+
 def same_keys(mixed, a, b, A_log, dt_bias):
     mixed[:, 256:512] = mixed[0, 256:512]                    # H = 2: every key the same, every step written in full
     b.fill_(8.0)
