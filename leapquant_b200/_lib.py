@@ -115,32 +115,30 @@ def conv1d(x, conv_state, weight, bias):
 
 def same_device(t, *others):
     """Refuses host tensors, and tensors on different devices."""
-    if not t.is_cuda:
+    d = t.get_device()                                       # -1: not on a CUDA device
+    if d < 0:
         not_cuda()
     for x in others:
-        if x is not None and x.device != t.device:
+        if x is not None and x.get_device() != d:
             if not x.is_cuda:
                 not_cuda()
             raise LeapQuantError(f"tensors on different devices: {t.device} and {x.device}")
 
 
 def rows(t, dtype, shape, what):
-    """Element stride between the rows of `t` (first dimension), whose other dimensions have to be packed; refuses another type or
-    shape."""
-    if t.dtype != dtype or tuple(t.shape) != shape:
-        raise LeapQuantError(f"{what}: expected {dtype} {shape}, got {t.dtype} {tuple(t.shape)}")
-    n = 1
-    for size, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-        if size > 1 and stride != n:
-            raise LeapQuantError(f"{what}: the elements of a row must be contiguous, got strides {t.stride()}")
-        n *= size
-    return t.stride(0) if t.shape[0] > 1 else max(n, 1)
+    """Element stride between the rows of the matrix `t`, whose columns have to be next to one another; refuses another type or shape."""
+    if t.dtype is not dtype or t.shape != shape:
+        raise LeapQuantError(f"{what}: expected {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    s = t.stride()
+    if s[1] != 1 and shape[1] > 1:
+        raise LeapQuantError(f"{what}: the elements of a row must be contiguous, got strides {s}")
+    return s[0] if shape[0] > 1 else shape[1]
 
 
 def whole(t, dtype, shape, what):
     """Refuses a tensor that is not contiguous with this type and shape."""
-    if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous():
-        raise LeapQuantError(f"{what}: expected contiguous {dtype} {shape}, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise LeapQuantError(f"{what}: expected contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)}, strides {t.stride()}")
 
 
 def ptr(t):

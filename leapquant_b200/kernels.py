@@ -239,30 +239,30 @@ def make_lowrank(K, V, R, ITERS, threads=128):
     return lowrank
 
 
-def _rule_operands(who, dims, S0, mixed, a, b, A_log, dt_bias, idx, o):
+def _rule_operands(shape, strides, C, HV, V, S0, mixed, a, b, A_log, dt_bias, idx, o):
     """Checks the tensors that both forms of the gated delta rule take; returns the row strides of mixed, a and b."""
-    NS, HV, H, K, V, SS = dims
     T = mixed.shape[0]
     _lib.same_device(S0, mixed, a, b, A_log, dt_bias, idx, o)
-    if S0.dtype != torch.float32 or tuple(S0.shape) != (NS, HV, V, K) or S0.stride() != (SS, V * K, K, 1):
-        raise _lib.LeapQuantError(f"{who}: expected float32 states {(NS, HV, V, K)} with strides {(SS, V * K, K, 1)}, got {S0.dtype} "
+    if S0.dtype is not torch.float32 or S0.shape != shape or S0.stride() != strides:
+        raise _lib.LeapQuantError(f"gated delta rule, states: expected float32 {shape} with strides {strides}, got {S0.dtype} "
                                   f"{tuple(S0.shape)}, strides {S0.stride()}")
-    _lib.whole(o, torch.bfloat16, (T, HV, V), f"{who}, outputs")
-    _lib.whole(A_log, torch.float32, (HV,), f"{who}, A_log")
-    _lib.whole(dt_bias, torch.float32, (HV,), f"{who}, dt_bias")
-    return (_lib.rows(mixed, torch.bfloat16, (T, 2 * H * K + HV * V), f"{who}, q | k | v rows"),
-            _lib.rows(a, torch.bfloat16, (T, HV), f"{who}, a"), _lib.rows(b, torch.bfloat16, (T, HV), f"{who}, b"))
+    _lib.whole(o, torch.bfloat16, (T, HV, V), "gated delta rule, outputs")
+    _lib.whole(A_log, torch.float32, (HV,), "gated delta rule, A_log")
+    _lib.whole(dt_bias, torch.float32, (HV,), "gated delta rule, dt_bias")
+    return (_lib.rows(mixed, torch.bfloat16, (T, C), "gated delta rule, q | k | v rows"),
+            _lib.rows(a, torch.bfloat16, (T, HV), "gated delta rule, a"), _lib.rows(b, torch.bfloat16, (T, HV), "gated delta rule, b"))
 
 
-def _sequences(who, cu, idx, has_initial):
+def _sequences(cu, idx, has_initial):
     """Checks the tensors that describe packed sequences; returns their number and the address of has_initial (or None)."""
     N = idx.shape[0]
-    _lib.whole(idx, torch.int32, (N,), f"{who}, slots")
-    _lib.whole(cu, torch.int32, (N + 1,), f"{who}, offsets of the sequences")
+    _lib.whole(idx, torch.int32, (N,), "packed sequences, slots")
+    _lib.whole(cu, torch.int32, (N + 1,), "packed sequences, offsets")
     if has_initial is None:
         return N, None
-    if has_initial.dtype not in (torch.bool, torch.uint8) or tuple(has_initial.shape) != (N,) or not has_initial.is_contiguous():
-        raise _lib.LeapQuantError(f"{who}, has_initial: expected contiguous bool ({N},), got {has_initial.dtype} {tuple(has_initial.shape)}")
+    if has_initial.dtype not in (torch.bool, torch.uint8) or has_initial.shape != (N,) or not has_initial.is_contiguous():
+        raise _lib.LeapQuantError(f"packed sequences, has_initial: expected contiguous bool ({N},), got {has_initial.dtype} "
+                                  f"{tuple(has_initial.shape)}")
     return N, has_initial.data_ptr()
 
 
@@ -274,14 +274,15 @@ def make_gdn_prefill(NS, HV, H, K, V, SS, scale=None):
     state; o bf16 [T, HV, V].  A sequence without tokens touches nothing; one with idx <= 0, idx >= NS or a slot that an earlier
     one names gets zeros in o and touches no state; rows of o that no sequence owns are left as they are."""
     _need_128(K, V, "make_gdn_prefill")
-    dims, d = (NS, HV, H, K, V, SS), _lib.dims(NS, HV, H, K, V, 0, 0, SS)
+    shape, strides, C = (NS, HV, V, K), (SS, V * K, K, 1), 2 * H * K + HV * V
+    d = ctypes.pointer(_lib.dims(NS, HV, H, K, V, 0, 0, SS))
     sc = float(K ** -0.5 if scale is None else scale)
     fn = _lib.lib().lq_gdn_prefill
 
     def prefill(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
-        ms, as_, bs = _rule_operands("gdn prefill", dims, S0, mixed, a, b, A_log, dt_bias, idx, o)
+        ms, as_, bs = _rule_operands(shape, strides, C, HV, V, S0, mixed, a, b, A_log, dt_bias, idx, o)
         _lib.same_device(S0, cu, has_initial)
-        N, hp = _sequences("gdn prefill", cu, idx, has_initial)
+        N, hp = _sequences(cu, idx, has_initial)
         _launch(fn, "lq_gdn_prefill", S0, d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
                 dt_bias.data_ptr(), cu.data_ptr(), idx.data_ptr(), hp, o.data_ptr(), N, mixed.shape[0], sc)
 
@@ -292,13 +293,14 @@ def make_gdn_recurrent(NS, HV, H, K, V, SS, scale=None):
     """Gated delta rule for one token per row on fp32 states.  Returns recurrent(S0, mixed, a, b, A_log, dt_bias, idx, o), the operands
     of make_gdn_prefill with T = N rows; rows with idx <= 0, idx >= NS or the slot of an earlier row write zeros and touch no state."""
     _need_128(K, V, "make_gdn_recurrent")
-    dims, d = (NS, HV, H, K, V, SS), _lib.dims(NS, HV, H, K, V, 0, 0, SS)
+    shape, strides, C = (NS, HV, V, K), (SS, V * K, K, 1), 2 * H * K + HV * V
+    d = ctypes.pointer(_lib.dims(NS, HV, H, K, V, 0, 0, SS))
     sc = float(K ** -0.5 if scale is None else scale)
     fn = _lib.lib().lq_gdn_recurrent
 
     def recurrent(S0, mixed, a, b, A_log, dt_bias, idx, o):
-        ms, as_, bs = _rule_operands("gdn recurrent", dims, S0, mixed, a, b, A_log, dt_bias, idx, o)
-        _lib.whole(idx, torch.int32, (mixed.shape[0],), "gdn recurrent, slots")
+        ms, as_, bs = _rule_operands(shape, strides, C, HV, V, S0, mixed, a, b, A_log, dt_bias, idx, o)
+        _lib.whole(idx, torch.int32, (mixed.shape[0],), "gated delta rule, slots")
         _launch(fn, "lq_gdn_recurrent", S0, d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
                 dt_bias.data_ptr(), idx.data_ptr(), o.data_ptr(), mixed.shape[0], sc)
 
@@ -315,7 +317,7 @@ def make_conv1d_prompt(NS, channels):
 
     def prompt(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out):
         _lib.same_device(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out)
-        N, hp = _sequences("conv1d prompt", cu, idx, has_initial)
+        N, hp = _sequences(cu, idx, has_initial)
         if x.dim() != 2 or x.shape[1] < channels or tuple(conv_weight.shape) != (channels, 4) or conv_state.shape[:2] != (NS, channels) or (
                 conv_bias is not None and tuple(conv_bias.shape) != (channels,)):
             raise _lib.LeapQuantError(f"conv1d prompt: x {tuple(x.shape)}, state {tuple(conv_state.shape)}, weight {tuple(conv_weight.shape)} "
@@ -364,10 +366,11 @@ def make_add_norm(D, eps=1e-6, scale=1.0):
     def norm(x, residual, weight, y):
         _lib.same_device(x, residual, weight, y)
         T = x.shape[0]
-        strides = [_lib.rows(t, torch.bfloat16, (T, D), f"add norm, {n}") for t, n in ((x, "x"), (residual, "residual"), (y, "y"))]
+        shape = (T, D)
+        xs, rs = _lib.rows(x, torch.bfloat16, shape, "add norm, x"), _lib.rows(residual, torch.bfloat16, shape, "add norm, residual")
+        ys = _lib.rows(y, torch.bfloat16, shape, "add norm, y")
         _lib.whole(weight, torch.bfloat16, (D,), "add norm, weight")
-        _launch(fn, "lq_add_norm", x, x.data_ptr(), strides[0], residual.data_ptr(), strides[1], weight.data_ptr(), y.data_ptr(),
-                strides[2], T, D, scale, eps)
+        _launch(fn, "lq_add_norm", x, x.data_ptr(), xs, residual.data_ptr(), rs, weight.data_ptr(), y.data_ptr(), ys, T, D, scale, eps)
 
     return norm
 
