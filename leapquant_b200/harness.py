@@ -8,7 +8,9 @@ It exists to compare, end to end and on identical weights and prompts, the 8-bit
 (`state="fp32"`: vLLM's own conv1d-update and packed-decode kernels on an fp32 state, where that vLLM is importable; else
 flash-linear-attention's recurrent kernel).  Everything that is not the recurrent state path -- projections, attention
 over a KV cache, MLP, norms, sampling, the chunked prefill of the delta rule -- is plain PyTorch or library code: it is the
-same in both arms and is not what this package accelerates.  The reference plugs into vLLM for this (leapquant/vllm/gdn.py);
+same in both arms and is not what this package accelerates.  With `operators="own"` a GDN layer's prompt (conv1d, chunked delta
+rule), its gated norm and the residual norms of all layers run on this package's kernels instead, and so does the decode on the fp32
+state: then nothing of a GDN layer but its projections is library code.  The reference plugs into vLLM for this (leapquant/vllm/gdn.py);
 the vLLM it pins is not the one of this image, so the model loop is written out here.
 
 The only communication is the tensor-parallel all-reduce (and the arg-max exchange of the sharded LM head); the recurrent
@@ -54,8 +56,8 @@ def rms_norm(x, weight, eps=1e-6):
 class HybridTP:
     """One rank's shard of the model, its KV cache, its recurrent states and its prefill / decode loops."""
 
-    def __init__(self, cfg, rank, world, device, state, batch, max_len):
-        assert state in ("int8", "fp32")
+    def __init__(self, cfg, rank, world, device, state, batch, max_len, operators="library"):
+        assert state in ("int8", "fp32") and operators in ("library", "own")
         self.cfg, self.rank, self.world, self.dev, self.state_mode = cfg, rank, world, device, state
         self.B, self.max_len = batch, max_len
         c = cfg
@@ -99,8 +101,16 @@ class HybridTP:
         ang = torch.arange(max_len, device=device).float()[:, None] * inv[None]
         self.cos, self.sin = ang.cos().to(torch.bfloat16), ang.sin().to(torch.bfloat16)
         self.slots = torch.arange(1, batch + 1, dtype=torch.int32, device=device)
+        self.own = operators == "own"
         self.fp32_kernels = None
-        if state == "fp32":
+        if self.own:
+            from . import kernels as KN
+            NS, D = batch + 1, self.D
+            self.k_gated_norm, self.k_add_norm = KN.make_gated_norm(D), KN.make_add_norm(hid)
+            self.k_conv_prompt, self.k_conv = KN.make_conv1d_prompt(NS, self.C), KN.make_conv1d_update(NS, self.C)
+            self.k_prefill = KN.make_gdn_prefill(NS, self.HV, self.H, D, D, self.HV * D * D)
+            self.k_recurrent = KN.make_gdn_recurrent(NS, self.HV, self.H, D, D, self.HV * D * D)
+        elif state == "fp32":
             self.fp32_kernels = self._find_fp32_kernels()
         self.lq = {}
         self.kv_attention = self._find_kv_attention()
@@ -138,6 +148,35 @@ class HybridTP:
         g, u = gu.split(self.mlp_l, -1)
         return self.all_reduce(F.linear(F.silu(g) * u, p["down"]))
 
+    def gated_norm(self, p, o, z):
+        """RMS norm of the heads' outputs o [rows, HV, D], times silu of the gate z [rows, HV * D] -> [rows, HV * D]."""
+        if self.own:
+            self.k_gated_norm(o, z, p["gnorm"], o)
+            return o.reshape(o.shape[0], -1)
+        return (rms_norm(o, p["gnorm"]) * F.silu(z.reshape(o.shape))).reshape(o.shape[0], -1)
+
+    def add_norm(self, x, y, weight):
+        """x + y and its RMS norm.  (own: x is updated in place, and the norm is that of the sum before its rounding.)"""
+        if self.own:
+            h = torch.empty_like(x)
+            self.k_add_norm(y.view(-1, self.cfg.hidden), x.view(-1, self.cfg.hidden), weight, h.view(-1, self.cfg.hidden))
+            return x, h
+        x = x + y
+        return x, rms_norm(x, weight)
+
+    def prompt_own(self, p, qkvz, b_, a_, lo):
+        """Raw projections [n, T, C + HV D] of the fresh prompts in the slots from lo + 1 on -> outputs [n T, HV, D]; conv and recurrent
+        states are left in their slots."""
+        n, T = qkvz.shape[:2]
+        rows = qkvz.view(n * T, -1)
+        cu = torch.arange(n + 1, dtype=torch.int32, device=self.dev) * T
+        slots, fresh = self.slots[lo:lo + n], torch.zeros(n, dtype=torch.bool, device=self.dev)
+        mixed = torch.empty(n * T, self.C, dtype=torch.bfloat16, device=self.dev)
+        o = torch.empty(n * T, self.HV, self.D, dtype=torch.bfloat16, device=self.dev)
+        self.k_conv_prompt(rows[:, : self.C], p["conv"].transpose(-1, -2), p["conv_w"], p["conv_b"], cu, slots, fresh, mixed)
+        self.k_prefill(p["ssm"], mixed, a_.reshape(n * T, self.HV), b_.reshape(n * T, self.HV), p["A_log"], p["dt_bias"], cu, slots, fresh, o)
+        return o
+
     @staticmethod
     def _find_fp32_kernels():
         try:
@@ -158,7 +197,8 @@ class HybridTP:
     @torch.no_grad()
     def prefill(self, tokens, seqs_per_pass=8):
         """tokens [B, T] -> next token ids [B] (greedy).  Fills the KV caches, the conv states and the recurrent states."""
-        from fla.ops.gated_delta_rule import chunk_gated_delta_rule
+        if not self.own:
+            from fla.ops.gated_delta_rule import chunk_gated_delta_rule
         B, T = tokens.shape
         last = torch.empty(B, self.cfg.hidden, dtype=torch.bfloat16, device=self.dev)
         pos = torch.arange(T, device=self.dev)
@@ -166,9 +206,13 @@ class HybridTP:
             b1 = min(B, b0 + seqs_per_pass)
             n = b1 - b0
             x = self.embed[tokens[b0:b1]]                                            # [n, T, hid]
+            h = rms_norm(x, self.layers[0]["norm1"])
             for l, p in enumerate(self.layers):
-                h = rms_norm(x, p["norm1"])
-                if p["kind"] == "gdn":
+                if p["kind"] == "gdn" and self.own:
+                    qkvz, ba = F.linear(h, p["in_qkvz"]), F.linear(h, p["in_ba"])
+                    o = self.prompt_own(p, qkvz, ba[..., : self.HV], ba[..., self.HV:], b0)
+                    y = F.linear(self.gated_norm(p, o, qkvz.view(n * T, -1)[:, self.C:]), p["out"]).view(n, T, -1)
+                elif p["kind"] == "gdn":
                     qkvz = F.linear(h, p["in_qkvz"])
                     raw, z = qkvz[..., : self.C], qkvz[..., self.C:]
                     ba = F.linear(h, p["in_ba"])
@@ -200,8 +244,12 @@ class HybridTP:
                     o = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
                     o = o.transpose(1, 2) * torch.sigmoid(qg[:, :, 1].float()).to(o.dtype)
                     y = F.linear(o.reshape(n, T, -1), p["out"])
-                x = x + self.all_reduce(y)
-                x = x + self.mlp(p, rms_norm(x, p["norm2"]))
+                x, h = self.add_norm(x, self.all_reduce(y), p["norm2"])
+                y = self.mlp(p, h)
+                if l + 1 < len(self.layers):
+                    x, h = self.add_norm(x, y, self.layers[l + 1]["norm1"])
+                else:
+                    x = x + y
             last[b0:b1] = x[:, -1]
         if self.state_mode == "int8":
             for l, p in enumerate(self.layers):
@@ -229,8 +277,8 @@ class HybridTP:
         """tokens [B] int64, pos [B] int64 (their positions) -> next tokens [B].  No host synchronisation: capturable."""
         B = self.B
         x = self.embed[tokens]
+        h = rms_norm(x, self.layers[0]["norm1"])
         for l, p in enumerate(self.layers):
-            h = rms_norm(x, p["norm1"])
             if p["kind"] == "gdn":
                 qkvz = F.linear(h, p["in_qkvz"])
                 raw, z = qkvz[:, : self.C], qkvz[:, self.C:]
@@ -241,6 +289,10 @@ class HybridTP:
                 if self.state_mode == "int8":
                     self.lq_state(l).decode_conv(p["ssm"], raw, conv_view, p["conv_w"], p["conv_b"], a_, b_, p["A_log"], p["dt_bias"],
                                                  self.slots, o)
+                elif self.own:
+                    mixed = torch.empty(B, self.C, dtype=torch.bfloat16, device=self.dev)
+                    self.k_conv(raw, conv_view, p["conv_w"], p["conv_b"], self.slots, mixed)
+                    self.k_recurrent(p["ssm"], mixed, a_, b_, p["A_log"], p["dt_bias"], self.slots, o)
                 else:
                     kind, conv, dec = self.fp32_kernels
                     if kind == "vllm":
@@ -261,8 +313,7 @@ class HybridTP:
                                     output_final_state=True, use_qk_l2norm_in_kernel=True)
                         p["ssm"][1:] = S.transpose(-1, -2)
                         o = oo[:, 0]
-                o = rms_norm(o, p["gnorm"]) * F.silu(z.reshape(B, self.HV, self.D))
-                y = F.linear(o.reshape(B, -1), p["out"])
+                y = F.linear(self.gated_norm(p, o, z), p["out"])
             else:
                 qg = F.linear(h, p["q"]).reshape(B, 2, self.QH, self.AD)
                 kv = F.linear(h, p["kv"]).reshape(B, 2, self.KVH, self.AD)
@@ -279,17 +330,21 @@ class HybridTP:
                     o = F.scaled_dot_product_attention(q[:, :, None], p["kc"], p["vc"], attn_mask=mask, enable_gqa=True)[:, :, 0]
                 o = o * torch.sigmoid(qg[:, 1].float()).to(o.dtype)
                 y = F.linear(o.reshape(B, -1), p["out"])
-            x = x + self.all_reduce(y)
-            x = x + self.mlp(p, rms_norm(x, p["norm2"]))
+            x, h = self.add_norm(x, self.all_reduce(y), p["norm2"])
+            y = self.mlp(p, h)
+            if l + 1 < len(self.layers):
+                x, h = self.add_norm(x, y, self.layers[l + 1]["norm1"])
+            else:
+                x = x + y
         return self.sample(x)
 
 
-def run_generation(cfg, state, batch, prompt_len, new_tokens, seed=0, use_graph=True):
+def run_generation(cfg, state, batch, prompt_len, new_tokens, seed=0, use_graph=True, operators="library"):
     """Greedy generation on random prompts; returns a dict with times (device-timed, max over ranks) and throughput."""
     world = dist.get_world_size() if dist.is_initialized() else 1
     rank = dist.get_rank() if dist.is_initialized() else 0
     dev = torch.device("cuda", torch.cuda.current_device())
-    model = HybridTP(cfg, rank, world, dev, state, batch, prompt_len + new_tokens + 1)
+    model = HybridTP(cfg, rank, world, dev, state, batch, prompt_len + new_tokens + 1, operators)
     g = torch.Generator(device="cpu").manual_seed(seed)
     prompts = torch.randint(0, cfg.vocab, (batch, prompt_len), generator=g).to(dev)
     ev = lambda: torch.cuda.Event(enable_timing=True)
@@ -348,7 +403,7 @@ def run_generation(cfg, state, batch, prompt_len, new_tokens, seed=0, use_graph=
     if world > 1:
         dist.all_reduce(t, op=dist.ReduceOp.MAX)
     t_prefill, t_decode = float(t[0]), float(t[1])
-    return {"state": state, "fp32_kernels": model.fp32_kernels[0] if model.fp32_kernels else None, "decode_mode": mode,
+    return {"state": state, "operators": operators, "fp32_kernels": model.fp32_kernels[0] if model.fp32_kernels else None, "decode_mode": mode,
             "attention": "flash_attn_with_kvcache" if model.kv_attention is not None else "torch sdpa, masked",
             "prefill_s": t_prefill, "decode_s": t_decode, "decode_steps_timed": steps, "ms_per_decode_step": 1e3 * t_decode / max(steps, 1),
             "decode_tokens_per_s": batch * steps / t_decode if steps else None, "first_tokens": first[:8].tolist(),

@@ -472,6 +472,34 @@ def test_layer_prompt_then_decode():
     clean()
 
 
+@gpu
+@pytest.mark.parametrize("state", ["fp32", "int8"])
+def test_harness_on_own_operators(state):
+    """The hybrid model with every operator of its GDN layers from this package: a prompt in one call leaves the states that its tokens
+    leave one by one, and generation runs in a CUDA graph.  (Two paths through bf16 layers: they agree to the roundings of a few layers,
+    2^-8 each, not to the bit.)"""
+    from leapquant_b200.harness import HybridConfig, HybridTP, run_generation
+    cfg = HybridConfig(hidden=256, layers=4, gdn_key_heads=2, gdn_value_heads=4, attn_q_heads=2, attn_kv_heads=1, mlp=512, vocab=512, window=16)
+    B, T = 3, 75
+    dev = torch.device("cuda", 0)
+    tokens = torch.randint(0, cfg.vocab, (B, T), generator=torch.Generator().manual_seed(2)).cuda()
+    whole = HybridTP(cfg, 0, 1, dev, "fp32", B, T + 2, operators="own")
+    whole.prefill(tokens)
+    single = HybridTP(cfg, 0, 1, dev, "fp32", B, T + 2, operators="own")
+    for t in range(T):
+        single.decode_step(tokens[:, t], torch.full((B,), t, dtype=torch.int64, device=dev))
+    for l, (p, q) in enumerate(zip(whole.layers, single.layers)):
+        if p["kind"] == "gdn":
+            for name in ("ssm", "conv"):
+                x, y = p[name][1:].double(), q[name][1:].double()
+                assert float((x - y).norm() / y.norm()) <= (4 * l + 2) * 2.0 ** -8, (l, name)
+            assert float(p["ssm"][0].abs().max()) == 0.0, "the null slot"
+    got = run_generation(cfg, state, batch=B, prompt_len=40, new_tokens=20, operators="own")
+    assert got["decode_mode"] == "cuda_graph", got["decode_mode"]
+    assert all(0 <= i < cfg.vocab for i in got["last_tokens"])
+    clean()
+
+
 # ---- refusals ----
 def test_argument_errors_are_codes():
     from leapquant_b200 import _lib
