@@ -24,10 +24,13 @@
 
 namespace lq {
 
-// Sequences of fewer tokens are run token by token, longer ones in chunks.  A chunk costs a CTA 18 us however many tokens it has, the
-// recurrence about 0.8 us a token once every SM has heads: 12 tokens of 64 sequences of 32 heads 155 against 261 us, 24 tokens 297 against 263;
-// one sequence, 16 tokens 15.1 against 19.2 us, 24 tokens 19.8 against 18.9.
-constexpr int RULE_SHORT = 20;
+// Sequences of fewer tokens are run token by token, longer ones in chunks.  A chunk costs a CTA 20 us however many tokens it has, the
+// recurrence 8.6 us a token of 64 sequences of 32 heads and 0.45 us of one sequence, which leaves most of the device idle either way:
+//     tokens                          24          28          32          40
+//     64 sequences, 32 heads      212 : 281   248 : 283   283 : 284   353 : 284   us, token by token : in chunks
+//      8 sequences, 32 heads       35 :  39    40 :  39    45 :  39    55 :  39
+//      one sequence, 32 heads      14 :  20    16 :  20    19 :  20    21 :  20
+constexpr int RULE_SHORT = 28;
 constexpr int RANKED = 128;                                  // batches up to which CTAs take the longest sequences first
 constexpr int CT = 64;                                       // tokens of a chunk
 // T and A lie within [-1, 1]; times 2^13 their small entries keep eleven bits down to 2^-27 as well
@@ -818,21 +821,29 @@ __device__ __forceinline__ int ck_sequence(ChunkSmem& s, const RuleParams& P, in
             for (int m = 0; m < P.N; ++m) rank += s.len[m] > mine || (s.len[m] == mine && m < tid);
             if (rank == r) s.seq = tid;
         }
-    } else {
+    } else {                                                 // every warp counts in a part of its own, and the one that has the r-th looks for it
+        const int lane = tid & 31, warp = tid >> 5, per = (P.N / (CK_THREADS / 32) + 32) & ~31, lo = warp * per, hi = P.N - lo < per ? P.N : lo + per;
+        int count = 0;
+#pragma unroll 4
+        for (int m = lo + lane; m < hi; m += 32) {
+            rule_span(P, m, t0, len);
+            count += len >= P.shorter;
+        }
+        count = __reduce_add_sync(0xffffffffu, count);
+        if (lane == 0) s.len[warp] = count;
         __syncthreads();
-        if (tid < 32) {
+        for (int w = 0; w < warp; ++w) r -= s.len[w];
+        if (r >= 0 && r < count) {
 #pragma unroll 1
-            for (int base = 0; base < P.N; base += 32) {
+            for (int base = lo; r >= 0; base += 32) {
                 bool in = false;
-                if (base + tid < P.N) {
-                    rule_span(P, base + tid, t0, len);
+                if (base + lane < hi) {
+                    rule_span(P, base + lane, t0, len);
                     in = len >= P.shorter;
                 }
                 const unsigned got = __ballot_sync(0xffffffffu, in);
-                const int before = __popc(got & ((1u << tid) - 1));
-                if (in && before == r) s.seq = base + tid;
+                if (in && __popc(got & ((1u << lane) - 1)) == r) s.seq = base + lane;
                 r -= __popc(got);
-                if (r < 0) break;
             }
         }
     }
@@ -916,7 +927,7 @@ static int rule_check(const lq_dims* d, const RuleParams& P) {
     if (d->K != KD || d->V != VD) return LQ_ERR_UNSUPPORTED;
     if (d->NS < 1 || d->HV < 1 || d->H < 1 || d->HV % d->H != 0 || d->SS < int64_t(d->HV) * d->V * d->K) return LQ_ERR_RANGE;
     if (d->SS & 3) return LQ_ERR_ALIGN;
-    if (P.N < 0 || P.T < 0) return LQ_ERR_RANGE;
+    if (P.N < 0 || P.T < 0 || P.T > 0x7fffffff) return LQ_ERR_RANGE;              // (offsets and coordinates of the tensor maps: 32 bits)
     if (P.N == 0 || P.T == 0) return LQ_OK;
     if (!P.ssm || !P.mixed || !P.a || !P.b || !P.A_log || !P.dt_bias || !P.idx || !P.o) return LQ_ERR_NULL;
     if (P.mixed_stride < 2 * int64_t(d->H) * KD + int64_t(d->HV) * VD || P.a_stride < d->HV || P.b_stride < d->HV) return LQ_ERR_RANGE;
@@ -949,7 +960,6 @@ static int encode_rows(CUtensorMap* m, const void* base, int64_t rows, int64_t c
 static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     constexpr size_t smem = sizeof(ChunkSmem) + 1024;
     static_assert(smem <= 227 * 1024, "the working set of a CTA");
-    if (P.T > 0x7fffffff) return LQ_ERR_RANGE;               // (coordinates of the tensor maps)
     CUtensorMap rows, outs;
     int rc = encode_rows(&rows, P.mixed, P.T, 2 * int64_t(P.H) * KD + int64_t(P.HV) * VD, P.mixed_stride, 64, CU_TENSOR_MAP_SWIZZLE_128B);
     if (!rc) rc = encode_rows(&outs, P.o, P.T, int64_t(P.HV) * VD, int64_t(P.HV) * VD, VD, CU_TENSOR_MAP_SWIZZLE_NONE);
