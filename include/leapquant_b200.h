@@ -67,7 +67,7 @@ int lq_device_status(int* status);
  * (row, head) in registers (GDN only; KDA keeps the default).  1 and 2 exist for debugging and comparison.
  * "pdl": 1 (default) launches the step and flush kernels with programmatic stream serialisation, so that the launch and
  * set-up of one overlap the tail of its predecessor on the stream; 0 = plain launches.
- * "rule_impl": how lq_gdn_prefill works: 0 = by the mean length of the sequences (default), 1 = token by token, 2 = in chunks.
+ * "rule_impl": how lq_gdn_prefill works: 0 = each sequence by its length (default), 1 = token by token, 2 = in chunks.
  * "work_list_min_programs": the fewest (row, head) programs of a fused decode call for which the `work` list passed to it
  * is used (-1 = default, sixteen per SM; 0 = whenever `work` is given).  The mailboxes cost an atomic round trip or two
  * per launch and save the flush of one head when the due heads sit unevenly on the CTAs. */
@@ -226,7 +226,7 @@ int lq_lowrank(const float* x, const float* Q0, float* U, float* Q, int32_t n, i
  *   - has_initial (u8 [N], may be NULL = all): 0 starts the sequence from a zero state instead of its slot's.
  *   - A sequence without tokens touches nothing.  idx[n] <= 0 or >= NS, or a slot that an earlier entry names too: padding, the
  *     sequence's rows of o are zeros and no state is touched.  Rows of o that no sequence owns are left as they are.  Offsets
- *     outside 0 .. T are cut to it. */
+ *     outside 0 .. T are cut to it.  o must not overlap mixed, a or b (LQ_ERR_RANGE). */
 int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                    const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
                    const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale, void* stream);
@@ -237,17 +237,18 @@ int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mi
 /* Causal conv1d + SiLU of packed prompts: per sequence and channel, with the inputs before the sequence's first token from its slot
  * (zeros where has_initial[n] is 0),  out[t] = silu(bias + sum_j weight[j] in[t - 3 + j])  in fp32, rounded once; the slot's state
  * becomes the last three inputs.  conv: the operands of lq_causal_conv1d_update, x with T rows; cu, idx, has_initial as above;
- * out bf16 [T, out_stride], not overlapping x.  Sequences without tokens or with a padding slot are skipped (nothing read or
+ * out bf16 [T, out_stride], not overlapping x (LQ_ERR_RANGE; columns of one buffer next to one another are fine).  Sequences without tokens or with a padding slot are skipped (nothing read or
  * written).  channels must be a multiple of 8 and bias 16-byte aligned. */
 int lq_causal_conv1d_prompt(const lq_conv1d* conv, const int32_t* cu, const int32_t* idx, const uint8_t* has_initial, int32_t N,
                             int64_t T, int32_t channels, int32_t NS, void* out, int64_t out_stride, void* stream);
 /* Gated RMS norm of the rule's output: y = o / sqrt(mean(o^2) + eps) * weight * silu(z) over every head's V = 128 values, in fp32,
- * rounded once.  o, y bf16 [T, HV, V] contiguous (y may be o); z bf16 [T, HV * V] with row stride z_stride; weight bf16 [V]. */
+ * rounded once.  o, y bf16 [T, HV, V] contiguous (y may be o, and overlaps
+ * nothing else: LQ_ERR_RANGE); z bf16 [T, HV * V] with row stride z_stride; weight bf16 [V]. */
 int lq_gated_norm(const void* o, const void* z, int64_t z_stride, const void* weight, void* y, int64_t T, int32_t HV, int32_t V,
                   float eps, void* stream);
 /* Residual and RMS norm: h = residual + scale x (fp32);  residual <- bf16(h);  y = h / sqrt(mean(h^2) + eps) * weight.
  * All bf16 [T, D] with row strides in elements (multiples of 8); weight bf16 [D]; D a multiple of 8 up to LQ_NORM_MAX_DIM.
- * y may be x, not residual. */
+ * y may be x, x may be residual; any other overlap is LQ_ERR_RANGE. */
 #define LQ_NORM_MAX_DIM 16384
 int lq_add_norm(const void* x, int64_t x_stride, void* residual, int64_t r_stride, const void* weight, void* y, int64_t y_stride,
                 int64_t T, int32_t D, float scale, float eps, void* stream);

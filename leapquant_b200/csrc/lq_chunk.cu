@@ -933,6 +933,10 @@ static int rule_check(const lq_dims* d, const RuleParams& P) {
     if (P.mixed_stride < 2 * int64_t(d->H) * KD + int64_t(d->HV) * VD || P.a_stride < d->HV || P.b_stride < d->HV) return LQ_ERR_RANGE;
     if ((P.mixed_stride & 7) || misaligned16({P.ssm, P.mixed, P.o})) return LQ_ERR_ALIGN;
     if (int64_t(P.N) * d->HV > (int64_t(1) << 29)) return LQ_ERR_RANGE;            // programs: the grid's first dimension
+    const int64_t ow = int64_t(d->HV) * VD;                  // (the outputs of a head are written while another's rows are still read)
+    if (rows_overlap(P.o, ow, ow, P.mixed, P.mixed_stride, 2 * int64_t(d->H) * KD + ow, P.T) ||
+        rows_overlap(P.o, ow, ow, P.a, P.a_stride, d->HV, P.T) || rows_overlap(P.o, ow, ow, P.b, P.b_stride, d->HV, P.T))
+        return LQ_ERR_RANGE;
     return LQ_OK;
 }
 static int launch_recurrent(const RuleParams& P, cudaStream_t st) {
@@ -999,9 +1003,9 @@ extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, i
     if (!d) return LQ_ERR_NULL;
     RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
                                      T, scale);
+    if (N > 0 && T > 0 && !cu) return LQ_ERR_NULL;
     const int rc = rule_check(d, P);
     if (rc || N == 0 || T == 0) return rc;
-    if (!cu) return LQ_ERR_NULL;
     // The lengths are on the device: a batch gets both kernels, and each of its sequences is run by one of them.
     const int impl = g_rule_impl.load(std::memory_order_relaxed);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

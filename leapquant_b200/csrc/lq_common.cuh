@@ -214,6 +214,16 @@ inline bool misaligned16(std::initializer_list<const void*> ptrs) {
     return (acc & 15) != 0;
 }
 void set_last_cuda_error(cudaError_t e);
+// true if two matrices of `rows` rows of aw and bw 16-bit elements, as and bs apart, have an element in common.  Matrices with the same
+// row stride may be columns of one buffer; with different ones they count as overlapping if their address ranges do.
+inline bool rows_overlap(const void* a, int64_t as, int64_t aw, const void* b, int64_t bs, int64_t bw, int64_t rows) {
+    const int64_t pa = int64_t(reinterpret_cast<uintptr_t>(a)), pb = int64_t(reinterpret_cast<uintptr_t>(b));
+    if (pa + 2 * ((rows - 1) * as + aw) <= pb || pb + 2 * ((rows - 1) * bs + bw) <= pa) return false;
+    if (as != bs || ((pb - pa) & 1)) return true;
+    int64_t d = (pb - pa) / 2 % as;                          // columns from a's first to b's first
+    if (d < 0) d += as;
+    return d < aw || d + bw > as;
+}
 
 // Programmatic dependent launch.  The decode path is a chain of short kernels on one stream (step, flush, step, ...); a
 // kernel launched with this attribute may be scheduled while its predecessor is still draining, runs its set-up

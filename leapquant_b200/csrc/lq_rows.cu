@@ -274,6 +274,7 @@ extern "C" int lq_causal_conv1d_prompt(const lq_conv1d* conv, const int32_t* cu,
     if ((conv->x_stride & 7) || (out_stride & 7) || misaligned16({conv->x, conv->weight, conv->bias, out})) return LQ_ERR_ALIGN;
     if (reinterpret_cast<uintptr_t>(conv->state) & 7) return LQ_ERR_ALIGN;
     if (conv->stride_dim == 1 && ((conv->stride_tap & 3) || (conv->stride_slot & 3))) return LQ_ERR_ALIGN;
+    if (rows_overlap(conv->x, conv->x_stride, channels, out, out_stride, channels, T)) return LQ_ERR_RANGE;
     const int64_t blocks = T / CP_TOKENS + N + 1;
     if (blocks > 0x7fffffff || (channels + 4 * CP_THREADS - 1) / (4 * CP_THREADS) > 65535) return LQ_ERR_RANGE;
     ConvPromptParams P;
@@ -296,6 +297,8 @@ extern "C" int lq_gated_norm(const void* o, const void* z, int64_t z_stride, con
     if (!o || !z || !weight || !y) return LQ_ERR_NULL;
     if (z_stride < int64_t(HV) * V) return LQ_ERR_RANGE;
     if ((z_stride & 7) || misaligned16({o, z, weight, y})) return LQ_ERR_ALIGN;
+    const int64_t width = int64_t(HV) * V;
+    if ((y != o && rows_overlap(y, width, width, o, width, width, T)) || rows_overlap(y, width, width, z, z_stride, width, T)) return LQ_ERR_RANGE;
     const int64_t rows = T * HV, blocks = (rows + 16 * GN_ROWS - 1) / (16 * GN_ROWS);
     if (blocks > 0x7fffffff) return LQ_ERR_RANGE;
     const cudaError_t e = launch_dependent(gated_norm_kernel, unsigned(blocks), 256, 0, static_cast<cudaStream_t>(stream),
@@ -314,6 +317,10 @@ extern "C" int lq_add_norm(const void* x, int64_t x_stride, void* residual, int6
     if (!x || !residual || !weight || !y) return LQ_ERR_NULL;
     if (x_stride < D || r_stride < D || y_stride < D) return LQ_ERR_RANGE;
     if (((x_stride | r_stride | y_stride) & 7) || misaligned16({x, residual, weight, y})) return LQ_ERR_ALIGN;
+    const auto apart = [&](const void* a, int64_t as, const void* b, int64_t bs) { return !rows_overlap(a, as, D, b, bs, D, T); };
+    if (!apart(y, y_stride, residual, r_stride) || !(apart(y, y_stride, x, x_stride) || (y == x && y_stride == x_stride)) ||
+        !(apart(x, x_stride, residual, r_stride) || (x == residual && x_stride == r_stride)))
+        return LQ_ERR_RANGE;
     const int vecs = D / 8;
     const int nv = vecs > 1024 ? 2 : 1;
     const unsigned threads = unsigned(((vecs + nv - 1) / nv + 31) / 32 * 32);

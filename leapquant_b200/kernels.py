@@ -357,7 +357,7 @@ def make_gated_norm(V, eps=1e-6):
 def make_add_norm(D, eps=1e-6, scale=1.0):
     """Residual stream and the norm that the next block reads.  Returns norm(x, residual, weight, y): residual <- residual + scale x;
     y = residual / sqrt(mean(residual^2) + eps) * weight, of the fp32 sum.  x, residual, y bf16 [T, D] (row strides free; y may be
-    x), weight bf16 [D]."""
+    x, but overlaps neither otherwise), weight bf16 [D]."""
     if D < 8 or D % 8 or D > 16384:
         raise NotImplementedError(f"make_add_norm: D = {D}; a multiple of 8 up to 16384 is supported")
     eps, scale = float(eps), float(scale)

@@ -541,6 +541,29 @@ def test_argument_errors_are_codes():
     assert an(x=None) == -1 and an(r=None) == -1 and an(xs=56) == -4 and an(ys=68) == -3 and an(r=mis) == -3
 
 
+def test_overlapping_operands_are_refused():
+    """Each call would launch if its operands were apart, and does not."""
+    from leapquant_b200 import _lib
+    L, P = _lib.lib(), ctypes.c_void_p
+    at = lambda i: P((1 << 20) + 2 * i)                      # element i of a buffer that is never read
+    far = P(1 << 40)
+    d = _lib.dims(8, 4, 2, 128, 128, 0, 0, 4 * 128 * 128)
+    C, W, T = 1024, 512, 100
+    for k in (0, 512, C - 8, C * (T - 1)):                   # outputs within the rows, in the last row
+        assert L.lq_gdn_prefill(d, far, at(0), C, far, 4, far, 4, far, far, far, far, None, at(k), 1, T, 0.0, None) == -4, k
+        assert L.lq_gdn_recurrent(d, far, at(0), C, far, 4, far, 4, far, far, far, at(k), T, 0.0, None) == -4, k
+    assert L.lq_gdn_prefill(d, far, far, C, at(8), 4, far, 4, far, far, far, far, None, at(0), 1, T, 0.0, None) == -4
+    assert L.lq_gdn_prefill(d, far, far, C, far, 4, at(W * T - 8), 4, far, far, far, far, None, at(0), 1, T, 0.0, None) == -4
+    for xs, os_, k in ((64, 64, 0), (64, 64, 8), (64, 64, -64), (64, 128, 64 * (T - 1)), (256, 256, 56), (256, 256, 200), (256, 256, -256 - 56)):
+        cv = _lib.LqConv1d(at(0), xs, far, 192, 1, 64, far, None, 4)
+        assert L.lq_causal_conv1d_prompt(cv, far, far, None, 1, T, 64, 4, at(k), os_, None) == -4, (xs, os_, k)
+    gn = lambda o, z, y, zs=W: L.lq_gated_norm(o, z, zs, far, y, T, 4, 128, 1e-6, None)
+    assert gn(at(0), far, at(8)) == -4 and gn(at(0), far, at(-W)) == -4 and gn(far, at(0), at(0)) == -4 and gn(far, at(0), at(W), 2 * W) == -4
+    an = lambda x, r, y, xs=64, rs=64, ys=64: L.lq_add_norm(x, xs, r, rs, P(1 << 41), y, ys, T, 64, 1.0, 1e-6, None)
+    assert an(far, at(0), at(0)) == -4 and an(at(0), far, at(8)) == -4 and an(at(0), far, at(0), xs=128) == -4 and an(at(0), at(8), far) == -4
+    assert an(far, at(0), at(64 * 99)) == -4 and an(at(0), at(40), far, xs=128, rs=128) == -4
+
+
 def test_factories_refuse_shapes_and_host_tensors():
     from leapquant_b200 import _lib, kernels as KN
     with pytest.raises(NotImplementedError):
