@@ -10,7 +10,22 @@
 // 128 rows of the tensor memory are the 128 value dimensions: a thread of the eight main warps owns half a row of the state (64
 // columns, fp32 registers) or half the tokens of a row of r, u and o, and no row needs another one.
 //     main warps   S -> f16 pieces in tensor memory (A operand); S k, S q; r -> pieces; u = T r; u -> pieces; o; S
-//     prep warps   one chunk ahead: norms, f16 rows of k and q in shared memory (B operand), K K^T and Q K^T, decays, T and A
+//     issue warp   their tensor-core instructions, the copies of v, the stores of the outputs
+//     prep warps   two groups of four, a chunk each in turn, ahead of the main warps: norms, f16 rows of k and q in shared memory
+//                  (B operand), K K^T and Q K^T, decays, T and A; rows of k and q by TMA
+//
+// What bounds it.  One sequence is a chain of chunks, and a chunk of one head is what one SM does at a time: 4.4 us (8 000 cycles), of
+// which the main chain, six hand-overs between registers, tensor memory and tensor cores, takes 6 900 by itself.  The two prep groups
+// need 16 000 for their two chunks, side by side with it.  Both are made of the same issue slots: 18 400 warp instructions a chunk, 0.5 an
+// SM quarter's cycle, in loops of 46 KB where the instruction cache holds 32 -- beyond it an instruction costs 2.7 cycles instead of
+// 1.7.  ALU 33 %, FMA 26 %, tensor pipe 25 % busy.
+//     one sequence of 8 192 tokens, 32 heads      570 us on 32 SMs
+//     16 sequences of 4 096 tokens, 32 heads    1 200 us on all, 512 heads on 148 SMs
+// On the way, one sequence of 8 192 tokens: token by token 6 750 us; in chunks with one prep group 1 920; two groups, values and outputs
+// through shared memory, instructions issued by a whole warp 810; the inverse on tensor cores, one scale per row 620; rows and outputs by
+// TMA 570.  16 sequences of 4 096: loops instead of straight code and outputs accumulated in tensor memory 1 330 -> 1 170 us.  Without gain:
+// sixteen main warps with a quarter of a row each, two accumulators for S k, loops rolled up to 38 KB (spills: 684 us), hints to
+// sleeping waits.
 //
 // Precision.  k and q are bf16 and become f16 without loss once a row is scaled by a power of two (what is lost lies 2^-25 below the
 // row's norm); an fp32 operand is the sum of two f16 pieces, 22 bits.  f16 has few exponents, so every row of S, r and u carries

@@ -28,8 +28,9 @@ __device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __e
 // cu.  The piece that holds a sequence's first token is the only reader of its conv state and writes the new one, from the last three
 // inputs, when it has read the old one: no two blocks touch a slot.
 // Memory bound, but not by far: two special functions per element alone take three quarters of the copy's time, so the kernel lives on warps
-// that overlap (32 an SM at 64 registers).  32 768 rows of 8 192 channels: 205 us, 82 % of the measured copy rate; eight channels a thread with
-// half the warps 238, four rows a batch (the past inputs have to be moved around) 229, pieces of 48 tokens 201 but twice the latency.
+// that overlap (32 an SM at 64 registers).  32 768 rows of 8 192 channels: 214 us, 77 % of the measured copy rate (205 on one input again and
+// again: what of it is still in L2); against those 205, eight channels a thread with half the warps 238, four rows a batch (the past inputs
+// have to be moved around) 229, pieces of 48 tokens 201 but twice the latency.
 constexpr int CP_TOKENS = 24, CP_BATCH = 6, CP_THREADS = 128;
 struct ConvPromptParams {
     const uint16_t* x;
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(CP_THREADS, 8) conv1d_prompt_kernel(ConvPrompt
 
 // ---- gated RMS norm of every head's output ----------------------------------------------------------------------------------
 // y = o / sqrt(mean(o^2) + eps) * w * silu(z), rows of 128: sixteen lanes share a row.  Memory bound; a thread has the loads of four rows in
-// flight.  32 768 x 32 rows: 131 us, 94 % of the measured copy rate (one row a thread 148, two 135, six 158).
+// flight.  32 768 x 32 rows: 146 us, 84 % of the measured copy rate; on one input again and again 131 (one row a thread 148, two 135, six 158).
 constexpr int GN_ROWS = 4;                                   // rows of a thread, sixteen apart
 __global__ void __launch_bounds__(256) gated_norm_kernel(const uint16_t* o, const uint16_t* z, int64_t z_stride, const uint16_t* w,
                                                          uint16_t* y, int64_t rows, int HV, float eps) {
