@@ -638,6 +638,8 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             const int en = scale_exponent(bound);
             int de = en - e;
             if (de >= 0 && de <= 3) de = 0;
+            // squares below 2^-126 are lost: a row that decayed that far within a chunk has a norm of up to sqrt(128) 2^-63, whatever the sum says
+            if (de > 60) de = 60;
             if (__any_sync(0xffffffffu, de != 0)) {
                 const float2 up = both(pow2f(de < -126 ? -126 : de > 127 ? 127 : de));
                 e += de;

@@ -222,8 +222,18 @@ def uneven_keys(mixed, a, b, A_log, dt_bias):
     mixed[:, 0:512:7] *= 2.0 ** -12                          # entries far below the others of their key
 
 
+def decayed_and_silent(mixed, a, b, A_log, dt_bias):
+    """Ten tokens that leave 2^-72 of the state, and no values: what is left of it is all there is."""
+    A_log.fill_(0.0)
+    dt_bias.fill_(0.0)
+    a.fill_(-20.0)
+    a[:10] = 5.0
+    a[150:160] = 5.0                                         # (the second sequence)
+    mixed[:, 512:] = 0
+
+
 @gpu
-@pytest.mark.parametrize("change", [same_keys, fast_decay, no_decay, large_values, small_values, large_keys, small_keys, tiny_keys,
+@pytest.mark.parametrize("change", [same_keys, fast_decay, decayed_and_silent, no_decay, large_values, small_values, large_keys, small_keys, tiny_keys,
                                     zero_rows, uneven_keys], ids=lambda f: f.__name__)
 def test_prefill_unusual_values(change, impl):
     S, S64, o, o64, size = run_rule(2, 4, [150, 66], [1, 2], 3, seed=6, fresh=[False, True], change=change)
