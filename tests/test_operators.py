@@ -223,12 +223,12 @@ def uneven_keys(mixed, a, b, A_log, dt_bias):
 
 
 def decayed_and_silent(mixed, a, b, A_log, dt_bias):
-    """Ten tokens that leave 2^-72 of the state, and no values: what is left of it is all there is."""
+    """Eleven tokens that leave 2^-79 of the state, and no values: what is left of it is all there is."""
     A_log.fill_(0.0)
     dt_bias.fill_(0.0)
     a.fill_(-20.0)
-    a[:10] = 5.0
-    a[150:160] = 5.0                                         # (the second sequence)
+    a[:11] = 5.0
+    a[150:161] = 5.0                                         # (the second sequence)
     mixed[:, 512:] = 0
 
 
