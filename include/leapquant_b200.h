@@ -229,7 +229,11 @@ int lq_lowrank(const float* x, const float* Q0, float* U, float* Q, int32_t n, i
  *     outside 0 .. T are cut to it.  o must not overlap mixed, a or b (LQ_ERR_RANGE). */
 int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                    const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
-                   const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale, void* stream);
+                   const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale, void* work,
+                   int64_t work_bytes, void* stream);
+/* Scratch with which lq_gdn_prefill splits long sequences over the SMs that N * HV heads leave idle (16-byte aligned, any contents; not
+ * shared by calls that overlap); 0 where that would not be faster.  With less than this (or NULL) a head's sequence runs on one SM. */
+int64_t lq_prefill_work_bytes(int32_t N, int32_t HV, int64_t T);
 /* The same rule for one token per row (row n is sequence n, and continues its state): the decode of states kept in fp32. */
 int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                      const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* idx, void* o,

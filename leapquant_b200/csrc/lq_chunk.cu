@@ -19,9 +19,9 @@
 // need 16 000 for their two chunks, side by side with it.  Both are made of the same issue slots: 18 400 warp instructions a chunk, 0.5 an
 // SM quarter's cycle, in loops of 46 KB where the instruction cache holds 32 -- beyond it an instruction costs 2.7 cycles instead of
 // 1.7.  ALU 33 %, FMA 26 %, tensor pipe 25 % busy.
-//     one sequence of 8 192 tokens, 32 heads      570 us on 32 SMs
+//     one sequence of 8 192 tokens, 32 heads      570 us on 32 SMs, 430 split over 96
 //     16 sequences of 4 096 tokens, 32 heads    1 200 us on all, 512 heads on 148 SMs
-// On the way, one sequence of 8 192 tokens: token by token 6 750 us; in chunks with one prep group 1 920; two groups, values and outputs
+// On the way, one sequence of 8 192 tokens, not split: token by token 6 750 us; in chunks with one prep group 1 920; two groups, values and outputs
 // through shared memory, instructions issued by a whole warp 810; the inverse on tensor cores, one scale per row 620; rows and outputs by
 // TMA 570.  16 sequences of 4 096: loops instead of straight code and outputs accumulated in tensor memory 1 330 -> 1 170 us.  Without gain:
 // sixteen main warps with a quarter of a row each, two accumulators for S k, loops rolled up to 38 KB (spills: 684 us), hints to
@@ -457,13 +457,14 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
     }
 }
 
-// The values of chunk c are there: rows behind the chunk's end cleared, and the sums for the bounds.
+// The values of chunk c are there: rows behind the chunk's end cleared (all of them: len = 0), and the sums for the bounds.
 __device__ __forceinline__ void ck_values(ChunkSmem& s, int c, int64_t len, int grp, int w, int lane, int& patience) {
     const int buf = c & 1, pt = 32 * w + lane;
     const int64_t left = len - int64_t(c) * CT;
     ck_wait(patience, &s.v_full[buf], uint32_t(c >> 1) & 1u);
     if (left < CT) {
         ck_clear(s.v, 2, int(left), pt, CK_PREP);
+        fence_async_smem();                                  // (the next copy of v goes to the same place)
         prep_bar(grp);
     }
     ck_vsum(s.v, s.vsum, w, lane);
@@ -471,7 +472,7 @@ __device__ __forceinline__ void ck_values(ChunkSmem& s, int c, int64_t len, int 
     if (pt == 0) mbar_arrive(&s.v_ready[buf]);
     __syncwarp();
 }
-__device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const CUtensorMap* rows, int hk, int hv, int64_t t0, int64_t len, int nchunk, uint32_t tm,
+__device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const CUtensorMap* rows, int hk, int hv, int64_t t0, int64_t len, int64_t vlen, int nchunk, uint32_t tm,
                                         int grp, int w, int lane, int& patience) {
     const uint32_t el = elect_one();
     const int pt = 32 * w + lane;
@@ -488,7 +489,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         if (w == 3)
             ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
         ck_wait(patience, &s.raw_full[grp], ph);
-        if (c != 1) ck_values(s, c == 0 ? 0 : c - 1, len, grp, w, lane, patience);     // of the chunk before: the other group has its hands full
+        if (c != 1) ck_values(s, c == 0 ? 0 : c - 1, vlen, grp, w, lane, patience);     // of the chunk before: the other group has its hands full
         if (n < CT) {
             ck_clear(s.raw, 4, n, pt, CK_PREP);
             prep_bar(grp);
@@ -552,7 +553,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         if (pt == 0) mbar_arrive(&s.ta_full[grp]);
         __syncwarp();
     }
-    if (nchunk > 1 && (nchunk & 1) == grp) ck_values(s, nchunk - 1, len, grp, w, lane, patience);
+    if (nchunk > 1 && (nchunk & 1) == grp) ck_values(s, nchunk - 1, vlen, grp, w, lane, patience);
     if (w == 0) umma_commit_if(el, &s.fin);
 }
 
@@ -576,15 +577,19 @@ __device__ __forceinline__ void ck_ready(uint64_t* bar, int lane) {
     __syncwarp();
 }
 // Chunk c's outputs are finished while S k of chunk c + 1 is under way, and leave for memory while T r of it is.
-__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, float* Sg, bool keep, uint32_t tm, int tid,
-                                        int& patience) {
+__device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int hv, int64_t t0, int nchunk, const float* Sin, bool unit, float* Sout, bool outputs,
+                                        uint32_t tm, int tid, int& patience) {
     const int lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), h = warp >> 2, v = 32 * (warp & 3) + lane;
     const uint32_t row = tm + (uint32_t(32 * (warp & 3)) << 16);
     float2 S[SP];                                            // S[v][2 SP h ..] times 2^e
-    float* Srow = Sg + v * KD + 2 * SP * h;
+    const int at = v * KD + 2 * SP * h;
 #pragma unroll
     for (int i = 0; i < SP / 2; ++i) {
-        const float4 x = keep ? *reinterpret_cast<const float4*>(Srow + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 x = Sin ? *reinterpret_cast<const float4*>(Sin + at + 4 * i) : make_float4(0.f, 0.f, 0.f, 0.f);
+        if (unit) {
+            const int d = v - 2 * SP * h - 4 * i;
+            x = make_float4(d == 0 ? 1.f : 0.f, d == 1 ? 1.f : 0.f, d == 2 ? 1.f : 0.f, d == 3 ? 1.f : 0.f);
+        }
         S[2 * i] = make_float2(x.x, x.y);
         S[2 * i + 1] = make_float2(x.z, x.w);
     }
@@ -679,7 +684,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         if (c == nchunk) {
             named_bar(1, CK_MAIN);
 #pragma unroll 1
-            for (int r = tid >> 4; r < plen; r += CK_MAIN / 16)
+            for (int r = tid >> 4; r < (outputs ? plen : 0); r += CK_MAIN / 16)
                 *reinterpret_cast<uint4*>(P.o + ((t0 + int64_t(c - 1) * CT + r) * P.HV + hv) * VD + 8 * (tid & 15)) =
                     *reinterpret_cast<const uint4*>(&s.o[r][8 * (tid & 15)]);
             break;
@@ -750,17 +755,19 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         }
         ck_ready(&s.u_ready, lane);
     }
+    if (!Sout) return;
     const float2 down = both(pow2f(-e));
 #pragma unroll
     for (int i = 0; i < SP / 2; ++i) {
         const float2 a = __fmul2_rn(S[2 * i], down), b = __fmul2_rn(S[2 * i + 1], down);
-        *reinterpret_cast<float4*>(Srow + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<float4*>(Sout + at + 4 * i) = make_float4(a.x, a.y, b.x, b.y);
     }
 }
 
 // The tensor-core instructions of the main chain, and the bulk stores of the outputs, by a warp of their own: whoever issues waits while
 // the tensor cores are busy.
-__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, const CUtensorMap* outs, int xv, int hv, int t0, int nchunk, uint32_t tm, int& patience) {
+__device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, const CUtensorMap* outs, int xv, int hv, int t0, int nchunk, bool outputs, uint32_t tm,
+                                         int& patience) {
     const uint32_t el = elect_one();
     if (el) ck_fetch_v(s, rows, xv, t0, &s.v_full[0]);
     __syncwarp();
@@ -799,7 +806,7 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
             tma_prefetch_2d(rows, xv, t0 + (c + 2) * CT);
             tma_prefetch_2d(rows, xv + 64, t0 + (c + 2) * CT);
         }
-        if (el && c > 0) tma_store_2d(outs, s.o, hv * VD, t0 + (c - 1) * CT);      // outputs of the chunk before, a full one
+        if (el && c > 0 && outputs) tma_store_2d(outs, s.o, hv * VD, t0 + (c - 1) * CT);      // outputs of the chunk before, a full one
         __syncwarp();
         ck_wait(patience, &s.u_ready, pc);
         tc_fence_after_sync();
@@ -868,6 +875,82 @@ __device__ __forceinline__ int ck_sequence(ChunkSmem& s, const RuleParams& P, in
     return s.seq;
 }
 
+// Where there are fewer heads than SMs, a long sequence is split into segments.  The rule is linear in the state, S -> S M + B over a
+// segment, and its M is the rule's own result from the unit matrix without values, its B that from zero:
+//     pass 1   segment 0 as it is; of every other but the last, M and B
+//     join     the state S_i that segment i starts from, S_{i+1} = S_i M_i + B_i
+//     pass 2   the segments 1 .. from their states
+// Every segment but the first and the last is run three times, but the chain is two segments long, with 30 us for two more launches and
+// 2.5 us a join.  One sequence, whole -> in segments:
+//     8 192 tokens  32 heads 570 -> 430 us (3 segments), 16 heads 249 (6), 8 heads 165 (10), 4 heads 138 (16; 8 segments 186)
+//     2 048 tokens  32 heads 158 -> 141 us,              16 heads 103,     8 heads 82,       4 heads 80
+struct Segments {
+    float* work;                                             // of this sequence and head
+    int64_t tokens;                                          // of a segment but the last: whole chunks
+    int count;
+    __device__ __forceinline__ float* start(int i) const { return work + int64_t(i - 1) * (VD * KD); }              // S_i; B_{i-1} until the join
+    __device__ __forceinline__ float* map(int segs, int i) const { return work + int64_t(segs - 1 + i - 1) * (VD * KD); }     // M_i
+};
+__device__ __forceinline__ Segments rule_segments(const RuleParams& P, int n, int hv, int64_t len) {
+    Segments g;
+    g.work = P.work + (int64_t(n) * P.HV + hv) * (2 * P.segs - 3) * (VD * KD);
+    const int64_t chunks = (len + CT - 1) / CT;
+    g.tokens = (chunks + P.segs - 1) / P.segs * CT;
+    g.count = int((len + g.tokens - 1) / g.tokens);
+    return g;
+}
+// Four rows of a head's states, through all its segments.  Half of the threads of a column take half of the sum, so that a thread can have
+// its part of M in flight at once: 64 KB of M from L2 and their latency is what a step takes.
+constexpr int JOIN_ROWS = 4;
+__global__ void __launch_bounds__(2 * KD) rule_join_kernel(RuleParams P) {
+    __shared__ alignas(16) float rows[JOIN_ROWS][KD], part[JOIN_ROWS][KD];
+    pdl_trigger();
+    pdl_wait();
+    constexpr int PARTS = VD / JOIN_ROWS, HALF = KD / 2;
+    const int prog = blockIdx.x / PARTS, n = prog / P.HV, hv = prog % P.HV, k = threadIdx.x & (KD - 1), h = threadIdx.x / KD;
+    int64_t t0, len;
+    rule_span(P, n, t0, len);
+    const int slot = P.idx[n];
+    if (len < P.shorter || slot <= 0 || slot >= P.NS || !first_of_slot(P.idx, n, slot, k & 31)) return;
+    const Segments g = rule_segments(P, n, hv, len);
+    const int at = (blockIdx.x % PARTS) * JOIN_ROWS * KD + k;
+    if (g.count > 2 && h == 0) {
+#pragma unroll
+        for (int r = 0; r < JOIN_ROWS; ++r) rows[r][k] = g.start(1)[at + r * KD];
+    }
+#pragma unroll 1
+    for (int i = 1; i <= g.count - 2; ++i) {
+        const float* m = g.map(P.segs, i) + h * HALF * KD + k;
+        float* next = g.start(i + 1) + at;
+        float x[HALF], acc[JOIN_ROWS];
+#pragma unroll
+        for (int j = 0; j < HALF; ++j) x[j] = m[j * KD];
+#pragma unroll
+        for (int r = 0; r < JOIN_ROWS; ++r) acc[r] = h ? 0.f : next[r * KD];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < HALF; j += 4)
+#pragma unroll
+            for (int r = 0; r < JOIN_ROWS; ++r) {
+                const float4 s = *reinterpret_cast<const float4*>(&rows[r][h * HALF + j]);
+                acc[r] = fmaf(s.w, x[j + 3], fmaf(s.z, x[j + 2], fmaf(s.y, x[j + 1], fmaf(s.x, x[j], acc[r]))));
+            }
+        if (h) {
+#pragma unroll
+            for (int r = 0; r < JOIN_ROWS; ++r) part[r][k] = acc[r];
+        }
+        __syncthreads();
+        if (!h) {
+#pragma unroll
+            for (int r = 0; r < JOIN_ROWS; ++r) {
+                acc[r] += part[r][k];
+                rows[r][k] = acc[r];
+                next[r * KD] = acc[r];
+            }
+        }
+    }
+}
+
 __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P, const __grid_constant__ CUtensorMap rows,
                                                                    const __grid_constant__ CUtensorMap outs) {
     extern __shared__ __align__(128) unsigned char rule_smem[];
@@ -897,16 +980,54 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     pdl_wait();
-    const int n = ck_sequence(s, P, int(blockIdx.x) / P.HV, tid), hv = blockIdx.x % P.HV, hk = hv / (P.HV / P.H);
-    if (n < 0) return;
+    int n, hv, role = 0;
+    if (P.segs == 0) {
+        n = ck_sequence(s, P, int(blockIdx.x) / P.HV, tid);
+        hv = int(blockIdx.x) % P.HV;
+        if (n < 0) return;
+    } else {
+        const int roles = P.pass == 1 ? 2 * P.segs - 3 : P.segs - 1, prog = int(blockIdx.x) / roles;
+        role = int(blockIdx.x) % roles;
+        n = prog / P.HV;
+        hv = prog % P.HV;
+    }
+    const int hk = hv / (P.HV / P.H);
     int64_t t0, len;
     rule_span(P, n, t0, len);
+    if (P.segs && len < P.shorter) return;
     const int slot = P.idx[n];
     if (slot <= 0 || slot >= P.NS || !first_of_slot(P.idx, n, slot, lane)) {       // padding: zeros, and no state
+        if (P.pass == 2 || role > 0) return;
 #pragma unroll 1
         for (int64_t i = tid; i < len * (VD / 8); i += CK_THREADS)
             *reinterpret_cast<uint4*>(P.o + ((t0 + i / (VD / 8)) * P.HV + hv) * VD + 8 * (i % (VD / 8))) = make_uint4(0u, 0u, 0u, 0u);
         return;
+    }
+    // what it starts from and where it leaves the state
+    float* const state = P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD;
+    const float* from = !P.has_initial || P.has_initial[n] ? state : nullptr;
+    float* to = state;
+    bool unit = false, outputs = true;
+    if (P.segs) {
+        const Segments g = rule_segments(P, n, hv, len);
+        int seg = 0;
+        if (P.pass == 1) {
+            if (role > 0) {
+                seg = (role + 1) / 2;
+                if (seg > g.count - 2) return;
+                unit = !(role & 1);
+                outputs = false;
+                from = nullptr;
+                to = unit ? g.map(P.segs, seg) : g.start(seg + 1);
+            } else if (g.count > 1) to = g.start(1);
+        } else {
+            seg = role + 1;
+            if (seg >= g.count) return;
+            from = g.start(seg);
+            if (seg < g.count - 1) to = nullptr;
+        }
+        t0 += seg * g.tokens;
+        len = len - seg * g.tokens < g.tokens ? len - seg * g.tokens : g.tokens;
     }
 #pragma unroll 1
     for (int i = tid; i < 4 * 8192 / 16; i += CK_THREADS) reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);   // the upper right
@@ -923,14 +1044,13 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
     const int uw = __shfl_sync(0xffffffffu, warp, 0);        // the warp's number, known to be the same in all lanes
     int patience = WAIT_LIMIT;
     if (uw == CK_THREADS / 32 - 1) {
-        ck_issue(s, &rows, &outs, 2 * P.H * KD + hv * VD, hv, int(t0), nchunk, tm, patience);
+        ck_issue(s, &rows, &outs, 2 * P.H * KD + hv * VD, hv, int(t0), nchunk, outputs, tm, patience);
     } else if (uw >= CK_MAIN / 32) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(CK_PREP_REGS));
-        ck_prep(s, P, &rows, hk, hv, t0, len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane, patience);
+        ck_prep(s, P, &rows, hk, hv, t0, len, unit ? 0 : len, nchunk, tm, (uw - CK_MAIN / 32) >> 2, uw & 3, lane, patience);
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(CK_MAIN_REGS));
-        ck_main(s, P, hv, t0, nchunk, P.ssm + int64_t(slot) * P.SS + int64_t(hv) * VD * KD, !P.has_initial || P.has_initial[n], tm, tid,
-                patience);
+        ck_main(s, P, hv, t0, nchunk, from, unit, to, outputs, tm, tid, patience);
     }
     ck_wait(patience, &s.fin, 0);                            // no tensor-core instruction is left
     if (patience == 0) s.dead = 1;
@@ -993,10 +1113,28 @@ static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     if (rc) return rc;
     // no more than T / P.shorter sequences can be that long
     const int64_t most = P.T / P.shorter < P.N ? P.T / P.shorter : P.N;
-    const cudaError_t e = launch_dependent(rule_chunk_kernel, unsigned(most) * unsigned(P.HV), CK_THREADS, smem, st, P, rows, outs);
+    const unsigned heads = unsigned(P.segs ? P.N : most) * unsigned(P.HV);
+    RuleParams Q = P;
+    Q.pass = 1;
+    cudaError_t e = launch_dependent(rule_chunk_kernel, heads * unsigned(P.segs ? 2 * P.segs - 3 : 1), CK_THREADS, smem, st, Q, rows, outs);
+    if (e == cudaSuccess && P.segs) {
+        e = launch_dependent(rule_join_kernel, heads * (VD / JOIN_ROWS), 2 * KD, 0, st, Q);
+        Q.pass = 2;
+        if (e == cudaSuccess) e = launch_dependent(rule_chunk_kernel, heads * unsigned(P.segs - 1), CK_THREADS, smem, st, Q, rows, outs);
+    }
     if (e != cudaSuccess) { set_last_cuda_error(e); return LQ_ERR_LAUNCH; }
     return finish_launch();
 }
+// Segments that sequences are split into, 0 if that would not be faster: both passes have to fit the SMs at once, and a sequence of mean
+// length has to save more by its shorter chain (4.4 us a chunk) than the launches and the joins cost.  (At the least 16 chunks in four segments
+// of four.)
+static int rule_segs(int64_t N, int64_t HV, int64_t T) {
+    const int64_t chunks = T / N / CT, fit = (device_sm_count() / (N * HV) + 3) / 2;
+    int64_t segs = fit < 16 ? fit : 16;
+    if (segs > chunks / 4) segs = chunks / 4;
+    return segs >= 3 && chunks * (segs - 2) >= 8 * segs ? int(segs) : 0;
+}
+static int64_t rule_work(int64_t N, int64_t HV, int segs) { return segs ? N * HV * (2 * segs - 3) * VD * KD * 4 : 0; }
 
 static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                               const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
@@ -1006,6 +1144,9 @@ static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, i
     P.b = (const uint16_t*)b; P.a_stride = a_stride; P.b_stride = b_stride; P.A_log = A_log; P.dt_bias = dt_bias; P.cu = cu;
     P.idx = idx; P.has_initial = has_initial; P.o = (uint16_t*)o; P.NS = d->NS; P.H = d->H; P.HV = d->HV; P.N = N; P.T = T;
     P.shorter = T + 1;
+    P.work = nullptr;
+    P.segs = 0;
+    P.pass = 1;
     P.scale = scale > 0.f ? scale : 1.0f / sqrtf(float(KD));
     return P;
 }
@@ -1015,12 +1156,13 @@ static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, i
 extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                               const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
                               const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale,
-                              void* stream) {
+                              void* work, int64_t work_bytes, void* stream) {
     using namespace lq;
     if (!d) return LQ_ERR_NULL;
     RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
                                      T, scale);
     if (N > 0 && T > 0 && !cu) return LQ_ERR_NULL;
+    if (misaligned16({work})) return LQ_ERR_ALIGN;
     const int rc = rule_check(d, P);
     if (rc || N == 0 || T == 0) return rc;
     // The lengths are on the device: a batch gets both kernels, and each of its sequences is run by one of them.
@@ -1033,7 +1175,17 @@ extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, i
         const int rc2 = launch_recurrent(P, st);
         if (rc2) return rc2;
     }
+    const int segs = rule_segs(N, d->HV, T);
+    if (work && segs && work_bytes >= rule_work(N, d->HV, segs)) {
+        P.work = static_cast<float*>(work);
+        P.segs = segs;
+    }
     return launch_chunk(P, st);
+}
+
+extern "C" int64_t lq_prefill_work_bytes(int32_t N, int32_t HV, int64_t T) {
+    using namespace lq;
+    return N < 1 || HV < 1 || T < 1 ? 0 : rule_work(N, HV, rule_segs(N, HV, T));
 }
 
 extern "C" int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,

@@ -26,6 +26,8 @@ struct RuleParams {
     int64_t T;
     float scale;
     int64_t shorter;                  // rule_recurrent_kernel takes the sequences with fewer tokens, rule_chunk_kernel the others
+    float* work;                      // matrices of the segments, where sequences are split
+    int32_t segs, pass;               // segments a sequence is split into (0: not), and which of the two passes over them this is
 };
 
 // log(1 + e^x) to fp32 precision for every x: 1 + e^x alone would cut e^x off at 2^-24, and a layer that starts with steps of a

@@ -205,7 +205,7 @@ class LeapQuantState:
 
         mixed bf16 [T, 2HK + HV*V], a, b bf16 [T, HV] (row strides free); sequence n owns the rows cu_seqlens[n] .. cu_seqlens[n + 1] - 1
         and slot idx[n]; has_initial bool [N] or None: False starts it from a zero state; out bf16 [T, HV, V] written in place.
-        Gated DeltaNet only.  No host synchronisation, no allocation when the dtypes match."""
+        Gated DeltaNet only.  No host synchronisation; scratch from torch's allocator where long sequences of few heads are split."""
         self._need_gdn("prefill")
         self.kprefill(ssm, mixed, a, b, A_log if A_log.dtype == torch.float32 else self._p32(A_log),
                       dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), cu_seqlens.to(torch.int32), idx.to(torch.int32),

@@ -177,6 +177,84 @@ def test_prefill_batches_of_short_and_long_sequences(lens):
     clean()
 
 
+def work_bytes(n, HV, T):
+    from leapquant_b200 import _lib
+    return _lib.lib().lq_prefill_work_bytes(n, HV, T)
+
+
+def test_only_few_long_sequences_are_split():
+    """Scratch is asked for where both passes fit 148 SMs and the chain is long enough; at least the states and maps of three segments."""
+    assert work_bytes(1, 32, 8192) == 32 * 3 * 65536 and work_bytes(1, 8, 8192) == 8 * 17 * 65536
+    for n, HV, T in ((1, 32, 512), (1, 64, 8192), (64, 32, 65536), (2, 32, 16384), (1, 1, 640), (0, 32, 8192), (1, 0, 8192), (1, 32, 0), (1 << 30, 1 << 30, 1 << 40)):
+        assert work_bytes(n, HV, T) == 0, (n, HV, T)
+
+
+@gpu
+@pytest.mark.parametrize("H,HV,lens,slots", [(1, 2, [1300], [1]), (2, 4, [2500], [2]), (1, 1, [4096], [1]), (1, 2, [1281], [1]), (2, 2, [3600, 900, 12], [3, 1, 2]),
+                                             (1, 2, [1400, 1400, 1500], [2, 0, 2]), (1, 1, [5, 0, 6000, 65], [1, 2, 3, 4]), (4, 32, [3000], [1])],
+                         ids=lambda x: "-".join(map(str, x)) if isinstance(x, list) else None)
+def test_prefill_split_over_segments(H, HV, lens, slots):
+    """Few long sequences, which are run as segments and joined: odd lengths, short and empty ones beside them, padding, a repeated slot."""
+    n = len(lens)
+    assert work_bytes(n, HV, sum(lens) + 3) > 0
+    for fresh in (None, [i % 2 == 0 for i in range(n)]):
+        S, S64, o, o64, size = run_rule(H, HV, lens, slots, max(slots) + 2, seed=sum(lens) + HV, fresh=fresh)
+        check_rule(S, S64, o, o64, size, max(lens))
+        assert bool((o[sum(lens):] == 7.0).all())
+        assert torch.equal(S[0].double(), S64[0])
+    clean()
+
+
+@gpu
+@pytest.mark.parametrize("change", ["same_keys", "no_decay", "large_values", "small_values", "uneven_keys"])
+def test_prefill_split_unusual_values(change):
+    S, S64, o, o64, size = run_rule(2, 4, [1500], [1], 3, seed=6, change=globals()[change])
+    check_rule(S, S64, o, o64, size, 1500, change)
+    clean()
+
+
+@gpu
+def test_prefill_split_without_scratch_on_streams_and_in_graphs():
+    """The same call twice, on a side stream, and captured and replayed beside another one: the same bits.  Without scratch the C entry
+    runs a head on one SM: the same to fp32 roundings."""
+    from leapquant_b200 import _lib
+    from leapquant_b200.kernels import make_gdn_prefill
+    H, HV, T = 2, 4, 1700
+    ssm, mixed, a, b, A_log, dt_bias = rule_inputs(H, HV, T, 3, 21)
+    f = make_gdn_prefill(3, HV, H, K, V, ssm.stride(0))
+    cu, idx = offsets([T]).cuda(), torch.tensor([2], dtype=torch.int32, device="cuda")
+    runs = []
+    for how in ("plain", "again", "stream", "graph"):
+        S, o = ssm.clone(), torch.zeros(T, HV, V, dtype=torch.bfloat16, device="cuda")
+        call = lambda: f(S, mixed, a, b, A_log, dt_bias, cu, idx, None, o)
+        torch.cuda.synchronize()
+        if how == "stream":
+            with torch.cuda.stream(torch.cuda.Stream()):
+                call()
+        elif how == "graph":
+            g, S2, o2 = torch.cuda.CUDAGraph(), ssm.clone(), torch.zeros_like(o)
+            with torch.cuda.graph(g):
+                call()
+                f(S2, mixed, a, b, A_log, dt_bias, cu, idx, None, o2)
+            for s in (S, S2):
+                s.copy_(ssm)
+            g.replay()
+            torch.cuda.synchronize()
+            runs.append((S2, o2))
+        else:
+            call()
+        torch.cuda.synchronize()
+        runs.append((S, o))
+    for S, o in runs[1:]:
+        assert torch.equal(S, runs[0][0]) and torch.equal(o, runs[0][1])
+    S, o = ssm.clone(), torch.zeros(T, HV, V, dtype=torch.bfloat16, device="cuda")
+    _lib.launch(_lib.lib().lq_gdn_prefill, "lq_gdn_prefill", S, _lib.dims(3, HV, H, K, V, 0, 0, S.stride(0)), S.data_ptr(), mixed.data_ptr(), mixed.stride(0),
+                a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(0), A_log.data_ptr(), dt_bias.data_ptr(), cu.data_ptr(), idx.data_ptr(), None, o.data_ptr(),
+                1, T, K ** -0.5, None, 0)
+    assert float((S - runs[0][0]).norm() / S.norm()) <= 2 * 2.0 ** -20 * math.sqrt(T)     # both within the bound of the 64-bit result
+    clean()
+
+
 def same_keys(mixed, a, b, A_log, dt_bias):
     mixed[:, 256:512] = mixed[0, 256:512]                    # H = 2: every key the same, every step written in full
     b.fill_(8.0)
@@ -520,7 +598,7 @@ def test_argument_errors_are_codes():
     C = 2 * 2 * 128 + 4 * 128
 
     def prefill(d=None, ssm=one, mixed=one, ms=C, a=one, as_=4, b=one, bs=4, A=one, dt=one, cu=one, idx=one, o=one, N=1, T=1):
-        return L.lq_gdn_prefill(d or D(), ssm, mixed, ms, a, as_, b, bs, A, dt, cu, idx, None, o, N, T, 0.0, None)
+        return L.lq_gdn_prefill(d or D(), ssm, mixed, ms, a, as_, b, bs, A, dt, cu, idx, None, o, N, T, 0.0, None, 0, None)
 
     assert prefill(N=0) == 0 and prefill(T=0) == 0 and prefill(N=0, ssm=None) == 0
     assert prefill(N=-1) == -4 and prefill(T=-1) == -4 and prefill(N=1 << 30) == -4
@@ -560,10 +638,10 @@ def test_overlapping_operands_are_refused():
     d = _lib.dims(8, 4, 2, 128, 128, 0, 0, 4 * 128 * 128)
     C, W, T = 1024, 512, 100
     for k in (0, 512, C - 8, C * (T - 1)):                   # outputs within the rows, in the last row
-        assert L.lq_gdn_prefill(d, far, at(0), C, far, 4, far, 4, far, far, far, far, None, at(k), 1, T, 0.0, None) == -4, k
+        assert L.lq_gdn_prefill(d, far, at(0), C, far, 4, far, 4, far, far, far, far, None, at(k), 1, T, 0.0, None, 0, None) == -4, k
         assert L.lq_gdn_recurrent(d, far, at(0), C, far, 4, far, 4, far, far, far, at(k), T, 0.0, None) == -4, k
-    assert L.lq_gdn_prefill(d, far, far, C, at(8), 4, far, 4, far, far, far, far, None, at(0), 1, T, 0.0, None) == -4
-    assert L.lq_gdn_prefill(d, far, far, C, far, 4, at(W * T - 8), 4, far, far, far, far, None, at(0), 1, T, 0.0, None) == -4
+    assert L.lq_gdn_prefill(d, far, far, C, at(8), 4, far, 4, far, far, far, far, None, at(0), 1, T, 0.0, None, 0, None) == -4
+    assert L.lq_gdn_prefill(d, far, far, C, far, 4, at(W * T - 8), 4, far, far, far, far, None, at(0), 1, T, 0.0, None, 0, None) == -4
     for xs, os_, k in ((64, 64, 0), (64, 64, 8), (64, 64, -64), (64, 128, 64 * (T - 1)), (256, 256, 56), (256, 256, 200), (256, 256, -256 - 56)):
         cv = _lib.LqConv1d(at(0), xs, far, 192, 1, 64, far, None, 4)
         assert L.lq_causal_conv1d_prompt(cv, far, far, None, 1, T, 64, 4, at(k), os_, None) == -4, (xs, os_, k)
