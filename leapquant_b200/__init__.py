@@ -3,7 +3,8 @@ NVIDIA B200 (sm_100a) as hand-written CUDA kernels behind a C ABI, with the refe
 
     leapquant_b200.state     LeapQuantState, state_views, get_state, WINDOW, RANK   (reference leapquant/state.py)
     leapquant_b200.kernels   make_gdn_step / make_kda_step / make_flush / make_dequant / make_quantize / make_lowrank
-                             (reference leapquant/kernels.py)
+                             (reference leapquant/kernels.py), and the operators around them: make_gdn_prefill,
+                             make_gdn_recurrent, make_conv1d_prompt, make_gated_norm, make_add_norm
     leapquant_b200.vllm      register(), gdn.install(), glm.install()               (reference leapquant/vllm/)
 
 `install_alias()` publishes the package under the name `leapquant`, so code written against the reference

@@ -165,8 +165,9 @@ def test_prefill_strides(kw, impl):
 
 @gpu
 @pytest.mark.parametrize("lens", [[18], [20], [1, 30, 5, 64, 19, 20, 21, 0, 100, 1], [(7 * i) % 45 for i in range(150)], [3] * 140 + [70],
-                                  [27], [28], [64, 27, 28, 29, 0, 130], [2] * 300 + [28] + [1] * 500 + [65, 3, 30]],
-                         ids=["18", "20", "mixed", "150", "141", "27", "28", "around28", "804"])
+                                  [27], [28], [64, 27, 28, 29, 0, 130], [2] * 300 + [28] + [1] * 500 + [65, 3, 30],
+                                  [900, 7, 8, 9, 1, 20, 1100]],
+                         ids=["18", "20", "mixed", "150", "141", "27", "28", "around28", "804", "among_long"])
 def test_prefill_batches_of_short_and_long_sequences(lens):
     """What a caller gets by default: each sequence in the form that suits its length, in batches that are ranked by it and larger ones."""
     n = len(lens)
