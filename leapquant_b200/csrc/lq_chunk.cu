@@ -16,9 +16,9 @@
 //
 // What bounds it.  One sequence is a chain of chunks, and a chunk of one head is what one SM does at a time: 4.4 us (8 000 cycles), of
 // which the main chain, six hand-overs between registers, tensor memory and tensor cores, takes 6 900 by itself.  The two prep groups
-// need 16 000 for their two chunks, side by side with it.  Both are made of the same issue slots: 18 400 warp instructions a chunk, 0.5 an
-// SM quarter's cycle, in loops of 46 KB where the instruction cache holds 32 -- beyond it an instruction costs 2.7 cycles instead of
-// 1.7.  ALU 33 %, FMA 26 %, tensor pipe 25 % busy.
+// need 16 000 for their two chunks, side by side with it.  Both are made of the same issue slots: 19 600 warp instructions a chunk, 0.5 an
+// SM quarter's cycle.  FMA pipe 30 %, ALU 24 %, tensor pipe 24 % busy: a warp waits for tensor memory, barriers and its own results.  The
+// loops are kept small, since an SM's instruction cache holds 32 KB (they have 46; when they were twice as long, fetching was the first stall).
 //     one sequence of 8 192 tokens, 32 heads      570 us on 32 SMs, 430 split over 96
 //     16 sequences of 4 096 tokens, 32 heads    1 200 us on all, 512 heads on 148 SMs
 // On the way, one sequence of 8 192 tokens, not split: token by token 6 750 us; in chunks with one prep group 1 920; two groups, values and outputs

@@ -49,7 +49,7 @@ __device__ __forceinline__ void rule_span(const RuleParams& P, int n, int64_t& t
 // no warp waits for another.  Both products take the state before the update, S q = e^g (S_old q) + u (k^ . q^).  The gates of 32 tokens
 // are computed at once, one token a lane.
 // One token per sequence is a copy of the states: 256 rows of 32 heads 163 us, the measured copy rate.  From four tokens on the FMA pipe
-// (224 instructions a token of 354) and the latency of a token share the time; four warps a scheduler at 128 registers: 4 tokens of 128
+// (60 % busy, 59 % of the cycles issue) and the latency of a token share the time; four warps a scheduler at 128 registers: 4 tokens of 128
 // sequences of 32 heads 124 us, with three 137, with plain multiply-adds, a sum per row and three 158.  Carrying the decays in a scalar beside
 // the state, which saves a fifth of the FMA instructions, was no faster.
 constexpr int RW_ROWS = 16, RW_WARPS = 4, RW_CTAS = 4;
