@@ -256,6 +256,41 @@ def test_prefill_split_without_scratch_on_streams_and_in_graphs():
     clean()
 
 
+@gpu
+def test_prefills_side_by_side():
+    """Calls on two streams at once, one that is split into segments and one that is not, on different slots of one state tensor, leave what
+    they leave one after the other; and their other operators run between them."""
+    from leapquant_b200.kernels import make_conv1d_prompt, make_gated_norm, make_gdn_prefill
+    H, HV, lens = 2, 4, ([1500], [40, 7, 200, 3, 90])
+    slots = ([6], [1, 2, 3, 4, 5])
+    ssm, mixed, a, b, A_log, dt_bias = rule_inputs(H, HV, 1500, 7, 31)
+    f, norm, conv = make_gdn_prefill(7, HV, H, K, V, ssm.stride(0)), make_gated_norm(V), make_conv1d_prompt(7, mixed.shape[1])
+    cu, idx = [offsets(x).cuda() for x in lens], [torch.tensor(x, dtype=torch.int32, device="cuda") for x in slots]
+    w = torch.randn(mixed.shape[1], 4, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    gw = torch.ones(V, dtype=torch.bfloat16, device="cuda")
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for together in (False, True, True, True):
+        S, taps = ssm.clone(), torch.zeros(7, 3, mixed.shape[1], dtype=torch.bfloat16, device="cuda")
+        outs = []
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            n = sum(lens[i])
+            with torch.cuda.stream(streams[i]):
+                x, o, y = torch.empty(n, mixed.shape[1], dtype=torch.bfloat16, device="cuda"), *(torch.empty(n, HV, V, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+                conv(mixed[:n], taps.transpose(1, 2), w, None, cu[i], idx[i], None, x)
+                f(S, x, a[:n], b[:n], A_log, dt_bias, cu[i], idx[i], None, o)
+                norm(o, mixed[:n, : HV * V], gw, y)
+                outs += [o, y]
+            if not together:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        got.append([S, taps] + outs)
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(other, got[0]))
+    clean()
+
+
 def same_keys(mixed, a, b, A_log, dt_bias):
     mixed[:, 256:512] = mixed[0, 256:512]                    # H = 2: every key the same, every step written in full
     b.fill_(8.0)
