@@ -30,8 +30,9 @@
 // Precision.  k and q are bf16 and become f16 without loss once a row is scaled by a power of two (what is lost lies 2^-25 below the
 // row's norm); an fp32 operand is the sum of two f16 pieces, 22 bits.  f16 has few exponents, so every row of S, r and u carries
 // a power of two of its own, from bounds that hold whatever the inputs: |k^| <= 1, 0 <= beta <= 1 and decays <= 1 make the rule a
-// contraction, |r_t|, |u_t| / 2, |S| <= |S_0| + sum |v_t| =: B per row.  T is bounded by 1 for the same reason.  The products that
-// only reach the bf16 outputs (S q, A u) take one piece, 2^-12.
+// contraction, |r_t|, |u_t| / 2, |S| <= |S_0| + sum |v_t| =: B per row.  T is bounded by 1 for the same reason.  The outputs get the
+// same pieces as the state: with one piece each in S q and A u (11 bits) they lay 1.0e-3 of their norm from those of the plain form in 32
+// bits, with two 5e-5, as those of the token-by-token form do.
 #include <cuda.h>
 #include <stddef.h>
 
@@ -62,10 +63,10 @@ constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_P
 constexpr int CK_REGS = 96, CK_MAIN_REGS = 128, CK_PREP_REGS = 64;
 static_assert(CK_MAIN * CK_MAIN_REGS + 2 * CK_PREP * CK_PREP_REGS + 32 * CK_REGS <= CK_THREADS * CK_REGS, "register split");
 
-// Tensor memory, 512 columns.  D takes the place of X | XQ once both have been read.  The operand of A u takes that of S's heads once S q
-// is through.  Two regions of 64 change roles with every chunk: one has S's remainders and, after S k, the outputs (e^G S q^ put there,
+// Tensor memory, 512 columns.  D takes the place of X | XQ once both have been read.  The pieces of u for A u take that of S's heads once
+// S q is through.  Two regions of 64 change roles with every chunk: one has S's remainders and, after S k, the outputs (e^G S q^ put there,
 // A u added by the tensor cores), the other has u = T r -- and under the next chunk, whose remainders go there, the outputs stay.
-constexpr uint32_t TM_SHI = 0, TM_UOP = 0, TM_X = 128, TM_XQ = 192, TM_D = 128, TM_PHI = 256, TM_PLO = 288;
+constexpr uint32_t TM_SHI = 0, TM_UHI = 0, TM_ULO = 32, TM_X = 128, TM_XQ = 192, TM_D = 128, TM_PHI = 256, TM_PLO = 288;
 __device__ __forceinline__ uint32_t tm_slo(int buf) { return buf ? 320u : 64u; }                    // and the outputs of the chunk
 __device__ __forceinline__ uint32_t tm_gram(int buf) { return buf ? 384u : 448u; }                  // of the even and of the odd chunks
 
@@ -77,7 +78,15 @@ constexpr uint32_t CK_IDESC_BF16 = (1u << 7) | (1u << 10);    // both operands b
 __device__ __forceinline__ uint64_t ck_desc(uint32_t addr, uint32_t lbo) {
     return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t((lbo >> 4) & 0x3FFFu) << 16) | (uint64_t(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
-// byte offset of 16-byte chunk c (of 8) of a row in such a tile
+// Descriptor of an operand without swizzle, cores of eight rows by 16 bytes: the next eight rows follow, the next 16 bytes of a row are
+// `kstep` bytes away.
+__device__ __forceinline__ uint64_t ck_desc_cores(uint32_t addr, uint32_t kstep) {
+    return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(kstep >> 4) << 16) | (uint64_t(128 >> 4) << 32) | (1ull << 46);
+}
+// A [t][s] is kept in such cores, without the block of t < 32 <= s, which is zero: 16-byte chunk c (of 8) of row t
+constexpr uint32_t AMAT_BYTES = 4096 + 2048;
+__device__ __forceinline__ uint32_t ck_aoff(int t, int c) { return c < 4 ? c * 1024 + t * 16 : 4096 + (c - 4) * 512 + (t - 32) * 16; }
+// byte offset of 16-byte chunk c (of 8) of a row in a swizzled tile
 __device__ __forceinline__ uint32_t ck_off(int row, int c) { return uint32_t(row) * 128u + (uint32_t(c ^ (row & 7)) << 4); }
 
 struct alignas(16) ChunkScalars {                                        // of one chunk, by token
@@ -89,7 +98,7 @@ struct alignas(16) ChunkScalars {                                        // of o
     int len;                                                 // tokens of the chunk, 1 .. 64
 };
 struct alignas(16) PrepSmem {                                // of one prep group
-    float L[CT][CT + 4];                                     // times 2^13, like all that becomes f16 on the way to T
+    float L[3][32][36];                                      // blocks (0, 0), (1, 0), (1, 1); times 2^13, like all that becomes f16 on the way to T
     float tt[2][32][36];                                     // T^T of the two diagonal blocks of 32, times 2^13
     float2 G[CT];                                            // log2 of the decay from the chunk's start, head and remainder
     float gh[CT], gl[CT];                                    // the two apart and negated
@@ -100,7 +109,8 @@ struct alignas(16) ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
     unsigned char raw[32768];                                // the same as it comes, bf16
-    unsigned char thi[8192], tlo[8192], amat[2][8192], v[16384];                   // v: bf16, two blocks of 64 values by 64 rows
+    unsigned char thi[8192], tlo[8192], v[16384];            // v: bf16, two blocks of 64 values by 64 rows
+    unsigned char ahi[2][AMAT_BYTES], alo[2][AMAT_BYTES];
     uint16_t o[CT][VD];                                      // outputs on their way out
     PrepSmem prep[2];
     ChunkScalars sc[2];
@@ -114,7 +124,7 @@ struct alignas(16) ChunkSmem {
 };
 
 static_assert(sizeof(ChunkScalars) % 16 == 0 && sizeof(PrepSmem) % 16 == 0 && offsetof(ChunkSmem, raw) % 1024 == 0 && offsetof(ChunkSmem, thi) % 1024 == 0 && offsetof(ChunkSmem, tlo) % 1024 == 0 &&
-                  offsetof(ChunkSmem, amat) % 1024 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
+                  offsetof(ChunkSmem, ahi) % 16 == 0 && offsetof(ChunkSmem, alo) % 16 == 0 && offsetof(ChunkSmem, v) % 1024 == 0 && offsetof(ChunkSmem, o) % 128 == 0 &&
                   offsetof(ChunkSmem, prep) % 16 == 0 && offsetof(ChunkSmem, sc) % 16 == 0 && offsetof(ChunkSmem, vsum) % 16 == 0 &&
                   offsetof(PrepSmem, gh) % 16 == 0 && offsetof(PrepSmem, gl) % 16 == 0 && offsetof(PrepSmem, ws) % 16 == 0 && offsetof(ChunkSmem, raw_full) % 8 == 0,
               "vector accesses and swizzled tiles");
@@ -301,20 +311,22 @@ __device__ __forceinline__ void ck_gates(PrepSmem& s, const uint16_t* a, int64_t
 }
 
 // eight columns of a row of A or L to their places
-__device__ __forceinline__ void ck_put8(PrepSmem& s, unsigned char* amat, bool isq, int t, int c8, const float2 (&y)[4]) {
+__device__ __forceinline__ void ck_put8(PrepSmem& s, unsigned char* ahi, unsigned char* alo, bool isq, int t, int c8, const float2 (&y)[4]) {
     if (isq) {
-        uint32_t h[4];
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = h2_bits(__floats2half2_rn(y[j].x, y[j].y));
-        *reinterpret_cast<uint4*>(amat + ck_off(t, c8)) = make_uint4(h[0], h[1], h[2], h[3]);
+        for (int j = 0; j < 4; ++j) split_h2(y[j], h[j], l[j]);
+        *reinterpret_cast<uint4*>(ahi + ck_aoff(t, c8)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(alo + ck_aoff(t, c8)) = make_uint4(l[0], l[1], l[2], l[3]);
     } else {
-        *reinterpret_cast<float4*>(&s.L[t][8 * c8]) = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
-        *reinterpret_cast<float4*>(&s.L[t][8 * c8 + 4]) = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
+        float* to = &s.L[(t >> 5) + (c8 >> 2)][t & 31][8 * (c8 & 3)];
+        *reinterpret_cast<float4*>(to) = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+        *reinterpret_cast<float4*>(to + 4) = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
     }
 }
-// Gram rows -> L (fp32, k rows) and A (f16 operand, q rows); a thread has a row.  Inside a diagonal block of 32 tokens the decay is
+// Gram rows -> L (fp32, k rows) and A (two f16 pieces, q rows); a thread has a row.  Inside a diagonal block of 32 tokens the decay is
 // taken pair by pair; from the first block to the second in two steps over token 31, neither of which exceeds 1.
-__device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32_t gram, int w, int lane) {
+__device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* ahi, unsigned char* alo, uint32_t gram, int w, int lane) {
     const bool isq = w >= 2;
     const int blk = w & 1, t = 32 * blk + lane;
     const float2 Gt = s.G[t];
@@ -329,7 +341,7 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
             tmem_ld_8(gram + 8 * c8, g);
 #pragma unroll
             for (int j = 0; j < 4; ++j) y[j] = __fmul2_rn(__fmul2_rn(f2_of(g[2 * j], g[2 * j + 1]), both(f)), *reinterpret_cast<const float2*>(&s.ws[8 * c8 + 2 * j]));
-            ck_put8(s, amat, isq, t, c8, y);
+            ck_put8(s, ahi, alo, isq, t, c8, y);
         }
     }
     const int last = isq ? lane : lane - 1;                  // last column of the diagonal block that counts
@@ -350,7 +362,7 @@ __device__ __forceinline__ void ck_gram(PrepSmem& s, unsigned char* amat, uint32
             y[j] = make_float2(c <= last ? z0.x : 0.f, c < last ? z0.y : 0.f);
             y[j + 1] = make_float2(c + 2 <= last ? z1.x : 0.f, c + 2 < last ? z1.y : 0.f);
         }
-        ck_put8(s, amat, isq, t, 4 * blk + c8, y);
+        ck_put8(s, ahi, alo, isq, t, 4 * blk + c8, y);
     }
 }
 struct Pieces { uint32_t hi, lo; };
@@ -382,20 +394,20 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
         float* tt = &s.tt[w >> 1][(o & 16) + c][o & 16];     // this column of T
 #pragma unroll
         for (int b = 0; b < 16; b += 4) {
-            const float* l = &s.L[o + b][o];
+            const float* l = &s.L[w & 2][(o & 16) + b][o & 16];
             float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int m = 0; m < b; m += 4) {
                 const float4 x = *reinterpret_cast<const float4*>(tt + m);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float4 y = *reinterpret_cast<const float4*>(l + r * (CT + 4) + m);
+                    const float4 y = *reinterpret_cast<const float4*>(l + r * 36 + m);
                     a[r] = fmaf(y.x, x.x, fmaf(y.y, x.y, fmaf(y.z, x.z, fmaf(y.w, x.w, a[r]))));
                 }
             }
-            const float l10 = l[CT + 4 + b];
-            const float2 l2 = *reinterpret_cast<const float2*>(l + 2 * (CT + 4) + b);
-            const float4 l3 = *reinterpret_cast<const float4*>(l + 3 * (CT + 4) + b);
+            const float l10 = l[36 + b];
+            const float2 l2 = *reinterpret_cast<const float2*>(l + 2 * 36 + b);
+            const float4 l3 = *reinterpret_cast<const float4*>(l + 3 * 36 + b);
             float4 x;
             x.x = fmaf(a[0], -MAT_DOWN, c == b ? MAT_UP : 0.f);
             x.y = fmaf(fmaf(l10, x.x, a[1]), -MAT_DOWN, c == b + 1 ? MAT_UP : 0.f);
@@ -419,7 +431,7 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
         const int o = h == 16 ? 32 * (w >> 1) : 0, n0 = h == 16 ? 0 : 16 * (w & 1), i0 = h == 16 ? 0 : 16 * (w >> 1);
         float* t11 = &s.tt[h == 16 ? w >> 1 : 0][0][0];      // T^T of the two diagonal blocks, rows of 36
         const float* t22 = h == 16 ? t11 + 16 * 36 + 16 : &s.tt[1][0][0];
-        const float* l21 = &s.L[o + h + gid][o + 2 * tig];
+        const float* l21 = h == 16 ? &s.L[w & 2][16 + gid][2 * tig] : &s.L[1][gid][2 * tig];
         float d[2][4] = {};
 #pragma unroll 1
         for (int k2 = 0; k2 <= i0; k2 += 16) {               // sixteen rows of L21 T11; T22 is lower triangular
@@ -432,7 +444,7 @@ __device__ __forceinline__ void ck_invert(PrepSmem& s, unsigned char* thi, unsig
                 for (int r = 0; r < 4; ++r) a[r] = pieces(*reinterpret_cast<const float2*>(ta + (r & 1) * 8 * 36 + (r >> 1) * 8));
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float* l = l21 + (k2 + 8 * j) * (CT + 4) + ks;
+                    const float* l = l21 + (k2 + 8 * j) * 36 + ks;
                     mma_pieces(X[j], a, pieces(*reinterpret_cast<const float2*>(l)), pieces(*reinterpret_cast<const float2*>(l + 8)));
                 }
             }
@@ -548,7 +560,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         }
         prep_bar(grp);
         tc_fence_after_sync();
-        ck_gram(ps, s.amat[grp], tm + tm_gram(grp), w, lane);
+        ck_gram(ps, s.ahi[grp], s.alo[grp], tm + tm_gram(grp), w, lane);
         tc_fence_before_sync();                              // (the matrix has been read)
         prep_bar(grp);
         ck_invert(ps, s.thi, s.tlo, c > 0 ? &s.y_full : nullptr, pc ^ 1u, patience, grp, w, lane);
@@ -624,9 +636,6 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 #pragma unroll
                 for (int i = 0; i < 8; ++i) S[8 * p + i] = __ffma2_rn(S[8 * p + i], both(decay), f2_of(r[2 * i], r[2 * i + 1]));
             }
-            // every product of that chunk is through, and its scalars have been read: its buffers are free
-            if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
-            __syncwarp();
         }
         if (c < nchunk) {
             // the row's power of two: B = |S| + sum |v| becomes 2^13 or more
@@ -655,6 +664,15 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 #pragma unroll
                 for (int i = 0; i < SP; ++i) S[i] = __fmul2_rn(S[i], up);
             }
+        }
+        if (c > 0) {
+            ck_wait(patience, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
+            tc_fence_after_sync();
+            // every product of that chunk is through, and its scalars have been read: its buffers are free
+            if (c + 1 < nchunk && lane == 0) mbar_arrive(&s.main_done[buf ^ 1]);
+            __syncwarp();
+        }
+        if (c < nchunk) {
 #pragma unroll
             for (int p = 0; p < SP / 8; ++p) {
                 uint32_t hi[8], lo[8];
@@ -668,8 +686,6 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             ck_ready(&s.s_ready, lane);
         }
         if (c > 0) {                                         // outputs of the chunk before
-            ck_wait(patience, &s.au_full[buf ^ 1], uint32_t((c - 1) >> 1) & 1u);
-            tc_fence_after_sync();
 #pragma unroll 2
             for (int p = 0; p < TP / 4; ++p) {
                 uint32_t x[8];
@@ -740,20 +756,20 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         ck_wait(patience, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
 #pragma unroll 2
-        for (int p = 0; p < TP / 4; ++p) {                   // u for A u (one piece), u e^{G_C - G} kr for the state (two)
-            uint32_t y[8], un[4], hi[4], lo[4];
+        for (int p = 0; p < TP / 4; ++p) {                   // the pieces of u for A u, and of u e^{G_C - G} kr for the state
+            uint32_t y[8], uhi[4], ulo[4], hi[4], lo[4];
             tmem_ld_8(row + tmy + 2 * TP * h + 8 * p, y);
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
                 const float4 cc = *reinterpret_cast<const float4*>(&q.c3[2 * TP * h + 8 * p + 2 * i]);
                 const float2 u0 = f2_of(y[2 * i], y[2 * i + 1]), u1 = f2_of(y[2 * i + 2], y[2 * i + 3]);
-                const float2 d0 = __fmul2_rn(u0, both(MAT_DOWN)), d1 = __fmul2_rn(u1, both(MAT_DOWN));
-                un[i] = h2_bits(__floats2half2_rn(d0.x, d0.y));
-                un[i + 1] = h2_bits(__floats2half2_rn(d1.x, d1.y));
+                split_h2(__fmul2_rn(u0, both(MAT_DOWN)), uhi[i], ulo[i]);
+                split_h2(__fmul2_rn(u1, both(MAT_DOWN)), uhi[i + 1], ulo[i + 1]);
                 split_h2(__fmul2_rn(u0, make_float2(cc.x, cc.y)), hi[i], lo[i]);
                 split_h2(__fmul2_rn(u1, make_float2(cc.z, cc.w)), hi[i + 1], lo[i + 1]);
             }
-            tmem_st_4(row + TM_UOP + TP * h + 4 * p, un);
+            tmem_st_4(row + TM_UHI + TP * h + 4 * p, uhi);
+            tmem_st_4(row + TM_ULO + TP * h + 4 * p, ulo);
             tmem_st_4(row + TM_PHI + TP * h + 4 * p, hi);
             tmem_st_4(row + TM_PLO + TP * h + 4 * p, lo);
         }
@@ -791,8 +807,11 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
         }
         umma_commit_if(el, &s.ks_full);
 #pragma unroll 2
-        for (int ks = 0; ks < 8; ++ks)                       // S q^T
-            umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, kq + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4), ck_idesc(64, false), ks > 0);
+        for (int ks = 0; ks < 8; ++ks) {                     // S q^T
+            const uint64_t d = kq + uint64_t(((ks >> 2) * 16384 + 8192 + (ks & 3) * 32) >> 4);
+            umma_f16_ts(el, tm + TM_XQ, tm + TM_SHI + 8 * ks, d, ck_idesc(64, false), ks > 0);
+            umma_f16_ts(el, tm + TM_XQ, slo + 8 * ks, d, ck_idesc(64, false), 1u);
+        }
         umma_commit_if(el, &s.qs_full);
         ck_wait(patience, &s.ta_full[buf], ph);
         ck_wait(patience, &s.r_ready, pc);
@@ -814,18 +833,24 @@ __device__ __forceinline__ void ck_issue(ChunkSmem& s, const CUtensorMap* rows, 
         __syncwarp();
         ck_wait(patience, &s.u_ready, pc);
         tc_fence_after_sync();
-        const uint64_t am = ck_desc(smem_u32(s.amat[buf]), 16);
 #pragma unroll 2
-        for (int ks = 0; ks < 4; ++ks) umma_f16_ts(el, slo, tm + TM_UOP + 8 * ks, am + 2 * ks, ck_idesc(64, false), 1u);       // A u
-        if (el) bulk_wait_read();                            // au_full says that the outputs' buffer is free, too
-        __syncwarp();
-        umma_commit_if(el, &s.au_full[buf]);
-#pragma unroll 2
-        for (int ks = 0; ks < 4; ++ks) {                     // the chunk's part of the state
+        for (int ks = 0; ks < 4; ++ks) {                     // the chunk's part of the state, which the next one waits for
             umma_f16_ts(el, tm + TM_D, tm + TM_PHI + 8 * ks, kt + 128 * ks, ck_idesc(128, true), ks > 0);
             umma_f16_ts(el, tm + TM_D, tm + TM_PLO + 8 * ks, kt + 128 * ks, ck_idesc(128, true), 1u);
         }
         umma_commit_if(el, &s.d_full);
+        const uint32_t ah = smem_u32(s.ahi[buf]), al = smem_u32(s.alo[buf]);
+#pragma unroll 2
+        for (int ks = 0; ks < 4; ++ks) {                     // A u; the values of tokens 32 .. reach the outputs of tokens 32 .. alone
+            const uint32_t at = ks < 2 ? 2048u * ks : 4096u + 1024u * (ks - 2), step = ks < 2 ? 1024u : 512u, to = ks < 2 ? slo : slo + 32u;
+            const uint32_t shape = ck_idesc(ks < 2 ? 64 : 32, false);
+            umma_f16_ts(el, to, tm + TM_UHI + 8 * ks, ck_desc_cores(ah + at, step), shape, 1u);
+            umma_f16_ts(el, to, tm + TM_UHI + 8 * ks, ck_desc_cores(al + at, step), shape, 1u);
+            umma_f16_ts(el, to, tm + TM_ULO + 8 * ks, ck_desc_cores(ah + at, step), shape, 1u);
+        }
+        if (el) bulk_wait_read();                            // au_full says that the outputs' buffer is free, too
+        __syncwarp();
+        umma_commit_if(el, &s.au_full[buf]);
     }
     umma_commit_if(el, &s.fin);
     if (el) bulk_wait_all();
@@ -1034,8 +1059,8 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
         len = len - seg * g.tokens < g.tokens ? len - seg * g.tokens : g.tokens;
     }
 #pragma unroll 1
-    for (int i = tid; i < 4 * 8192 / 16; i += CK_THREADS) reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);   // the upper right
-                                                                                    // blocks of T (head, remainder) and both A stay zero
+    for (int i = tid; i < 2 * 8192 / 16; i += CK_THREADS) reinterpret_cast<uint4*>(s.thi)[i] = make_uint4(0u, 0u, 0u, 0u);   // the upper right
+                                                                                    // blocks of T (head, remainder) stay zero
 #pragma unroll 1
     for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
     if (warp == 0) tmem_alloc(&s.tm, 512);
