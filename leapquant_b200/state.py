@@ -111,14 +111,13 @@ class LeapQuantState:
         self._kconv_prompt = None
         self._vkey = None
         self._v = None
-        self._f32 = {}
 
-    def _p32(self, t):
-        """fp32 copy of a layer parameter, cached per tensor (several layers can share one state tensor)."""
-        c = self._f32.get(t.data_ptr())
-        if c is None:
-            c = self._f32[t.data_ptr()] = t.detach().to(torch.float32).contiguous()
-        return c
+    @staticmethod
+    def _p32(t):
+        """fp32 copy of a layer parameter, made anew for every call on the call's stream.  (Kept copies went stale: weights are reloaded in
+        place without a new version number, addresses are used again, other streams read too early.)  A layer that has its parameters
+        in fp32 saves the launch."""
+        return t.detach().to(torch.float32).contiguous()
 
     def views(self, ssm):
         k = _ident(ssm)
