@@ -231,6 +231,10 @@ int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixe
                    const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
                    const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale, void* work,
                    int64_t work_bytes, void* stream);
+/* What lq_gdn_prefill would answer to these operands without its launches: for a caller that changes something else first. */
+int lq_gdn_prefill_check(const lq_dims* d, const float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
+                         const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
+                         const int32_t* idx, const void* o, int32_t N, int64_t T);
 /* Scratch with which lq_gdn_prefill splits long sequences over the SMs that N * HV heads leave idle (16-byte aligned, any contents; not
  * shared by calls that overlap); 0 where that would not be faster.  With less than this (or NULL) a head's sequence runs on one SM. */
 int64_t lq_prefill_work_bytes(int32_t N, int32_t HV, int64_t T);

@@ -15,8 +15,8 @@ LIB_PATH = os.environ.get("LEAPQUANT_B200_LIB") or os.path.join(_HERE, "libleapq
 EXPORTS = ("lq_version", "lq_strerror", "lq_last_cuda_error", "lq_device_status", "lq_set_option", "lq_gdn_step", "lq_kda_step",
            "lq_flush", "lq_gdn_decode", "lq_kda_decode", "lq_gdn_decode_conv", "lq_kda_decode_conv", "lq_causal_conv1d_update",
            "lq_decode_work_bytes", "lq_gdn_decode_noalloc",
-           "lq_quantize", "lq_dequant", "lq_lowrank", "lq_gdn_prefill", "lq_prefill_work_bytes", "lq_gdn_recurrent", "lq_causal_conv1d_prompt",
-           "lq_gated_norm", "lq_add_norm")
+           "lq_quantize", "lq_dequant", "lq_lowrank", "lq_gdn_prefill", "lq_gdn_prefill_check", "lq_prefill_work_bytes", "lq_gdn_recurrent",
+           "lq_causal_conv1d_prompt", "lq_gated_norm", "lq_add_norm")
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
@@ -74,6 +74,7 @@ def lib():
         L.lq_dequant.argtypes = [D, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _P]
         L.lq_lowrank.argtypes = [_P, _P, _P, _P, _I, _I, _I, _I, _I, _P]
         L.lq_gdn_prefill.argtypes = [D, _P, _P, I64, _P, I64, _P, I64, _P, _P, _P, _P, _P, _P, _I, I64, _F, _P, I64, _P]
+        L.lq_gdn_prefill_check.argtypes = [D, _P, _P, I64, _P, I64, _P, I64, _P, _P, _P, _P, _P, _I, I64]
         L.lq_prefill_work_bytes.argtypes = [_I, _I, I64]
         L.lq_prefill_work_bytes.restype = I64
         L.lq_gdn_recurrent.argtypes = [D, _P, _P, I64, _P, I64, _P, I64, _P, _P, _P, _P, _I, _F, _P]
@@ -82,7 +83,7 @@ def lib():
         L.lq_add_norm.argtypes = [_P, I64, _P, I64, _P, _P, I64, I64, _I, _F, _F, _P]
         for name in ("lq_device_status", "lq_gdn_step", "lq_kda_step", "lq_flush", "lq_quantize", "lq_dequant", "lq_lowrank",
                      "lq_gdn_decode", "lq_kda_decode", "lq_gdn_decode_conv", "lq_kda_decode_conv", "lq_causal_conv1d_update",
-                     "lq_gdn_decode_noalloc", "lq_gdn_prefill", "lq_gdn_recurrent", "lq_causal_conv1d_prompt", "lq_gated_norm",
+                     "lq_gdn_decode_noalloc", "lq_gdn_prefill", "lq_gdn_prefill_check", "lq_gdn_recurrent", "lq_causal_conv1d_prompt", "lq_gated_norm",
                      "lq_add_norm"):
             getattr(L, name).restype = _I
         _lib = L

@@ -1182,18 +1182,27 @@ static RuleParams rule_params(const lq_dims* d, float* ssm, const void* mixed, i
 
 }  // namespace lq
 
+extern "C" int lq_gdn_prefill_check(const lq_dims* d, const float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
+                                    const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
+                                    const int32_t* idx, const void* o, int32_t N, int64_t T) {
+    using namespace lq;
+    if (!d) return LQ_ERR_NULL;
+    if (N > 0 && T > 0 && !cu) return LQ_ERR_NULL;
+    return rule_check(d, rule_params(d, const_cast<float*>(ssm), mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, nullptr,
+                                     const_cast<void*>(o), N, T, 1.f));
+}
+
 extern "C" int lq_gdn_prefill(const lq_dims* d, float* ssm, const void* mixed, int64_t mixed_stride, const void* a, int64_t a_stride,
                               const void* b, int64_t b_stride, const float* A_log, const float* dt_bias, const int32_t* cu,
                               const int32_t* idx, const uint8_t* has_initial, void* o, int32_t N, int64_t T, float scale,
                               void* work, int64_t work_bytes, void* stream) {
     using namespace lq;
-    if (!d) return LQ_ERR_NULL;
+    const int rc = lq_gdn_prefill_check(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, o, N, T);
+    if (rc) return rc;
+    if (misaligned16({work})) return LQ_ERR_ALIGN;
+    if (N == 0 || T == 0) return LQ_OK;
     RuleParams P = rule_params(d, ssm, mixed, mixed_stride, a, a_stride, b, b_stride, A_log, dt_bias, cu, idx, has_initial, o, N,
                                      T, scale);
-    if (N > 0 && T > 0 && !cu) return LQ_ERR_NULL;
-    if (misaligned16({work})) return LQ_ERR_ALIGN;
-    const int rc = rule_check(d, P);
-    if (rc || N == 0 || T == 0) return rc;
     // The lengths are on the device: a batch gets both kernels, and each of its sequences is run by one of them.
     const int impl = g_rule_impl.load(std::memory_order_relaxed);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -273,23 +273,33 @@ def make_gdn_prefill(NS, HV, H, K, V, SS, scale=None):
     every sequence and the end of the last; idx i32 [N], their slots; has_initial bool [N] or None (all): False starts from a zero
     state; o bf16 [T, HV, V].  A sequence without tokens touches nothing; one with idx <= 0, idx >= NS or a slot that an earlier
     one names gets zeros in o and touches no state; rows of o that no sequence owns are left as they are.  Long sequences of few
-    heads are split over the SMs, for which the call takes scratch from torch's allocator (a few MB)."""
+    heads are split over the SMs, for which the call takes scratch from torch's allocator (a few MB).
+    prefill.check takes the same operands and only refuses what prefill would refuse."""
     _need_128(K, V, "make_gdn_prefill")
     shape, strides, C = (NS, HV, V, K), (SS, V * K, K, 1), 2 * H * K + HV * V
     d = ctypes.pointer(_lib.dims(NS, HV, H, K, V, 0, 0, SS))
     sc = float(K ** -0.5 if scale is None else scale)
-    fn, work_bytes = _lib.lib().lq_gdn_prefill, _lib.lib().lq_prefill_work_bytes
+    fn, fn_check, work_bytes = _lib.lib().lq_gdn_prefill, _lib.lib().lq_gdn_prefill_check, _lib.lib().lq_prefill_work_bytes
 
-    def prefill(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
+    def operands(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
         ms, as_, bs = _rule_operands(shape, strides, C, HV, V, S0, mixed, a, b, A_log, dt_bias, idx, o)
         _lib.same_device(S0, cu, has_initial)
         N, hp = _sequences(cu, idx, has_initial)
-        T = mixed.shape[0]
+        return ms, as_, bs, N, hp, mixed.shape[0]
+
+    def check(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
+        ms, as_, bs, N, _, T = operands(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o)
+        _lib.check(fn_check(d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(), dt_bias.data_ptr(),
+                            cu.data_ptr(), idx.data_ptr(), o.data_ptr(), N, T), "lq_gdn_prefill")
+
+    def prefill(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o):
+        ms, as_, bs, N, hp, T = operands(S0, mixed, a, b, A_log, dt_bias, cu, idx, has_initial, o)
         nw = work_bytes(N, HV, T) if T >= 768 and 0 < N * HV <= 256 else 0
         work = torch.empty(nw, dtype=torch.uint8, device=S0.device) if nw else None
         _launch(fn, "lq_gdn_prefill", S0, d, S0.data_ptr(), mixed.data_ptr(), ms, a.data_ptr(), as_, b.data_ptr(), bs, A_log.data_ptr(),
                 dt_bias.data_ptr(), cu.data_ptr(), idx.data_ptr(), hp, o.data_ptr(), N, T, sc, work.data_ptr() if nw else None, nw)
 
+    prefill.check = check
     return prefill
 
 

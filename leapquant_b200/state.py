@@ -212,7 +212,8 @@ class LeapQuantState:
 
     def prefill_conv(self, ssm, x, conv_state, conv_weight, conv_bias, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial=None):
         """prefill() from the raw q | k | v projections x: the causal conv1d of the prompts first (operands as for decode_conv; the
-        conv state of every sequence is advanced, or starts at zero where has_initial is False).  The T activated rows are
+        conv state of every sequence is advanced, or starts at zero where has_initial is False; a call that is refused changes
+        neither).  The T activated rows are
         allocated from torch's allocator for the call."""
         self._need_gdn("prefill_conv")
         C = 2 * self.H * self.K + self.HV * self.V
@@ -220,6 +221,10 @@ class LeapQuantState:
             self._kconv_prompt = KN.make_conv1d_prompt(self.NS, C)
         mixed = torch.empty(x.shape[0], C, dtype=torch.bfloat16, device=x.device)
         idx, cu_seqlens = idx.to(torch.int32), cu_seqlens.to(torch.int32)
+        A_log = A_log if A_log.dtype == torch.float32 else self._p32(A_log)
+        dt_bias = dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias)
+        # the conv advances its state in place: what the rule would refuse is refused before it
+        self.kprefill.check(ssm, mixed, a, b, A_log, dt_bias, cu_seqlens, idx, has_initial, out)
         self._kconv_prompt(x, conv_state, conv_weight, conv_bias, cu_seqlens, idx, has_initial, mixed)
         self.prefill(ssm, mixed, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial)
 

@@ -88,3 +88,58 @@ def test_bf16_parameters_in_graphs_and_on_streams():
         assert torch.equal(o, want[0]) and torch.equal(S.view(torch.int32), want[1])
         A_log.add_(1.0)
         want = calls(st, ssm, mixed, a, b, A_log.float(), dt_bias.float(), "decode_dense")
+
+
+@gpu
+def test_a_refused_prefill_conv_changes_nothing():
+    """Whatever the rule refuses, the conv states have not been advanced; the corrected call then gives what it gives by itself."""
+    from leapquant_b200 import _lib
+    st, ssm, mixed, a, b, A_log, dt_bias = layer(53)
+    A_log, dt_bias = A_log.float(), dt_bias.float()
+    T, C = mixed.shape
+    conv = torch.randn(3, 3, C, generator=torch.Generator().manual_seed(2)).bfloat16().cuda()
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    idx, cu = torch.tensor([1, 2], dtype=torch.int32, device="cuda"), offsets([60, 10]).cuda()
+    o = torch.zeros(T, 4, V, dtype=torch.bfloat16, device="cuda")
+    good = dict(a=a, b=b, A_log=A_log, dt_bias=dt_bias, out=o, ssm=ssm, has_initial=None)
+    buf = torch.zeros(T * 4 * V + 8, dtype=torch.bfloat16, device="cuda")
+    over = torch.zeros(T * 4 * V + T * 8, dtype=torch.bfloat16, device="cuda")
+    bad = [dict(a=a[:, :3]), dict(b=b.float()), dict(a=a[:T - 1]), dict(A_log=A_log[:3]), dict(dt_bias=dt_bias.double()[:2]), dict(out=o[:T - 1]),
+           dict(out=o.float()), dict(ssm=ssm[:2]), dict(ssm=ssm.bfloat16()), dict(has_initial=torch.ones(3, dtype=torch.bool, device="cuda")), dict(out=o.cpu()),
+           dict(out=buf[4:4 + T * 4 * V].view(T, 4, V)),                                 # outputs that start off 16 bytes
+           dict(out=over[:T * 4 * V].view(T, 4, V), a=over[8:8 + T * 8].view(T, 8)[:, :4])]      # a inside the outputs
+    x, before, states = mixed.contiguous(), conv.clone(), ssm.clone()
+
+    def call(conv, ssm, a, b, A_log, dt_bias, out, has_initial):
+        st.prefill_conv(ssm, x, conv.transpose(1, 2), w, None, a, b, A_log, dt_bias, idx, cu, out, has_initial)
+        torch.cuda.synchronize()
+
+    for kw in bad:
+        with pytest.raises(_lib.LeapQuantError):
+            call(conv, **{**good, **kw})
+        assert torch.equal(conv, before) and torch.equal(ssm, states), list(kw)
+    call(conv, **good)
+    assert not torch.equal(conv[1:], before[1:]) and torch.equal(conv[0], before[0])
+    act = torch.empty(T, C, dtype=torch.bfloat16, device="cuda")
+    again, S, o2 = before.clone(), states.clone(), torch.zeros_like(o)
+    st._kconv_prompt(x, again.transpose(1, 2), w, None, cu, idx, None, act)
+    st.prefill(S, act, a, b, A_log, dt_bias, idx, cu, o2)
+    assert torch.equal(again, conv) and torch.equal(S, ssm) and torch.equal(o2, o)
+
+
+def test_the_check_of_a_prefill_answers_like_the_call():
+    """lq_gdn_prefill_check on operands that lq_gdn_prefill refuses: the same codes, without a launch in either."""
+    import ctypes
+    from leapquant_b200 import _lib
+    L, P = _lib.lib(), ctypes.c_void_p
+    d = _lib.dims(8, 4, 2, 128, 128, 0, 0, 4 * 128 * 128)
+    base = dict(ssm=P(1 << 40), mixed=P(1 << 41), ms=1024, a=P(1 << 42), as_=4, b=P(1 << 43), bs=4, A=P(256), dt=P(256), cu=P(256), idx=P(256), o=P(1 << 44), N=1, T=5)
+    assert L.lq_gdn_prefill_check(d, *base.values()) == 0
+    for kw, rc in ((dict(N=0), 0), (dict(T=0), 0), (dict(N=-1), -4), (dict(T=-1), -4), (dict(cu=None), -1), (dict(o=None), -1), (dict(ms=1028), -3), (dict(ms=1016), -4),
+                   (dict(as_=3), -4), (dict(o=P((1 << 44) + 8)), -3), (dict(o=P((1 << 41) + 1024)), -4), (dict(o=P((1 << 42) + 16)), -4), (dict(ssm=P((1 << 40) + 4)), -3)):
+        v = {**base, **kw}
+        assert L.lq_gdn_prefill_check(d, *v.values()) == rc, kw
+        N, T = v.pop("N"), v.pop("T")
+        o = v.pop("o")
+        assert L.lq_gdn_prefill(d, *v.values(), None, o, N, T, 0.0, None, 0, None) == rc, kw
+    assert L.lq_gdn_prefill_check(None, *base.values()) == -1
