@@ -61,6 +61,7 @@ constexpr int CK_MAIN = 128 * MG, CK_PREP = 128, CK_THREADS = CK_MAIN + 2 * CK_P
 // Registers: 17 warps get 96 each (five of them share a quarter of the SM).  The main warps take over what the prep warps give up,
 // 256 * 128 + 256 * 64 + 32 * 96 = 544 * 96; the launch looks that the kernel was built so, or they would wait for good.
 constexpr int CK_REGS = 96, CK_MAIN_REGS = 128, CK_PREP_REGS = 64;
+static_assert(MG == 2, "a thread exchanges its half of a row with one other");
 static_assert(CK_MAIN * CK_MAIN_REGS + 2 * CK_PREP * CK_PREP_REGS + 32 * CK_REGS <= CK_THREADS * CK_REGS, "register split");
 
 // Tensor memory, 512 columns.  D takes the place of X | XQ once both have been read.  The pieces of u for A u take that of S's heads once
@@ -142,10 +143,12 @@ __device__ __forceinline__ void ck_wait(int& patience, uint64_t* bar, uint32_t p
     }
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }
-// exponent e with b 2^e in [2^13, 2^14), within what fp32 scaling can carry
+// Exponent e with B 2^e in [2^13, 2^14), of b = B / 256 (a B beyond fp32's range is one as well: 2^128 of state and 64 values of 2^128).  At
+// most 100: a row with a smaller bound, below 2^-87, is carried to 2^-125 at least, where fp32 ends.
+constexpr int E_MIN = -122, E_MAX = 100;
 __device__ __forceinline__ int scale_exponent(float b) {
-    const int e = 140 - int((__float_as_uint(b) >> 23) & 255u);
-    return e < -100 ? -100 : e > 100 ? 100 : e;
+    const int e = 132 - int((__float_as_uint(b) >> 23) & 255u);
+    return e < E_MIN ? E_MIN : e > E_MAX ? E_MAX : e;
 }
 __device__ __forceinline__ uint32_t b2_bits(__nv_bfloat162 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -198,11 +201,12 @@ __device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
     float s = (u2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, u2 ? b[0] : b[1], 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
-// Sums of |v| over the tokens g, g + 8, ... of a chunk (g: this half of a warp), for a bound: bf16 will do, rounded up by the reader.  A
+// Sums of |v| / 256 over the tokens g, g + 8, ... of a chunk (g: this half of a warp), for a bound: bf16 will do, rounded up by the reader.  A
 // lane reads one 16-byte piece of the rows, the same eight values in all of them, since the swizzle goes by the row's number mod 8.
 __device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)[8][VD], int w, int lane) {
     const int g = 2 * w + (lane >> 4), c = lane & 15;
     v += (c >> 3) * 8192 + g * 128 + (c & 7) * 16;
+    const __nv_bfloat162 part = __floats2bfloat162_rn(1.f / 256, 1.f / 256);
     __nv_bfloat162 sum[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) sum[j] = __floats2bfloat162_rn(0.f, 0.f);
@@ -211,7 +215,7 @@ __device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)
         const uint4 x = *reinterpret_cast<const uint4*>(v + 1024 * i);
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[j] = __hadd2(sum[j], __habs2(*reinterpret_cast<const __nv_bfloat162*>(&xw[j])));
+        for (int j = 0; j < 4; ++j) sum[j] = __hfma2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&xw[j])), part, sum[j]);
     }
     *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3]));
 }
@@ -609,7 +613,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         S[2 * i] = make_float2(x.x, x.y);
         S[2 * i + 1] = make_float2(x.z, x.w);
     }
-    int e = 0, plen = 0;
+    int e = Sin || unit ? 0 : E_MAX, plen = 0;
     float decay = 0.f, of = 0.f;                             // of the chunk before: its decay, and what its outputs are multiplied with
     const int vc = (v >> 3) & 7, voff = (v >> 6) * 8192 + 2 * TP * h * 128 + 2 * (v & 7);
 #pragma unroll 1
@@ -624,7 +628,7 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             ck_wait(patience, &s.v_ready[buf], ph);
 #pragma unroll
             for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[g][v]);
-            va *= 1.125f;                                    // (sums in bf16: not below the true one)
+            va *= 1.125f;                                    // (sums in bf16: not below the true one, of |v| / 256)
         }
         if (c > 0) {                                         // the state behind the chunk before
             ck_wait(patience, &s.d_full, uint32_t(c - 1) & 1u);
@@ -639,30 +643,45 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
         }
         if (c < nchunk) {
             // the row's power of two: B = |S| + sum |v| becomes 2^13 or more
-            float2 n2[4];
+            const int pair = 4 + (warp & 3);                 // barrier of the warps that share these rows
+#pragma unroll 1
+            for (bool again = false;; again = true) {
+                float2 n2[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
+                for (int i = 0; i < 4; ++i) n2[i] = __fmul2_rn(S[i], S[i]);
 #pragma unroll
-            for (int i = 4; i < SP; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
-            n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
-            const float mine = n2[0].x + n2[0].y;
-            s.part[buf][tid] = mine;
-            named_bar(4 + (warp & 3), 32 * MG);              // the warps that share these rows
-            float sum2 = mine;
+                for (int i = 4; i < SP; ++i) n2[i & 3] = __ffma2_rn(S[i], S[i], n2[i & 3]);
+                n2[0] = __fadd2_rn(__fadd2_rn(n2[0], n2[1]), __fadd2_rn(n2[2], n2[3]));
+                const float mine = n2[0].x + n2[0].y;
+                s.part[buf][tid] = mine;
+                named_bar(pair, 32 * MG);
+                const float sum2 = mine + s.part[buf][tid ^ 128];
+                // (kept while the bound stays between 2^10 and 2^14)
+                int de = scale_exponent(fmaf(sqrt_approx(sum2), pow2f(-e - 8), va)) - e;
+                if (de >= 0 && de <= 3) de = 0;
+                // Squares stand for their row while they are well inside fp32's range; at the largest exponent only those of zeros are not
+                const bool beyond = !again && !(sum2 < 0x1p120f && (sum2 > 0x1p-100f || e == E_MAX));
+                if (__all_sync(0xffffffffu, de == 0 && !beyond)) break;
+                if (__any_sync(0xffffffffu, beyond)) {
+                    // a state as the caller gives it, or one that decayed far within a chunk: first to a largest value in [1, 2).  (Both warps of
+                    // the rows have seen the same sums.)
+                    float big = 0.f;
 #pragma unroll
-            for (int g = 1; g < MG; ++g) sum2 += s.part[buf][tid ^ (128 * g)];
-            const float bound = fmaf(sqrt_approx(sum2), pow2f(-e), va);
-            // (kept while the bound stays between 2^10 and 2^14)
-            const int en = scale_exponent(bound);
-            int de = en - e;
-            if (de >= 0 && de <= 3) de = 0;
-            // squares below 2^-126 are lost: a row that decayed that far within a chunk has a norm of up to sqrt(128) 2^-63, whatever the sum says
-            if (de > 60) de = 60;
-            if (__any_sync(0xffffffffu, de != 0)) {
-                const float2 up = both(pow2f(de < -126 ? -126 : de > 127 ? 127 : de));
+                    for (int i = 0; i < SP; ++i) big = fmaxf(big, fmaxf(fabsf(S[i].x), fabsf(S[i].y)));
+                    s.part[buf ^ 1][tid] = big;
+                    named_bar(pair, 32 * MG);
+                    big = fmaxf(big, s.part[buf ^ 1][tid ^ 128]);
+                    de = 127 - int((__float_as_uint(big) >> 23) & 255u);
+                    de = de < E_MIN - e ? E_MIN - e : de > E_MAX - e ? E_MAX - e : de;
+                    de = de > 126 ? 126 : de;
+                    if (big == 0.f) de = -e;
+                    again = true;
+                } else again = false;
+                const float2 up = both(de < -126 ? 0.f : pow2f(de));
                 e += de;
 #pragma unroll
                 for (int i = 0; i < SP; ++i) S[i] = __fmul2_rn(S[i], up);
+                if (!again) break;
             }
         }
         if (c > 0) {
