@@ -30,9 +30,10 @@
 // Precision.  k and q are bf16 and become f16 without loss once a row is scaled by a power of two (what is lost lies 2^-25 below the
 // row's norm); an fp32 operand is the sum of two f16 pieces, 22 bits.  f16 has few exponents, so every row of S, r and u carries
 // a power of two of its own, from bounds that hold whatever the inputs: |k^| <= 1, 0 <= beta <= 1 and decays <= 1 make the rule a
-// contraction, |r_t|, |u_t| / 2, |S| <= |S_0| + sum |v_t| =: B per row.  T is bounded by 1 for the same reason.  The outputs get the
-// same pieces as the state: with one piece each in S q and A u (11 bits) they lay 1.0e-3 of their norm from those of the plain form in 32
-// bits, with two 5e-5, as those of the token-by-token form do.
+// contraction, |r_t|, |u_t|, |S| <= |S_0| + sum |v_t| =: B per row, which is brought to 2^13 .. 2^15 for every chunk.  What a chunk
+// makes of a row below 2^-38 of its B, as behind a decay of that much, is lost: the last bit of an f16.  T is bounded by 1 for the same
+// reason.  The outputs get the same pieces as the state: with one piece each in S q and A u (11 bits) they lay 1.0e-3 of their norm from
+// those of the plain form in 32 bits, with two 5e-5, as those of the token-by-token form do.
 #include <cuda.h>
 #include <stddef.h>
 
@@ -656,9 +657,9 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                 s.part[buf][tid] = mine;
                 named_bar(pair, 32 * MG);
                 const float sum2 = mine + s.part[buf][tid ^ 128];
-                // (kept while the bound stays between 2^10 and 2^14)
+                // (kept while the bound stays between 2^13 and 2^15)
                 int de = scale_exponent(fmaf(sqrt_approx(sum2), pow2f(-e - 8), va)) - e;
-                if (de >= 0 && de <= 3) de = 0;
+                if (de == -1) de = 0;
                 // Squares stand for their row while they are well inside fp32's range; at the largest exponent only those of zeros are not
                 const bool beyond = !again && !(sum2 < 0x1p120f && (sum2 > 0x1p-100f || e == E_MAX));
                 if (__all_sync(0xffffffffu, de == 0 && !beyond)) break;

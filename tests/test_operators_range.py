@@ -17,14 +17,14 @@ gpu = pytest.mark.gpu
 H, HV = 2, 4
 
 
-def check_rows(S, S64, o, o64, size, start, values, lens, slots, scale, T, rel=2.0 ** -15):
+def check_rows(S, S64, o, o64, size, start, values, lens, slots, scale, T, rel=2.0 ** -15, B=None):
     """S, o against the 64-bit ones, every row of every sequence within its own bound."""
     t0 = 0
     for ln, slot in zip(lens, slots):
         M = size[t0:t0 + ln] / scale                         # [ln, HV, V]
         # B of any of the sequence's chunks: the state it starts from, and 64 values
-        B = torch.maximum(M.amax(0), start[slot]) + 64 * values[t0:t0 + ln].amax(0)
-        end = 2.0 ** -31 * B + 2.0 ** -118
+        most = torch.maximum(M.amax(0), start[slot]) + 64 * values[t0:t0 + ln].amax(0) if B is None else B
+        end = 2.0 ** -31 * most + 2.0 ** -118
         x, x64 = o[t0:t0 + ln].double(), o64[t0:t0 + ln]
         off = (x - x64).abs() - half_step(x64) - scale * (rel * M + end)
         assert float(off.max()) <= 0, ("outputs", slot, float(off.max()), float((off / (scale * M).clamp(min=1e-300)).max()))
@@ -33,7 +33,7 @@ def check_rows(S, S64, o, o64, size, start, values, lens, slots, scale, T, rel=2
         t0 += ln
 
 
-def run(lens, change, seed, fresh=None, state=1.0, rel=2.0 ** -15):
+def run(lens, change, seed, fresh=None, state=1.0, rel=2.0 ** -15, B=None):
     from leapquant_b200.kernels import make_gdn_prefill
     n, T = len(lens), sum(lens)
     slots = list(range(1, n + 1))
@@ -47,7 +47,7 @@ def run(lens, change, seed, fresh=None, state=1.0, rel=2.0 ** -15):
     o = torch.zeros(T, HV, V, dtype=torch.bfloat16, device="cuda")
     hi = torch.tensor([not f for f in fresh], device="cuda")
     make_gdn_prefill(n + 1, HV, H, K, V, ssm.stride(0))(ssm, mixed, a, b, A_log, dt_bias, offsets(lens).cuda(), torch.tensor(slots, dtype=torch.int32).cuda(), hi, o)
-    check_rows(ssm, S64, o, o64, size, start, mixed[:, 2 * H * K:].double().abs().view(T, HV, V), lens, slots, K ** -0.5, T, rel)
+    check_rows(ssm, S64, o, o64, size, start, mixed[:, 2 * H * K:].double().abs().view(T, HV, V), lens, slots, K ** -0.5, T, rel, B)
     clean()
 
 
@@ -106,3 +106,28 @@ def test_ends_of_the_range_in_segments(case):
     assert _lib.lib().lq_prefill_work_bytes(1, HV, 1400) > 0
     change, state = CASES[case]
     run([1400], change, 62, state=state, rel=2.0 ** -14)
+
+
+@gpu
+def test_a_row_that_shrank_keeps_its_bits(impl):
+    """A row's power of two is chosen so that its bound B becomes 2^13 or more, also in the chunk after one that left an eighth of it.  The
+    state starts at 1.001 2^m and loses 2^-2.95 in the first chunk and 2^-24 with the first token of the second; then 63 tokens write
+    a little of it back along one key, all with the same rounding.  With the bound at 2^10 these add up to 50 2^-25 2^-10 = 2^-29.4 of B, with
+    2^13 to 2^-32.4, against the 2^-31 of B that are promised: of the second chunk's B, 2^-2.95, since the first one, whose key meets zeros,
+    writes nothing."""
+    def change(ssm, mixed, a, b, A_log, dt_bias):
+        A_log.fill_(0.0)
+        dt_bias.fill_(0.0)
+        a.fill_(-40.0)
+        a[3] = 1.90625                                       # softplus: 2.0446 = 2.95 log 2
+        a[64] = 16.625                                       # 23.98 log 2
+        b.fill_(-4.84)                                       # beta = 2^-7
+        mixed.zero_()
+        for h in range(2 * H):                               # q and k
+            mixed[:64, h * K + 5] = 1.0
+            mixed[64:, h * K + 1] = 1.0
+        ssm.zero_()
+        ssm[1, :, :, 0] = 0.7
+        ssm[1, :, :, 1] = 0.7 * (1 + torch.linspace(0, 0.4, V, device="cuda"))         # (their roundings differ)
+        ssm *= 1.001 / ssm[1].norm(dim=-1).clamp(min=1e-30)[None, ..., None]
+    run([128], change, 63, B=1.001 * 2.0 ** -2.949)
