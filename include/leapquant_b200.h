@@ -223,6 +223,9 @@ int lq_lowrank(const float* x, const float* Q0, float* U, float* Q, int32_t n, i
  *     S <- e^g S;  u = beta (v - S k^);  S <- S + u k^T;  o = S q^                    (fp32; o rounded to bf16 once)
  * A sequence of 28 tokens or more (8 in a batch of few heads and long sequences) is taken in chunks of 64 tokens, where the factors of
  * fp32 products carry 22 bits and what falls below 2^-38 of |S row| + sum |v row| of the chunk, as behind a decay of that much, is lost.
+ * Infinities and NaN reach what depends on them as values that are not finite, and nothing before their token: of q its token's outputs, of
+ * k, a and b the head from there on, of v and of a state's row that value dimension from there on.  |q|^2 and |k|^2 are fp32 sums: a row
+ * whose sum overflows counts as zeros.
  *   - mixed bf16 rows q | k | v (2 H K + HV V elements, row stride mixed_stride, a multiple of 8); a, b bf16 [T, HV] with row strides;
  *     A_log, dt_bias f32 [HV]; cu i32 [N + 1], ascending; idx i32 [N]; o bf16 [T, HV, V] contiguous.  scale <= 0 selects K^-1/2.
  *   - has_initial (u8 [N], may be NULL = all): 0 starts the sequence from a zero state instead of its slot's.

@@ -107,6 +107,14 @@ struct alignas(16) PrepSmem {                                // of one prep grou
     float kr[CT], qr[CT], ws[32], beta[CT];                  // 1 / |k|, 1 / |q|; ws: kr_s times the decay from s to token 31, for s < 32
     float down[2 * CT];                                      // powers of two that take the rows of k and q to f16
 };
+// Infinities and NaN.  A product with zero would carry them to tokens before their own, so they are taken out of a chunk's operands, and
+// what depends on them becomes NaN at the end: a head's outputs and state from token `from` on (a key, a gate), the outputs of single
+// tokens (q: bits by token), and a value dimension from its first such value on, which the main warps learn from the sums of |v|.
+struct alignas(16) ChunkOdd {
+    int from;                                                // CT: none
+    uint32_t q[2];
+};
+constexpr int ODD_RING = 8;                                  // chunk c's: set up during chunk c - 4, last read when the outputs of c are written
 struct alignas(16) ChunkSmem {
     // start: 1 KB aligned.  tile: two blocks of 64 elements, each 64 rows of k and then 64 rows of q.
     unsigned char tile[2][32768];
@@ -118,6 +126,8 @@ struct alignas(16) ChunkSmem {
     ChunkScalars sc[2];
     uint16_t vsum[8][VD];                                    // bf16 sums of |v| of a value dimension, over every eighth token each
     float part[2][CK_MAIN];
+    ChunkOdd odd[ODD_RING];
+    uint8_t vfrom[2][CK_MAIN];                               // by main thread: first token of its value dimension that is not finite
     uint64_t raw_full[2], v_full[2], v_ready[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
     uint32_t tm;
     int dead;                                                // a wait has run out
@@ -202,9 +212,11 @@ __device__ __forceinline__ float fold8(const float (&v)[8], int lane) {
     float s = (u2 ? b[1] : b[0]) + __shfl_xor_sync(0xffffffffu, u2 ? b[0] : b[1], 2);
     return s + __shfl_xor_sync(0xffffffffu, s, 1);
 }
+// whether one of two bf16 values is an infinity or NaN
+__device__ __forceinline__ bool not_finite(uint32_t two) { return (two & 0x7f80u) == 0x7f80u || (two & 0x7f800000u) == 0x7f800000u; }
 // Sums of |v| / 256 over the tokens g, g + 8, ... of a chunk (g: this half of a warp), for a bound: bf16 will do, rounded up by the reader.  A
 // lane reads one 16-byte piece of the rows, the same eight values in all of them, since the swizzle goes by the row's number mod 8.
-__device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)[8][VD], int w, int lane) {
+__device__ __forceinline__ void ck_vsum(unsigned char* v, uint16_t (&vsum)[8][VD], int w, int lane) {
     const int g = 2 * w + (lane >> 4), c = lane & 15;
     v += (c >> 3) * 8192 + g * 128 + (c & 7) * 16;
     const __nv_bfloat162 part = __floats2bfloat162_rn(1.f / 256, 1.f / 256);
@@ -218,7 +230,23 @@ __device__ __forceinline__ void ck_vsum(const unsigned char* v, uint16_t (&vsum)
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum[j] = __hfma2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&xw[j])), part, sum[j]);
     }
-    *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3]));
+    uint32_t out[4] = {b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3])};
+    const uint32_t all = b2_bits(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])));
+    if (__builtin_expect(not_finite(all), 0)) {              // cleared; the place of a sum takes a NaN with the first such token in it
+#pragma unroll 1
+        for (int i = 7; i >= 0; --i) {
+            uint32_t* x = reinterpret_cast<uint32_t*>(v + 1024 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = x[j], lo = not_finite(w << 16) ? 0xffffu : 0u, hi = not_finite(w & 0xffff0000u) ? 0xffff0000u : 0u;
+                x[j] = w & ~(lo | hi);
+                if (lo) out[j] = (out[j] & 0xffff0000u) | 0x7fc0u | uint32_t(i);
+                if (hi) out[j] = (out[j] & 0xffffu) | (0x7fc0u | uint32_t(i)) << 16;
+            }
+        }
+        fence_async_smem();                                  // (the next copy of v goes to the same place)
+    }
+    *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(out[0], out[1], out[2], out[3]);
 }
 // rows behind the chunk's last token, which belong to other sequences, become zeros; pieces of 16 bytes, blocks of 64 rows
 __device__ __forceinline__ void ck_clear(unsigned char* p, int blocks, int len, int pt, int threads) {
@@ -227,7 +255,7 @@ __device__ __forceinline__ void ck_clear(unsigned char* p, int blocks, int len, 
         if (((i >> 3) & 63) >= len) *reinterpret_cast<uint4*>(p + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
 }
 // Norms of the rows of k (warps 0 and 1) and q.  A lane takes the same 16 bytes of sixteen rows, whichever they are in the swizzle.
-__device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* down, int w, int lane) {
+__device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* down, ChunkOdd& odd, int w, int lane) {
     const int c = lane & 15;
     raw += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
 #pragma unroll 1
@@ -240,12 +268,21 @@ __device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* d
             const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2)), c2 = __fadd2_rn(a, b);
             ss[i] = c2.x + c2.y;
         }
-        const float sum = fold8(ss, lane);
-        // a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does
-        if (__any_sync(0xffffffffu, sum > 3.4e38f)) {
+        float sum = fold8(ss, lane);
+        // a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does, and so does an infinity or NaN, which is noted
+        if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 3.4e38f)), 0)) {
 #pragma unroll 1
-            for (int i = 0; i < 8; ++i)
-                if (__shfl_sync(0xffffffffu, sum, (lane & 16) | (i << 1)) > 3.4e38f) *reinterpret_cast<uint4*>(raw + 2048 * p + 256 * i) = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < 8; ++i) {
+                uint4* at = reinterpret_cast<uint4*>(raw + 2048 * p + 256 * i);
+                const unsigned bad = __ballot_sync(0xffffffffu, not_finite(at->x) || not_finite(at->y) || not_finite(at->z) || not_finite(at->w));
+                if (!(__shfl_sync(0xffffffffu, sum, (lane & 16) | (i << 1)) <= 3.4e38f)) *at = make_uint4(0u, 0u, 0u, 0u);
+                if (c == 0 && (bad >> (lane & 16) & 0xffffu)) {
+                    const int t = 16 * p + 2 * i + (lane >> 4);
+                    if (w < 2) atomicMin(&odd.from, 32 * w + t);
+                    else atomicOr(&odd.q[w & 1], 1u << t);
+                }
+            }
+            sum = fminf(sum, __int_as_float(0x7f800000));    // (of NaN: the infinity)
         }
         // the row times 2^-e has a norm in [1, 2)
         int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
@@ -292,16 +329,22 @@ __device__ __forceinline__ float softplus_log2(float x) {
     return fmaf(2.0f * 1.4426950408889634f * r, p, x > 0.f ? x * 1.4426950408889634f : 0.f);
 }
 // decays and beta of the chunk, by one warp: lane l has the tokens 2 l and 2 l + 1; sums in fp64
-__device__ __forceinline__ void ck_gates(PrepSmem& s, const uint16_t* a, int64_t a_step, const uint16_t* b, int64_t b_step, int len, float ea,
+__device__ __forceinline__ void ck_gates(PrepSmem& s, ChunkOdd& odd, const uint16_t* a, int64_t a_step, const uint16_t* b, int64_t b_step, int len, float ea,
                                          float dtb, int lane) {
     double g[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int t = 2 * lane + i, u = t < len ? t : 0;
         const float x = -ea * softplus_log2(bf16_to_f(__ldg(a + u * a_step)) + dtb), y = bf16_to_f(__ldg(b + u * b_step));
-        // a decay of 2^-200 leaves nothing in fp32; bounded, the differences stay finite
-        g[i] = t < len ? double(x < -200.f ? -200.f : x) : 0.0;
-        s.beta[t] = t < len ? __fdividef(1.0f, 1.0f + ex2(-1.4426950408889634f * y)) : 0.f;
+        const float be = __fdividef(1.0f, 1.0f + ex2(-1.4426950408889634f * y));
+        bool in = t < len;
+        if (__builtin_expect(in && !(x <= 0.f && be >= 0.f), 0)) {
+            atomicMin(&odd.from, t);
+            in = false;
+        }
+        // a decay of 2^-300 leaves nothing in fp32; bounded, the differences stay finite
+        g[i] = in ? double(x < -300.f ? -300.f : x) : 0.0;
+        s.beta[t] = in ? be : 0.f;
     }
     double sum = g[0] + g[1];
 #pragma unroll
@@ -507,17 +550,23 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
         const uint32_t ph = uint32_t(c >> 1) & 1u, pc = uint32_t(c) & 1u;
         const int64_t at = t0 + int64_t(c) * CT, left = len - int64_t(c) * CT;
         const int n = int(left < CT ? left : CT);
+        ChunkOdd& odd = s.odd[c & (ODD_RING - 1)];
         if (w == 3)
-            ck_gates(ps, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
+            ck_gates(ps, odd, P.a + at * P.a_stride + hv, P.a_stride, P.b + at * P.b_stride + hv, P.b_stride, n, ea, dtb, lane);
         ck_wait(patience, &s.raw_full[grp], ph);
         if (c != 1) ck_values(s, c == 0 ? 0 : c - 1, vlen, grp, w, lane, patience);     // of the chunk before: the other group has its hands full
         if (n < CT) {
             ck_clear(s.raw, 4, n, pt, CK_PREP);
             prep_bar(grp);
         }
-        ck_norms(s.raw, w < 2 ? ps.kr : ps.qr, ps.down, w, lane);
+        ck_norms(s.raw, w < 2 ? ps.kr : ps.qr, ps.down, odd, w, lane);
         fence_async_smem();
         prep_bar(grp);
+        if (pt == 0) {
+            ChunkOdd& later = s.odd[(c + 4) & (ODD_RING - 1)];
+            later.from = CT;
+            later.q[0] = later.q[1] = 0;
+        }
         if (w == 0) {                                        // K K^T and Q K^T of the rows as they are
             tc_fence_after_sync();
             const uint64_t d0 = ck_desc(smem_u32(s.raw), 16);
@@ -630,6 +679,18 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 #pragma unroll
             for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[g][v]);
             va *= 1.125f;                                    // (sums in bf16: not below the true one, of |v| / 256)
+            int from = CT;
+            if (__builtin_expect(!(va < 3.4e38f), 0)) {      // some were not finite: when the first, and the sum of the others
+                va = 0.f;
+                const unsigned char* all = s.v + (v >> 6) * 8192 + 2 * (v & 7);
+#pragma unroll 1
+                for (int t = 0; t < CT; ++t) {
+                    const uint32_t g = s.vsum[t & 7][v];
+                    if ((g & 0x7f80u) == 0x7f80u && int(g & 7u) == t >> 3) from = min(from, t);
+                    va += (1.f / 256) * fabsf(bf16_to_f(*reinterpret_cast<const uint16_t*>(all + t * 128 + ((vc ^ (t & 7)) << 4))));
+                }
+            }
+            s.vfrom[buf][tid] = uint8_t(from);
         }
         if (c > 0) {                                         // the state behind the chunk before
             ck_wait(patience, &s.d_full, uint32_t(c - 1) & 1u);
@@ -719,12 +780,19 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                     op[(2 * i + 1) * VD] = uint16_t(b >> 16);
                 }
             }
+            if (__builtin_expect(plen >> 8 != CT, 0)) {      // what depends on an infinity or NaN
+                const uint32_t late = plen >> 8 & 255, bits = s.odd[(c - 1) & (ODD_RING - 1)].q[h];
+#pragma unroll 1
+                for (int i = 0; i < 2 * TP; ++i)
+                    if (2 * TP * h + i >= late || (bits >> i & 1u)) s.o[2 * TP * h + i][v] = 0x7fff;
+                plen &= 255;
+            }
             fence_async_smem();
         }
         if (c == nchunk) {
             named_bar(1, CK_MAIN);
 #pragma unroll 1
-            for (int r = tid >> 4; r < (outputs ? plen : 0); r += CK_MAIN / 16)
+            for (int r = tid >> 4; r < (outputs ? plen & 255 : 0); r += CK_MAIN / 16)
                 *reinterpret_cast<uint4*>(P.o + ((t0 + int64_t(c - 1) * CT + r) * P.HV + hv) * VD + 8 * (tid & 15)) =
                     *reinterpret_cast<const uint4*>(&s.o[r][8 * (tid & 15)]);
             break;
@@ -770,8 +838,12 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             }
             tmem_st_8(row + slo + 2 * TP * h + 8 * p, x);
         }
-        decay = q.decay;
-        plen = q.len;
+        {
+            const ChunkOdd& odd = s.odd[c & (ODD_RING - 1)];
+            const int from = min(int(s.vfrom[buf][tid]), odd.from);
+            decay = from < CT ? __int_as_float(0x7fffffff) : q.decay;
+            plen = q.len | from << 8 | ((odd.q[0] | odd.q[1]) ? 1 << 16 : 0);
+        }
         of = P.scale * pow2f(-e) * MAT_DOWN;
         ck_wait(patience, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
@@ -1083,6 +1155,10 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
                                                                                     // blocks of T (head, remainder) stay zero
 #pragma unroll 1
     for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
+    if (tid < ODD_RING) {
+        s.odd[tid].from = CT;
+        s.odd[tid].q[0] = s.odd[tid].q[1] = 0;
+    }
     if (warp == 0) tmem_alloc(&s.tm, 512);
     fence_async_smem();
     tc_fence_before_sync();
