@@ -97,7 +97,7 @@ struct alignas(16) ChunkScalars {                                        // of o
     float c2[CT];                                            // e^{G_t} qr_t 2^13, the scale of A u
     float c3[CT];                                            // e^{G_C - G_t} kr_t 2^-13 (u comes with the 2^13 of T)
     float decay;                                             // e^{G_C}
-    int len;                                                 // tokens of the chunk, 1 .. 64
+    int len;                                                 // tokens of the chunk, 1 .. 64; from bit 8 on ChunkOdd's `from`, bit 16: some bit of its q
 };
 struct alignas(16) PrepSmem {                                // of one prep group
     float L[3][32][36];                                      // blocks (0, 0), (1, 0), (1, 1); times 2^13, like all that becomes f16 on the way to T
@@ -127,7 +127,7 @@ struct alignas(16) ChunkSmem {
     uint16_t vsum[8][VD];                                    // bf16 sums of |v| of a value dimension, over every eighth token each
     float part[2][CK_MAIN];
     ChunkOdd odd[ODD_RING];
-    uint8_t vfrom[2][CK_MAIN];                               // by main thread: first token of its value dimension that is not finite
+    uint8_t vfrom[CK_MAIN];                                  // by main thread: first token of its value dimension that is not finite
     uint64_t raw_full[2], v_full[2], v_ready[2], tile_full[2], ta_full[2], main_done[2], au_full[2], g_full[2], ks_full, qs_full, y_full, d_full, s_ready, r_ready, u_ready, fin;
     uint32_t tm;
     int dead;                                                // a wait has run out
@@ -230,23 +230,20 @@ __device__ __forceinline__ void ck_vsum(unsigned char* v, uint16_t (&vsum)[8][VD
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum[j] = __hfma2(__habs2(*reinterpret_cast<const __nv_bfloat162*>(&xw[j])), part, sum[j]);
     }
-    uint32_t out[4] = {b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3])};
-    const uint32_t all = b2_bits(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])));
-    if (__builtin_expect(not_finite(all), 0)) {              // cleared; the place of a sum takes a NaN with the first such token in it
+    uint16_t* to = &vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)];
+    *reinterpret_cast<uint4*>(to) = make_uint4(b2_bits(sum[0]), b2_bits(sum[1]), b2_bits(sum[2]), b2_bits(sum[3]));
+    if (__builtin_expect(not_finite(b2_bits(__hadd2(__hadd2(sum[0], sum[1]), __hadd2(sum[2], sum[3])))), 0)) {
+        // cleared; the place of a sum takes a NaN with the first such token in it
 #pragma unroll 1
-        for (int i = 7; i >= 0; --i) {
-            uint32_t* x = reinterpret_cast<uint32_t*>(v + 1024 * i);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = x[j], lo = not_finite(w << 16) ? 0xffffu : 0u, hi = not_finite(w & 0xffff0000u) ? 0xffff0000u : 0u;
-                x[j] = w & ~(lo | hi);
-                if (lo) out[j] = (out[j] & 0xffff0000u) | 0x7fc0u | uint32_t(i);
-                if (hi) out[j] = (out[j] & 0xffffu) | (0x7fc0u | uint32_t(i)) << 16;
+        for (int i = 63; i >= 0; --i) {
+            uint16_t* x = reinterpret_cast<uint16_t*>(v + 1024 * (i >> 3)) + (i & 7);
+            if (not_finite(*x)) {
+                *x = 0;
+                to[i & 7] = uint16_t(0x7fc0 | i >> 3);
             }
         }
         fence_async_smem();                                  // (the next copy of v goes to the same place)
     }
-    *reinterpret_cast<uint4*>(&vsum[g][64 * (c >> 3) + 8 * ((c & 7) ^ g)]) = make_uint4(out[0], out[1], out[2], out[3]);
 }
 // rows behind the chunk's last token, which belong to other sequences, become zeros; pieces of 16 bytes, blocks of 64 rows
 __device__ __forceinline__ void ck_clear(unsigned char* p, int blocks, int len, int pt, int threads) {
@@ -258,6 +255,8 @@ __device__ __forceinline__ void ck_clear(unsigned char* p, int blocks, int len, 
 __device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* down, ChunkOdd& odd, int w, int lane) {
     const int c = lane & 15;
     raw += (c >> 3) * 16384 + (32 * w + (lane >> 4)) * 128 + (c & 7) * 16;
+    rs += 32 * (w & 1);
+    bool large = false;
 #pragma unroll 1
     for (int p = 0; p < 2; ++p) {
         float ss[8];
@@ -268,29 +267,35 @@ __device__ __forceinline__ void ck_norms(unsigned char* raw, float* rs, float* d
             const float2 a = __ffma2_rn(f1, f1, __fmul2_rn(f0, f0)), b = __ffma2_rn(f3, f3, __fmul2_rn(f2, f2)), c2 = __fadd2_rn(a, b);
             ss[i] = c2.x + c2.y;
         }
-        float sum = fold8(ss, lane);
-        // a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does, and so does an infinity or NaN, which is noted
-        if (__builtin_expect(__any_sync(0xffffffffu, !(sum <= 3.4e38f)), 0)) {
-#pragma unroll 1
-            for (int i = 0; i < 8; ++i) {
-                uint4* at = reinterpret_cast<uint4*>(raw + 2048 * p + 256 * i);
-                const unsigned bad = __ballot_sync(0xffffffffu, not_finite(at->x) || not_finite(at->y) || not_finite(at->z) || not_finite(at->w));
-                if (!(__shfl_sync(0xffffffffu, sum, (lane & 16) | (i << 1)) <= 3.4e38f)) *at = make_uint4(0u, 0u, 0u, 0u);
-                if (c == 0 && (bad >> (lane & 16) & 0xffffu)) {
-                    const int t = 16 * p + 2 * i + (lane >> 4);
-                    if (w < 2) atomicMin(&odd.from, 32 * w + t);
-                    else atomicOr(&odd.q[w & 1], 1u << t);
-                }
-            }
-            sum = fminf(sum, __int_as_float(0x7f800000));    // (of NaN: the infinity)
-        }
+        const float sum = fold8(ss, lane);
+        large |= !(sum <= 3.4e38f);
         // the row times 2^-e has a norm in [1, 2)
         int e = (int((__float_as_uint(sum) >> 23) & 255u) - 127) >> 1;
         e = e < -60 ? -60 : e;
         if (!(lane & 1)) {
             const int r = 16 * p + 2 * ((lane >> 1) & 7) + (lane >> 4);
-            rs[32 * (w & 1) + r] = rsqrtf(sum + 1e-6f);
+            rs[r] = rsqrtf(sum + 1e-6f);
             down[32 * w + r] = pow2f(-e);
+        }
+    }
+    // a sum of squares beyond fp32 makes the row zero, as 1 / sqrt(inf) does, and so does an infinity or NaN, which is noted
+    if (__builtin_expect(__any_sync(0xffffffffu, large), 0)) {
+        __syncwarp();                                        // (rs is another lane's)
+#pragma unroll 1
+        for (int i = 0; i < 16; ++i) {
+            const int r = 2 * i + (lane >> 4);
+            uint4* at = reinterpret_cast<uint4*>(raw + 256 * i);
+            const unsigned bad = __ballot_sync(0xffffffffu, not_finite(at->x) || not_finite(at->y) || not_finite(at->z) || not_finite(at->w));
+            const bool zero = !(rs[r] > 0.f);
+            __syncwarp();
+            if (zero) *at = make_uint4(0u, 0u, 0u, 0u);
+            if (zero && c == 0) {
+                rs[r] = 0.f;
+                if (bad >> (lane & 16) & 0xffffu) {
+                    if (w < 2) atomicMin(&odd.from, 32 * w + r);
+                    else atomicOr(&odd.q[w & 1], 1u << r);
+                }
+            }
         }
     }
 }
@@ -600,7 +605,7 @@ __device__ __forceinline__ void ck_prep(ChunkSmem& s, const RuleParams& P, const
             q.c3[tk] = decay_between(Gc, G) * kr * MAT_DOWN;
             if (tk == 0) {
                 q.decay = ex2(Gc.x + Gc.y);
-                q.len = n;
+                q.len = n | odd.from << 8 | ((odd.q[0] | odd.q[1]) != 0) << 16;
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&s.tile_full[grp]);
@@ -679,8 +684,8 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
 #pragma unroll
             for (int g = 0; g < 8; ++g) va += bf16_to_f(s.vsum[g][v]);
             va *= 1.125f;                                    // (sums in bf16: not below the true one, of |v| / 256)
-            int from = CT;
             if (__builtin_expect(!(va < 3.4e38f), 0)) {      // some were not finite: when the first, and the sum of the others
+                int from = CT;
                 va = 0.f;
                 const unsigned char* all = s.v + (v >> 6) * 8192 + 2 * (v & 7);
 #pragma unroll 1
@@ -689,8 +694,8 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
                     if ((g & 0x7f80u) == 0x7f80u && int(g & 7u) == t >> 3) from = min(from, t);
                     va += (1.f / 256) * fabsf(bf16_to_f(*reinterpret_cast<const uint16_t*>(all + t * 128 + ((vc ^ (t & 7)) << 4))));
                 }
+                s.vfrom[tid] = uint8_t(from);
             }
-            s.vfrom[buf][tid] = uint8_t(from);
         }
         if (c > 0) {                                         // the state behind the chunk before
             ck_wait(patience, &s.d_full, uint32_t(c - 1) & 1u);
@@ -838,12 +843,13 @@ __device__ __forceinline__ void ck_main(ChunkSmem& s, const RuleParams& P, int h
             }
             tmem_st_8(row + slo + 2 * TP * h + 8 * p, x);
         }
-        {
-            const ChunkOdd& odd = s.odd[c & (ODD_RING - 1)];
-            const int from = min(int(s.vfrom[buf][tid]), odd.from);
-            decay = from < CT ? __int_as_float(0x7fffffff) : q.decay;
-            plen = q.len | from << 8 | ((odd.q[0] | odd.q[1]) ? 1 << 16 : 0);
+        decay = q.decay;
+        plen = q.len;
+        if (__builtin_expect(s.vfrom[tid] != CT, 0)) {
+            plen = min(int(s.vfrom[tid]), plen >> 8 & 255) << 8 | (plen & ~0xff00);
+            s.vfrom[tid] = CT;
         }
+        if ((plen >> 8 & 255) != CT) decay = __int_as_float(0x7fffffff);
         of = P.scale * pow2f(-e) * MAT_DOWN;
         ck_wait(patience, &s.y_full, uint32_t(c) & 1u);
         tc_fence_after_sync();
@@ -1155,6 +1161,7 @@ __global__ void __launch_bounds__(CK_THREADS, 1) rule_chunk_kernel(RuleParams P,
                                                                                     // blocks of T (head, remainder) stay zero
 #pragma unroll 1
     for (int i = tid; i < 2 * 2 * 32 * 36; i += CK_THREADS) (&s.prep[i / (2 * 32 * 36)].tt[0][0][0])[i % (2 * 32 * 36)] = 0.f;
+    if (tid < CK_MAIN) s.vfrom[tid] = CT;
     if (tid < ODD_RING) {
         s.odd[tid].from = CT;
         s.odd[tid].q[0] = s.odd[tid].q[1] = 0;
