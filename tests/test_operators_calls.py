@@ -143,3 +143,30 @@ def test_the_check_of_a_prefill_answers_like_the_call():
         o = v.pop("o")
         assert L.lq_gdn_prefill(d, *v.values(), None, o, N, T, 0.0, None, 0, None) == rc, kw
     assert L.lq_gdn_prefill_check(None, *base.values()) == -1
+
+
+@gpu
+def test_a_layers_norms_and_residual():
+    """Rule -> gated norm -> scaled residual norm of one prompt: every output of the last two and the residual stream, against 64 bits on
+    the bf16 rows that each of them reads (the tolerances of the operators by themselves: half a bf16 step of 2^-8, and 2^-19 of the
+    terms that cancel; one fp32 rounding of |h| < 16 for the stream)."""
+    from leapquant_b200.kernels import make_add_norm, make_gated_norm
+    st, ssm, mixed, a, b, A_log, dt_bias = layer(54)
+    T, D = mixed.shape[0], 4 * V
+    g = torch.Generator().manual_seed(4)
+    z = torch.randn(T, D + 128, generator=g).bfloat16().cuda()[:, 128:]
+    gw, nw = (1 + 0.1 * torch.randn(V, generator=g)).bfloat16().cuda(), (1 + 0.1 * torch.randn(D, generator=g)).bfloat16().cuda()
+    res = torch.randn(T, D, generator=g).bfloat16().cuda()
+    before = res.double()
+    o = torch.zeros(T, 4, V, dtype=torch.bfloat16, device="cuda")
+    y, out = torch.empty_like(o), torch.empty(T, D, dtype=torch.bfloat16, device="cuda")
+    st.prefill(ssm, mixed, a, b, A_log.float(), dt_bias.float(), torch.tensor([1, 2], dtype=torch.int32, device="cuda"), offsets([60, 10]).cuda(), o)
+    make_gated_norm(V)(o, z, gw, y)
+    make_add_norm(D, scale=0.5)(y.view(T, D), res, nw, out)
+    od, zd = o.double(), z.double().reshape(T, 4, V)
+    y64 = od / torch.sqrt((od * od).mean(-1, keepdim=True) + 1e-6) * gw.double() * zd * torch.sigmoid(zd)
+    assert float(((y.double() - y64).abs() - 2.0 ** -8 * y64.abs()).max()) <= 2.0 ** -19 * float(y64.abs().max())
+    h = before + 0.5 * y.double().view(T, D)
+    assert float(((res.double() - h).abs() - 2.0 ** -8 * h.abs()).max()) <= 2.0 ** -21
+    out64 = h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6) * nw.double()
+    assert float(((out.double() - out64).abs() - 2.0 ** -8 * out64.abs()).max()) <= 2.0 ** -19 * float(out64.abs().max())

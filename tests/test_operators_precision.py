@@ -31,3 +31,18 @@ def test_outputs_are_rounded_once(H, HV, lens, impl):
     assert float(off.max()) <= 0, float(off.max())
     check_rule(S, S64, o, o64, (size, largest), max(lens))
     clean()
+
+
+@gpu
+def test_more_heads_than_sms():
+    """Chunked heads in more than one wave (seven sequences of 32 heads, 224 CTAs for 148 SMs) at an ordinary layer's head counts,
+    short sequences between them."""
+    lens = [70, 3, 131, 64, 29, 100, 65, 90, 12]
+    n = len(lens)
+    S, S64, o, o64, (size, largest) = run_rule(16, 32, lens, list(range(n, 0, -1)), n + 1, seed=77, fresh=[i % 3 == 0 for i in range(n)])
+    T = sum(lens)
+    off = (o.double() - o64).abs()[:T] - half_step(o64[:T]) - 2.0 ** -15 * size[:T] - 2.0 ** -31 * largest
+    assert float(off.max()) <= 0, float(off.max())
+    check_rule(S, S64, o, o64, (size, largest), max(lens))
+    assert bool((o[T:] == 7.0).all())
+    clean()
