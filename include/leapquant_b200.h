@@ -225,7 +225,7 @@ int lq_lowrank(const float* x, const float* Q0, float* U, float* Q, int32_t n, i
  * fp32 products carry 22 bits and what falls below 2^-38 of |S row| + sum |v row| of the chunk, as behind a decay of that much, is lost.
  * Infinities and NaN reach what depends on them as values that are not finite, and nothing before their token: of q its token's outputs, of
  * k, a and b the head from there on, of v and of a state's row that value dimension from there on.  |q|^2 and |k|^2 are fp32 sums: a row
- * whose sum overflows counts as zeros.
+ * whose sum overflows counts as zeros.  Token by token the product of a state's row with the key as it is has to stay within fp32, too.
  *   - mixed bf16 rows q | k | v (2 H K + HV V elements, row stride mixed_stride, a multiple of 8); a, b bf16 [T, HV] with row strides;
  *     A_log, dt_bias f32 [HV]; cu i32 [N + 1], ascending; idx i32 [N]; o bf16 [T, HV, V] contiguous.  scale <= 0 selects K^-1/2.
  *   - has_initial (u8 [N], may be NULL = all): 0 starts the sequence from a zero state instead of its slot's.
@@ -250,18 +250,21 @@ int lq_gdn_recurrent(const lq_dims* d, float* ssm, const void* mixed, int64_t mi
 /* Causal conv1d + SiLU of packed prompts: per sequence and channel, with the inputs before the sequence's first token from its slot
  * (zeros where has_initial[n] is 0),  out[t] = silu(bias + sum_j weight[j] in[t - 3 + j])  in fp32, rounded once; the slot's state
  * becomes the last three inputs.  conv: the operands of lq_causal_conv1d_update, x with T rows; cu, idx, has_initial as above;
- * out bf16 [T, out_stride], not overlapping x (LQ_ERR_RANGE; columns of one buffer next to one another are fine).  Sequences without tokens or with a padding slot are skipped (nothing read or
- * written).  channels must be a multiple of 8 and bias 16-byte aligned. */
+ * out bf16 [T, out_stride], not overlapping x (LQ_ERR_RANGE; columns of one buffer next to one another are fine).  Sequences without tokens
+ * or with a padding slot are skipped (nothing read or written).  channels must be a multiple of 8 and bias 16-byte aligned.
+ * lq_causal_conv1d_update rounds every tap's product to bf16, as the engine's kernel does; the same tokens one by one therefore differ
+ * from a prompt's by those roundings. */
 int lq_causal_conv1d_prompt(const lq_conv1d* conv, const int32_t* cu, const int32_t* idx, const uint8_t* has_initial, int32_t N,
                             int64_t T, int32_t channels, int32_t NS, void* out, int64_t out_stride, void* stream);
 /* Gated RMS norm of the rule's output: y = o / sqrt(mean(o^2) + eps) * weight * silu(z) over every head's V = 128 values, in fp32,
- * rounded once.  o, y bf16 [T, HV, V] contiguous (y may be o, and overlaps
- * nothing else: LQ_ERR_RANGE); z bf16 [T, HV * V] with row stride z_stride; weight bf16 [V]. */
+ * rounded once.  o, y bf16 [T, HV, V] contiguous (y may be o, and overlaps nothing else: LQ_ERR_RANGE); z bf16 [T, HV * V] with row stride
+ * z_stride; weight bf16 [V].  The sum of squares is fp32: a row in which it overflows (values beyond 1.6e18) comes out as zeros. */
 int lq_gated_norm(const void* o, const void* z, int64_t z_stride, const void* weight, void* y, int64_t T, int32_t HV, int32_t V,
                   float eps, void* stream);
 /* Residual and RMS norm: h = residual + scale x (fp32);  residual <- bf16(h);  y = h / sqrt(mean(h^2) + eps) * weight.
  * All bf16 [T, D] with row strides in elements (multiples of 8); weight bf16 [D]; D a multiple of 8 up to LQ_NORM_MAX_DIM.
- * y may be x, x may be residual; any other overlap is LQ_ERR_RANGE. */
+ * y may be x, x may be residual; any other overlap is LQ_ERR_RANGE.  weight multiplies as it is (a layer that keeps its weight as w - 1 adds
+ * the 1 itself).  The sum of squares is fp32, as in lq_gated_norm. */
 #define LQ_NORM_MAX_DIM 16384
 int lq_add_norm(const void* x, int64_t x_stride, void* residual, int64_t r_stride, const void* weight, void* y, int64_t y_stride,
                 int64_t T, int32_t D, float scale, float eps, void* stream);

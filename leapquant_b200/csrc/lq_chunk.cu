@@ -14,18 +14,20 @@
 //     prep warps   two groups of four, a chunk each in turn, ahead of the main warps: norms, f16 rows of k and q in shared memory
 //                  (B operand), K K^T and Q K^T, decays, T and A; rows of k and q by TMA
 //
-// What bounds it.  One sequence is a chain of chunks, and a chunk of one head is what one SM does at a time: 4.4 us (8 000 cycles), of
-// which the main chain, six hand-overs between registers, tensor memory and tensor cores, takes 6 900 by itself.  The two prep groups
-// need 16 000 for their two chunks, side by side with it.  Both are made of the same issue slots: 19 600 warp instructions a chunk, 0.5 an
-// SM quarter's cycle.  FMA pipe 30 %, ALU 24 %, tensor pipe 24 % busy: a warp waits for tensor memory, barriers and its own results.  The
-// loops are kept small, since an SM's instruction cache holds 32 KB (they have 46; when they were twice as long, fetching was the first stall).
-//     one sequence of 8 192 tokens, 32 heads      570 us on 32 SMs, 430 split over 96
-//     16 sequences of 4 096 tokens, 32 heads    1 200 us on all, 512 heads on 148 SMs
+// What bounds it.  One sequence is a chain of chunks, and a chunk of one head is what one SM does at a time: 4.7 us, most of it the main
+// chain, six hand-overs between registers, tensor memory and tensor cores; the two prep groups take about as long for a chunk, side by
+// side with it.  Both are made of the same issue slots: 21 200 warp instructions a chunk, 0.51 an SM quarter's cycle.  FMA pipe 31 %, ALU 24 %,
+// tensor pipe 27 % busy: a warp waits for tensor memory, barriers and its own results.  The loops are kept small, since an SM's
+// instruction cache holds 32 KB (they are larger; when they were twice as long, fetching was the first stall), and what is seldom needed
+// stands behind them.
+//     one sequence of 8 192 tokens, 32 heads      600 us on 32 SMs, 447 split over 96
+//     16 sequences of 4 096 tokens, 32 heads    1 269 us on all, 512 heads on 148 SMs
 // On the way, one sequence of 8 192 tokens, not split: token by token 6 750 us; in chunks with one prep group 1 920; two groups, values and outputs
 // through shared memory, instructions issued by a whole warp 810; the inverse on tensor cores, one scale per row 620; rows and outputs by
-// TMA 570.  16 sequences of 4 096: loops instead of straight code and outputs accumulated in tensor memory 1 330 -> 1 170 us.  Without gain:
-// sixteen main warps with a quarter of a row each, two accumulators for S k, loops rolled up to 38 KB (spills: 684 us), hints to
-// sleeping waits.
+// TMA 570.  16 sequences of 4 096: loops instead of straight code and outputs accumulated in tensor memory 1 330 -> 1 170 us; roles and starts
+// of the segments in the same kernel 1 207; outputs from two pieces 1 244 (1 263 with A u ahead of the state's products); the whole range of
+// states and values, infinities and NaN 1 269.  Without gain: sixteen main warps with a quarter of a row each, two accumulators for S k,
+// loops rolled up to 38 KB (spills: 684 us), hints to sleeping waits.
 //
 // Precision.  k and q are bf16 and become f16 without loss once a row is scaled by a power of two (what is lost lies 2^-25 below the
 // row's norm); an fp32 operand is the sum of two f16 pieces, 22 bits.  f16 has few exponents, so every row of S, r and u carries
@@ -41,16 +43,20 @@
 
 namespace lq {
 
-// Sequences of fewer tokens are run token by token, longer ones in chunks.  A chunk costs a CTA 20 us however many tokens it has, the
+// Sequences of fewer tokens are run token by token, longer ones in chunks.  A chunk costs a CTA 19 us however many tokens it has, the
 // recurrence 8.6 us a token of 64 sequences of 32 heads and 0.45 us of one sequence, which leaves most of the device idle either way:
 //     tokens                          24          28          32          40
-//     64 sequences, 32 heads      212 : 281   248 : 283   283 : 284   353 : 284   us, token by token : in chunks
-//      8 sequences, 32 heads       35 :  39    40 :  39    45 :  39    55 :  39
-//      one sequence, 32 heads      14 :  20    16 :  20    19 :  20    21 :  20
+//     64 sequences, 32 heads      212 : 279   248 : 280   282 : 282   352 : 281   us, token by token : in chunks
+//      8 sequences, 32 heads       34 :  38    39 :  38    44 :  39    54 :  38
+//      one sequence, 32 heads      13 :  19    14 :  19    16 :  19    20 :  19
 constexpr int RULE_SHORT = 28;
 // A batch of few heads whose sequences are long on average ends with its longest one, and SMs are idle by then: short sequences cost nothing
-// in the chunked launch, but 0.45 us a token ahead of it.  37 sequences of 1 to 2 969 tokens (mean 467) of 8 heads 255 us with 28, 236 with 8;
-// 60 of the kind of 32 heads, which fill the SMs to the end, 527 and 543.
+// in the chunked launch, but 0.45 us a token ahead of it.  Time with 8 against 28, lengths from 1 on evenly over their logarithm:
+//     sequences x heads, per SM  0.6            1.3            2.0            2.6            2.9 .. 3.2     5.2 .. 5.4     8 .. 13        22
+//     mean length 50 .. 130      0.87           0.92           0.73 .. 0.79   0.84           0.82 .. 0.91   0.97 .. 1.01   0.99 .. 1.12   1.06
+//     mean length 150 .. 1 060   0.91 .. 0.97   0.81 .. 0.96   0.89 .. 0.97   0.91 .. 0.95   0.86 .. 0.99   0.93 .. 1.00   0.99 .. 1.06   1.02 .. 1.04
+// It is used up to three heads an SM and from a mean of 256 tokens on: below that a batch may be drafts and single tokens, which the
+// recurrence is for.  (8 heads and 32, 12 to 100 sequences.)
 constexpr int RULE_SHORT_AMONG_LONG = 8;
 constexpr int RANKED = 128;                                  // batches up to which CTAs take the longest sequences first
 constexpr int CT = 64;                                       // tokens of a chunk
@@ -1009,8 +1015,8 @@ __device__ __forceinline__ int ck_sequence(ChunkSmem& s, const RuleParams& P, in
 //     pass 2   the segments 1 .. from their states
 // Every segment but the first and the last is run three times, but the chain is two segments long, with 30 us for two more launches and
 // 2.5 us a join.  One sequence, whole -> in segments:
-//     8 192 tokens  32 heads 570 -> 430 us (3 segments), 16 heads 249 (6), 8 heads 165 (10), 4 heads 138 (16; 8 segments 186)
-//     2 048 tokens  32 heads 158 -> 141 us,              16 heads 103,     8 heads 82,       4 heads 80
+//     8 192 tokens  32 heads 600 -> 447 us (3 segments), 16 heads 262 (6), 8 heads 173 (10), 4 heads 140 (16)
+//     2 048 tokens  32 heads 160 -> 148 us,              16 heads 108,     8 heads 84,       4 heads 81
 struct Segments {
     float* work;                                             // of this sequence and head
     int64_t tokens;                                          // of a segment but the last: whole chunks
@@ -1258,7 +1264,7 @@ static int launch_chunk(const RuleParams& P, cudaStream_t st) {
     return finish_launch();
 }
 // Segments that sequences are split into, 0 if that would not be faster: both passes have to fit the SMs at once, and a sequence of mean
-// length has to save more by its shorter chain (4.4 us a chunk) than the launches and the joins cost.  (At the least 16 chunks in four segments
+// length has to save more by its shorter chain (4.7 us a chunk) than the launches and the joins cost.  (At the least 16 chunks in four segments
 // of four.)
 static int rule_segs(int64_t N, int64_t HV, int64_t T) {
     const int64_t chunks = T / N / CT, fit = (device_sm_count() / (N * HV) + 3) / 2;

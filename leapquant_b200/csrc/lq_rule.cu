@@ -5,7 +5,8 @@
 //     g_t = -exp(A_log) softplus(a_t + dt_bias),  beta_t = sigmoid(b_t)
 //     q^_t = q_t scale / sqrt(|q_t|^2 + 1e-6),  k^_t = k_t / sqrt(|k_t|^2 + 1e-6)
 //     S <- e^{g_t} S;   u_t = beta_t (v_t - S k^_t);   S <- S + u_t k^_t^T;   o_t = S q^_t
-// States, gates, norms and sums are fp32 (sums of gates fp64); outputs are rounded to bf16 once.
+// States, gates, norms and sums are fp32 (in chunks: sums of gates fp64, factors of fp32 products two f16 pieces, 22 bits); outputs are rounded
+// to bf16 once.
 #include "lq_common.cuh"
 
 namespace lq {

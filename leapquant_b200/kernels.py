@@ -272,7 +272,8 @@ def make_gdn_prefill(NS, HV, H, K, V, SS, scale=None):
     mixed bf16 [T, 2HK + HV V] and a, b bf16 [T, HV] (row strides free); A_log, dt_bias f32 [HV]; cu i32 [N + 1], the first row of
     every sequence and the end of the last; idx i32 [N], their slots; has_initial bool [N] or None (all): False starts from a zero
     state; o bf16 [T, HV, V].  A sequence without tokens touches nothing; one with idx <= 0, idx >= NS or a slot that an earlier
-    one names gets zeros in o and touches no state; rows of o that no sequence owns are left as they are.  Long sequences of few
+    one names gets zeros in o and touches no state; rows of o that no sequence owns are left as they are.  The state after the last token
+    is what remains: drafts that may be rejected need a copy of the state, or a call per token.  Long sequences of few
     heads are split over the SMs, for which the call takes scratch from torch's allocator (a few MB).
     prefill.check takes the same operands and only refuses what prefill would refuse."""
     _need_128(K, V, "make_gdn_prefill")
@@ -325,7 +326,8 @@ def make_conv1d_prompt(NS, channels):
     """Causal conv1d (width 4) + SiLU of packed prompts.  Returns prompt(x, conv_state, conv_weight, conv_bias, cu, idx, has_initial, out):
     x bf16 [T, >= channels], conv_state, conv_weight, conv_bias as for make_conv1d_update, cu, idx, has_initial as for
     make_gdn_prefill, out bf16 [T, channels] (not overlapping x).  conv_state receives the last three inputs of every sequence.
-    The sums are fp32 and rounded once, without the update's rounding of every tap's product.  Sequences without tokens, and those
+    The sums are fp32 and rounded once, without the update's rounding of every tap's product (so the same tokens one by one give other
+    roundings).  Sequences without tokens, and those
     with idx <= 0, idx >= NS or the slot of an earlier one, are skipped (nothing read or written)."""
     fn = _lib.lib().lq_causal_conv1d_prompt
 
@@ -371,7 +373,7 @@ def make_gated_norm(V, eps=1e-6):
 def make_add_norm(D, eps=1e-6, scale=1.0):
     """Residual stream and the norm that the next block reads.  Returns norm(x, residual, weight, y): residual <- residual + scale x;
     y = residual / sqrt(mean(residual^2) + eps) * weight, of the fp32 sum.  x, residual, y bf16 [T, D] (row strides free; y may be
-    x, but overlaps neither otherwise), weight bf16 [D]."""
+    x, but overlaps neither otherwise), weight bf16 [D], which multiplies as it is: a layer that keeps w - 1 adds the 1 itself."""
     if D < 8 or D % 8 or D > 16384:
         raise NotImplementedError(f"make_add_norm: D = {D}; a multiple of 8 up to 16384 is supported")
     eps, scale = float(eps), float(scale)
