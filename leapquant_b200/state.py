@@ -119,6 +119,11 @@ class LeapQuantState:
         in fp32 saves the launch."""
         return t.detach().to(torch.float32).contiguous()
 
+    @staticmethod
+    def _i32(t):
+        """Slots or offsets as the kernels read them: dense int32 (t itself, where it is)."""
+        return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
+
     def views(self, ssm):
         k = _ident(ssm)
         if self._vkey != k:
@@ -207,8 +212,8 @@ class LeapQuantState:
         Gated DeltaNet only.  No host synchronisation; scratch from torch's allocator where long sequences of few heads are split."""
         self._need_gdn("prefill")
         self.kprefill(ssm, mixed, a, b, A_log if A_log.dtype == torch.float32 else self._p32(A_log),
-                      dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), cu_seqlens.to(torch.int32), idx.to(torch.int32),
-                      has_initial, out)
+                      dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), self._i32(cu_seqlens), self._i32(idx),
+                      None if has_initial is None else has_initial.contiguous(), out)
 
     def prefill_conv(self, ssm, x, conv_state, conv_weight, conv_bias, a, b, A_log, dt_bias, idx, cu_seqlens, out, has_initial=None):
         """prefill() from the raw q | k | v projections x: the causal conv1d of the prompts first (operands as for decode_conv; the
@@ -220,7 +225,8 @@ class LeapQuantState:
         if self._kconv_prompt is None:
             self._kconv_prompt = KN.make_conv1d_prompt(self.NS, C)
         mixed = torch.empty(x.shape[0], C, dtype=torch.bfloat16, device=x.device)
-        idx, cu_seqlens = idx.to(torch.int32), cu_seqlens.to(torch.int32)
+        idx, cu_seqlens = self._i32(idx), self._i32(cu_seqlens)
+        has_initial = None if has_initial is None else has_initial.contiguous()
         A_log = A_log if A_log.dtype == torch.float32 else self._p32(A_log)
         dt_bias = dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias)
         # the conv advances its state in place: what the rule would refuse is refused before it
@@ -233,7 +239,7 @@ class LeapQuantState:
         the other side of a comparison).  Operands as for decode(), a and b with free row strides.  Gated DeltaNet only."""
         self._need_gdn("decode_dense")
         self.kdense(ssm, mixed, a, b, A_log if A_log.dtype == torch.float32 else self._p32(A_log),
-                    dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), idx.to(torch.int32), out)
+                    dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias), self._i32(idx), out)
 
     def dequantize(self, ssm, idx):
         """Materialize the fp32 state of the slots idx in place (before the engine's own prefill kernel runs on them)."""

@@ -170,3 +170,42 @@ def test_a_layers_norms_and_residual():
     assert float(((res.double() - h).abs() - 2.0 ** -8 * h.abs()).max()) <= 2.0 ** -21
     out64 = h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6) * nw.double()
     assert float(((out.double() - out64).abs() - 2.0 ** -8 * out64.abs()).max()) <= 2.0 ** -19 * float(out64.abs().max())
+
+
+@gpu
+def test_slots_and_offsets_in_other_layouts():
+    """Slots, offsets and flags as columns of a scheduler's table and in 64 bits, as dequantize() and quantize() take slots: the same bits as
+    from dense int32 tensors."""
+    st, ssm, mixed, a, b, A_log, dt_bias = layer(55)
+    A_log, dt_bias = A_log.float(), dt_bias.float()
+    T, C = mixed.shape
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    idx, cu, hi = torch.tensor([2, 1], device="cuda"), offsets([60, 10]).cuda().long(), torch.tensor([True, False], device="cuda")
+    table = lambda t: torch.stack([t, torch.zeros_like(t)], 1)[:, 0]
+    got = []
+    for i, c, h in ((idx.int(), cu.int(), hi), (idx, cu, hi), (table(idx.int()), table(cu.int()), table(hi)), (table(idx), table(cu), hi)):
+        S, conv = ssm.clone(), torch.ones(3, 3, C, dtype=torch.bfloat16, device="cuda")
+        o, o1, o2 = torch.zeros(T, 4, V, dtype=torch.bfloat16, device="cuda"), torch.zeros(T, 4, V, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 4, V, dtype=torch.bfloat16, device="cuda")
+        st.prefill_conv(S, mixed, conv.transpose(1, 2), w, None, a, b, A_log, dt_bias, i, c, o, h)
+        st.prefill(S, mixed, a, b, A_log, dt_bias, i, c, o1, h)
+        st.decode_dense(S, mixed[:2], a[:2], b[:2], A_log, dt_bias, i, o2)
+        got.append((S, conv, o, o1, o2))
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(other, got[0]))
+
+
+@gpu
+def test_calls_without_tokens_or_sequences():
+    st, ssm, mixed, a, b, A_log, dt_bias = layer(56)
+    A_log, dt_bias = A_log.float(), dt_bias.float()
+    C = mixed.shape[1]
+    w, conv, before = torch.ones(C, 4, dtype=torch.bfloat16, device="cuda"), torch.ones(3, 3, C, dtype=torch.bfloat16, device="cuda"), ssm.clone()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for T, cu, idx in ((0, i32(0, 0, 0), i32(1, 2)), (0, i32(0), i32()), (5, i32(0), i32()), (5, i32(3, 3), i32(1))):
+        o = torch.full((T, 4, V), 7.0, dtype=torch.bfloat16, device="cuda")
+        st.prefill(ssm, mixed[:T], a[:T], b[:T], A_log, dt_bias, idx, cu, o)
+        st.prefill_conv(ssm, mixed[:T], conv.transpose(1, 2), w, None, a[:T], b[:T], A_log, dt_bias, idx, cu, o)
+        assert bool((o == 7.0).all())
+    st.decode_dense(ssm, mixed[:0], a[:0], b[:0], A_log, dt_bias, i32(), torch.empty(0, 4, V, dtype=torch.bfloat16, device="cuda"))
+    torch.cuda.synchronize()
+    assert torch.equal(ssm, before) and bool((conv == 1).all())

@@ -120,3 +120,32 @@ def test_rows_of_nobody(lens, slots, form):
     assert bool(torch.isfinite(got[0][1]).all()) and bool((got[1][1][sum(lens):] == 7.0).all())
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
     clean()
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[1300], [150, 66], [5, 3]], ids=["segments", "long", "short"])
+@pytest.mark.parametrize("form", [0, 1, 2])
+def test_fresh_sequences_on_slots_that_hold_anything(lens, form):
+    """has_initial False: the slot's bits are not read, be they a checkpoint's or NaN; the conv's neither."""
+    from leapquant_b200 import _lib
+    from leapquant_b200.kernels import make_conv1d_prompt, make_gdn_prefill
+    n, T = len(lens), sum(lens)
+    ssm, mixed, a, b, A_log, dt_bias = rule_inputs(H, HV, T, n + 1, 73)
+    C = mixed.shape[1]
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    cu, idx, fresh = offsets(lens).cuda(), torch.arange(1, n + 1, dtype=torch.int32, device="cuda"), torch.zeros(n, dtype=torch.bool, device="cuda")
+    got = []
+    _lib.set_option("rule_impl", form)
+    try:
+        for fill in (0.0, NAN, INF):
+            S, taps = torch.full_like(ssm, fill), torch.full((n + 1, 3, C), fill, dtype=torch.bfloat16, device="cuda")
+            x, o = torch.empty(T, C, dtype=torch.bfloat16, device="cuda"), torch.empty(T, HV, V, dtype=torch.bfloat16, device="cuda")
+            make_conv1d_prompt(n + 1, C)(mixed, taps.transpose(1, 2), w, None, cu, idx, fresh, x)
+            make_gdn_prefill(n + 1, HV, H, K, V, S.stride(0))(S, x, a, b, A_log, dt_bias, cu, idx, fresh, o)
+            got.append((x, o, S[1:], taps[1:]))
+    finally:
+        _lib.set_option("rule_impl", 0)
+    assert all(bool(torch.isfinite(t).all()) for t in got[0])
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(other, got[0]))
+    clean()
