@@ -145,8 +145,7 @@ class LeapQuantState:
             a = a.reshape(a.shape[0], HV, KA).contiguous()
         if not dt_bias.is_contiguous() or dt_bias.numel() != HV * KA:
             dt_bias = dt_bias.reshape(HV, KA).contiguous()
-        if idx.dtype != torch.int32:
-            idx = idx.to(torch.int32)
+        idx = self._i32(idx)
         if self.fused:
             if ssm.dim() != 4:
                 raise ValueError(f"the state tensor is [slots, heads, V, K], got {tuple(ssm.shape)}")
@@ -186,7 +185,7 @@ class LeapQuantState:
                     self._mixed_old.append(self._mixed)
                 self._mixed = torch.empty(max(64, 1 << (N - 1).bit_length()), C, dtype=torch.bfloat16, device=x.device)
             mixed = self._mixed if self._mixed.shape[0] == N else self._mixed[:N]
-            i32 = idx if idx.dtype == torch.int32 else idx.to(torch.int32)
+            i32 = self._i32(idx)
             self._kconv(x, conv_state, conv_weight, conv_bias, i32, mixed)
             return self.decode(ssm, mixed, a, b, A_log, dt_bias, i32, out)
         A_log = A_log if A_log.dtype == torch.float32 else self._p32(A_log)
@@ -194,7 +193,7 @@ class LeapQuantState:
         KA = self.K if self.kda else 1
         a = a.reshape(a.shape[0], self.HV, KA).contiguous()
         dt_bias = dt_bias.reshape(self.HV, KA).contiguous()
-        idx = idx if idx.dtype == torch.int32 else idx.to(torch.int32)
+        idx = self._i32(idx)
         v = self.views(ssm)
         bufs = (self.Kbuf, self.Ubuf, self.Wbuf, self.Pbuf) + ((self.Gbuf,) if self.kda else ()) + (self.hcnt,)
         self.kdecode_conv(v["q32"], *bufs, x, conv_state, conv_weight, conv_bias, a, b, A_log, dt_bias, self.Q0, idx, out, self.work)

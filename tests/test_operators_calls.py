@@ -209,3 +209,28 @@ def test_calls_without_tokens_or_sequences():
     st.decode_dense(ssm, mixed[:0], a[:0], b[:0], A_log, dt_bias, i32(), torch.empty(0, 4, V, dtype=torch.bfloat16, device="cuda"))
     torch.cuda.synchronize()
     assert torch.equal(ssm, before) and bool((conv == 1).all())
+
+
+@gpu
+@pytest.mark.parametrize("how", ["fused", "step_flush", "conv", "conv_one_launch"])
+def test_decode_takes_slots_in_any_layout(how):
+    """A column of a table of slots names the slots in it, not the numbers that lie next to one another in memory."""
+    st, ssm, mixed, a, b, A_log, dt_bias = layer(57, N=4)
+    A_log, dt_bias = A_log.float(), dt_bias.float()
+    C = mixed.shape[1]
+    w = torch.randn(C, 4, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    idx = torch.tensor([3, 1], dtype=torch.int32, device="cuda")
+    table = torch.stack([idx, torch.tensor([2, 4], dtype=torch.int32, device="cuda")], 1)[:, 0]
+    every = torch.arange(1, 5, dtype=torch.int32, device="cuda")
+    st.fused, st.conv_one_launch = how != "step_flush", how == "conv_one_launch"
+    got = []
+    for i in (idx, table):
+        S, conv, o = ssm.clone(), torch.ones(5, 3, C, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 4, V, dtype=torch.bfloat16, device="cuda")
+        st.quantize(S, every)
+        x, ga, gb = mixed[:2].contiguous(), a[:2].contiguous(), b[:2].contiguous()
+        if how.startswith("conv"):
+            st.decode_conv(S, x, conv.transpose(1, 2), w, None, ga, gb, A_log, dt_bias, i, o)
+        else:
+            st.decode(S, x, ga, gb, A_log, dt_bias, i, o)
+        got.append((o, conv, S.view(torch.int32), st.hcnt.clone()))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
