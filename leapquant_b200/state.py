@@ -141,6 +141,12 @@ class LeapQuantState:
             dt_bias = self._p32(dt_bias)
         # the kernels take addresses: a tensor that is contiguous and has the right number of elements is passed as it is
         HV, KA = self.HV, self.K if self.kda else 1
+        if not out.is_contiguous():
+            raise ValueError(f"decode writes dense outputs, got strides {out.stride()}")
+        if not mixed.is_contiguous():
+            mixed = mixed.contiguous()
+        if not b.is_contiguous():
+            b = b.contiguous()
         if not a.is_contiguous() or a.numel() != a.shape[0] * HV * KA:
             a = a.reshape(a.shape[0], HV, KA).contiguous()
         if not dt_bias.is_contiguous() or dt_bias.numel() != HV * KA:
@@ -174,6 +180,8 @@ class LeapQuantState:
         bf16 [channels, 4], conv_bias bf16 [channels] or None.  Two launches of this library (update kernel, decode), or, with
         conv_one_launch, one, in which the activated q | k | v row is never written to memory; the results are the same bit for
         bit.  No counterpart in the reference, whose plugin calls vLLM's causal_conv1d_update first."""
+        if not out.is_contiguous():                          # (before the conv state is advanced)
+            raise ValueError(f"decode writes dense outputs, got strides {out.stride()}")
         if not self.conv_one_launch:
             C = 2 * self.H * self.K + self.HV * self.V
             N = x.shape[0]
@@ -191,7 +199,7 @@ class LeapQuantState:
         A_log = A_log if A_log.dtype == torch.float32 else self._p32(A_log)
         dt_bias = dt_bias if dt_bias.dtype == torch.float32 else self._p32(dt_bias)
         KA = self.K if self.kda else 1
-        a = a.reshape(a.shape[0], self.HV, KA).contiguous()
+        a, b = a.reshape(a.shape[0], self.HV, KA).contiguous(), b.contiguous()
         dt_bias = dt_bias.reshape(self.HV, KA).contiguous()
         idx = self._i32(idx)
         v = self.views(ssm)

@@ -234,3 +234,34 @@ def test_decode_takes_slots_in_any_layout(how):
             st.decode(S, x, ga, gb, A_log, dt_bias, i, o)
         got.append((o, conv, S.view(torch.int32), st.hcnt.clone()))
     assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+@gpu
+@pytest.mark.parametrize("kda", [False, True], ids=["gdn", "kda"])
+@pytest.mark.parametrize("how", ["fused", "step_flush", "conv", "conv_one_launch"])
+def test_decode_takes_rows_where_the_projections_left_them(how, kda):
+    """q | k | v rows, a and b as slices of wider projections: the same bits as from dense tensors.  Outputs have to be dense."""
+    from leapquant_b200.state import LeapQuantState
+    H, HV, N = 2, 4, 3
+    C, A = 2 * H * K + HV * V, HV * (K if kda else 1)
+    ssm, mixed, _, _, A_log, dt_bias = rule_inputs(H, HV, N, N + 1, 58)
+    dt_bias = dt_bias.repeat_interleave(K) if kda else dt_bias
+    st = LeapQuantState(ssm, H, kda=kda)
+    g = torch.Generator().manual_seed(5)
+    wide = torch.randn(N, C + 64 + A + HV + (-(A + HV)) % 8, generator=g).bfloat16().cuda()       # (rows start on 16 bytes)
+    w = torch.randn(C, 4, generator=g).bfloat16().cuda()
+    idx = torch.tensor([3, 1, 2], dtype=torch.int32, device="cuda")
+    st.fused, st.conv_one_launch = how != "step_flush", how == "conv_one_launch"
+    rows, a, b = wide[:, :C], wide[:, C + 64:C + 64 + A], wide[:, C + 64 + A:C + 64 + A + HV]
+    got = []
+    for x, ga, gb in ((rows.contiguous(), a.contiguous(), b.contiguous()), (rows, a, b)):
+        S, conv, o = ssm.clone(), torch.ones(N + 1, 3, C, dtype=torch.bfloat16, device="cuda"), torch.zeros(N, HV, V, dtype=torch.bfloat16, device="cuda")
+        st.quantize(S, torch.arange(1, N + 1, dtype=torch.int32, device="cuda"))
+        if how.startswith("conv"):
+            st.decode_conv(S, x, conv.transpose(1, 2), w, None, ga, gb, A_log, dt_bias, idx, o)
+        else:
+            st.decode(S, x, ga, gb, A_log, dt_bias, idx, o)
+        got.append((o, conv, S.view(torch.int32), st.hcnt.clone()))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    with pytest.raises(ValueError):
+        st.decode(S, rows, a, b, A_log, dt_bias, idx, torch.zeros(N, HV, 2 * V, dtype=torch.bfloat16, device="cuda")[:, :, :V])
