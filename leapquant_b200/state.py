@@ -180,7 +180,7 @@ class LeapQuantState:
         bf16 [channels, 4], conv_bias bf16 [channels] or None.  Two launches of this library (update kernel, decode), or, with
         conv_one_launch, one, in which the activated q | k | v row is never written to memory; the results are the same bit for
         bit.  No counterpart in the reference, whose plugin calls vLLM's causal_conv1d_update first."""
-        if not out.is_contiguous():                          # (before the conv state is advanced)
+        if out is not None and not out.is_contiguous():      # (before the conv state is advanced)
             raise ValueError(f"decode writes dense outputs, got strides {out.stride()}")
         if not self.conv_one_launch:
             C = 2 * self.H * self.K + self.HV * self.V
